@@ -201,8 +201,7 @@ __device__ __forceinline__ float erf_gelu(float x) {
 __device__ __forceinline__ float gelu_f(float x) {
   return 0.5f * x * (1.0f + erf_gelu(x * 0.70710678118654752440f));
 }
-// the same on two values with the packed fp32 VALU (v_pk_fma_f32 / v_pk_mul_f32: two lanes' worth per
-// instruction; the reciprocal and exponential stay scalar): ~12 instead of ~20 VALU instructions per value
+// the same on a pair of values (the library is built without the packed fp32 instructions: each half is scalar code)
 typedef float dmf_f2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ dmf_f2 gelu_f2(dmf_f2 x) {
   const dmf_f2 z = x * 0.70710678118654752440f;
