@@ -1,0 +1,178 @@
+// Entry points of the masked attention (masked_attn.h): argument checks, the split of the keys, the spans of a
+// document mask. The kernels are instantiated per storage type in masked_attn_{fwd,bwd}_{bf16,f16,f32}.hip.
+#include "masked_attn.h"
+
+namespace dmf {
+
+int mattn_fwd_bf16(const AtArgs& a, int nw, hipStream_t stream);
+int mattn_fwd_f16(const AtArgs& a, int nw, hipStream_t stream);
+int mattn_fwd_f32(const AtArgs& a, int nw, hipStream_t stream);
+int mattn_bwd_bf16(const AtArgs& a, hipStream_t stream);
+int mattn_bwd_f16(const AtArgs& a, hipStream_t stream);
+int mattn_bwd_f32(const AtArgs& a, hipStream_t stream);
+
+// Spans of a document mask: a document is a maximal run of equal ids >= 0 in the first kv_len positions; query i stands
+// at position p = kv_len - lq + i and sees its document, under `causal` only up to itself or the document's first
+// `prefix` tokens. One workgroup per batch row: each thread owns a stretch of positions, the run that enters it from
+// the left and the end that follows it on the right come from a scan of the threads' last / first run starts.
+__global__ void __launch_bounds__(1024) k_mattn_spans(const int* __restrict__ docs, long long doc_sb,
+                                                      const int* kv_lens, const int* prefix, int lq, int lk, int causal,
+                                                      int2* __restrict__ spans) {
+  __shared__ int left[1024], right[1024];
+  const int b = blockIdx.x, t = threadIdx.x;
+  const int n = kv_lens ? min(max(kv_lens[b], 0), lk) : lk;
+  const int pre = prefix ? prefix[b] : 0, q0 = n - lq;  // position of query 0
+  const int* id = docs + b * doc_sb;
+  int2* out = spans + (long long)b * lq;
+  const int per = (n + 1023) / 1024, j0 = min(n, t * per), j1 = min(n, j0 + per);
+  int first = n, last = -1;  // run starts within [j0, j1)
+  for (int j = j0; j < j1; ++j)
+    if (j == 0 || id[j] != id[j - 1]) {
+      if (last < 0) first = j;
+      last = j;
+    }
+  left[t] = last;
+  right[t] = first;
+  __syncthreads();
+  for (int s = 1; s < 1024; s <<= 1) {
+    const int l = t >= s ? left[t - s] : -1, r = t + s < 1024 ? right[t + s] : n;
+    __syncthreads();
+    left[t] = max(left[t], l);
+    right[t] = min(right[t], r);
+    __syncthreads();
+  }
+  int start = t > 0 ? left[t - 1] : -1, end = t < 1023 ? right[t + 1] : n;
+  for (int j = j0; j < j1; ++j) {
+    if (j == 0 || id[j] != id[j - 1]) start = j;
+    if (j >= q0) out[j - q0].x = start;
+  }
+  for (int j = j1 - 1; j >= j0; --j) {
+    if (j >= q0) {
+      const int lo = out[j - q0].x;
+      const int hi = causal ? (int)min((long long)end, max((long long)j + 1, (long long)lo + max(pre, 0))) : end;
+      out[j - q0] = id[j] < 0 ? make_int2(0, 0) : make_int2(lo, hi);
+    }
+    if (j == 0 || id[j] != id[j - 1]) end = j;
+  }
+  for (int i = t; i < min(lq, -q0); i += 1024) out[i] = make_int2(0, 0);  // queries before the first position
+}
+
+struct AtPlan {
+  int nw, chunk, splits;
+};
+// Rows of 32 or fewer per key head take the one-wave workgroups; their keys are cut until about AT_FEW_BLOCKS workgroups
+// run. More rows take workgroups of 128 rows, cut only while they do not fill the card's 512 places (two per CU).
+constexpr long long AT_FEW_BLOCKS = 4096, AT_BLOCKS = 512;
+static AtPlan at_plan(int batch, int lq, int lk, int hk, int group) {
+  const long long rows = (long long)lq * group, nbh = (long long)batch * hk;
+  AtPlan p;
+  p.nw = rows <= 32 ? 1 : 4;
+  const long long blocks = ((rows + 32 * p.nw - 1) / (32 * p.nw)) * nbh;
+  const long long want = p.nw == 1 ? AT_FEW_BLOCKS : AT_BLOCKS, least = p.nw == 1 ? 64 : 256;
+  long long chunk = ((long long)lk * blocks + want - 1) / want;
+  chunk = (chunk + 63) / 64 * 64;
+  if (chunk < least) chunk = least;
+  if (chunk * 32768 < lk) chunk = ((long long)lk / 32768 + 64) / 64 * 64;
+  p.splits = (int)((lk + chunk - 1) / chunk);
+  if (p.splits < 1 || blocks * 2 > want) p.splits = 1;
+  p.chunk = p.splits > 1 ? (int)chunk : (lk > 0 ? lk : 1);
+  return p;
+}
+
+static int at_check(const char* who, const AtArgs& a, int dtype) {
+  DMF_CHECK_ARG(dtype == DMF_F32 || dtype == DMF_BF16 || dtype == DMF_F16, "%s: dtype %d", who, dtype);
+  DMF_CHECK_ARG(a.batch >= 0 && a.lq >= 0 && a.lk >= 0 && a.hk >= 1 && a.hq >= 1 && a.hq % a.hk == 0,
+                "%s: %d query heads must be a multiple of %d key heads", who, a.hq, a.hk);
+  DMF_CHECK_ARG(a.d >= 8 && a.d <= 128 && a.d % 8 == 0, "%s: head dim %d must be a multiple of 8 up to 128", who, a.d);
+  DMF_CHECK_ARG(a.scale > 0.f && a.scale < INFINITY, "%s: scale %g must be positive", who, a.scale);
+  DMF_CHECK_ARG(a.cap >= 0.f && a.cap < INFINITY, "%s: softcap %g must be 0 (none) or positive", who, a.cap);
+  DMF_CHECK_ARG(a.causal || !a.prefix, "%s: a prefix needs causal", who);
+  const long long rows = (long long)a.lq * a.group, nbh = (long long)a.batch * a.hk;
+  DMF_CHECK_ARG(rows * a.group < (1LL << 31) && ((rows + 31) / 32 + (a.lk + 127) / 128 + 1) * (nbh + 1) < (1LL << 31),
+                "%s: %d queries x %d heads x %d rows exceed the launch", who, a.lq, a.hq, a.batch);
+  const int e = dtype == DMF_F32 ? 4 : 2;
+  const long long st[] = {a.q_sb, a.q_sl, a.q_sh, a.k_sb, a.k_sl, a.k_sh, a.v_sb, a.v_sl, a.v_sh};
+  for (long long s : st) DMF_CHECK_ARG(s >= 0 && s * e % 16 == 0, "%s: stride %lld is not a multiple of 16 bytes", who, s);
+  DMF_CHECK_ARG((uintptr_t)a.q % 16 == 0 && (uintptr_t)a.k % 16 == 0 && (uintptr_t)a.v % 16 == 0,
+                "%s: q, k and v must be aligned to 16 bytes", who);
+  DMF_CHECK_ARG(130 * a.k_sl * e < (1LL << 31) && 130 * a.v_sl * e < (1LL << 31) &&
+                    (130 * a.q_sl + a.group * a.q_sh) * e < (1LL << 31) &&
+                    (130LL * a.hq * a.d + (long long)a.hq * a.d) * e < (1LL << 31),
+                "%s: a tile of rows spans more than 2 GiB", who);
+  return 0;
+}
+
+}  // namespace dmf
+
+using namespace dmf;
+
+extern "C" int dmf_mattn_spans(const int* documents, long long doc_sb, const int* kv_lens, const int* prefix, int batch,
+                               int lq, int lk, int causal, int* spans, void* stream) {
+  DMF_CHECK_ARG(batch >= 0 && lq >= 0 && lk >= 0, "dmf_mattn_spans: batch %d, lengths %d / %d", batch, lq, lk);
+  if (batch == 0 || lq == 0) return 0;
+  DMF_CHECK_ARG((documents || lk == 0) && spans && (uintptr_t)spans % 8 == 0, "dmf_mattn_spans: null operand");
+  hipLaunchKernelGGL(k_mattn_spans, dim3((unsigned)batch), dim3(1024), 0, (hipStream_t)stream, documents, doc_sb,
+                     kv_lens, prefix, lq, lk, causal, (int2*)spans);
+  DMF_LAUNCH_CHECK("dmf_mattn_spans");
+  return 0;
+}
+
+extern "C" long long dmf_mattn_fwd_ws_floats(int batch, int lq, int lk, int hq, int hk, int d) {
+  if (batch <= 0 || lq <= 0 || lk <= 0 || hk <= 0 || hq < hk) return 0;
+  const AtPlan p = at_plan(batch, lq, lk, hk, hq / hk);
+  return p.splits > 1 ? (long long)p.splits * batch * lq * hq * (d + 2) : 0;
+}
+
+extern "C" int dmf_mattn_fwd(int dtype, const void* q, long long q_sb, long long q_sl, long long q_sh, const void* k,
+                             long long k_sb, long long k_sl, long long k_sh, const void* v, long long v_sb,
+                             long long v_sl, long long v_sh, int batch, int lq, int lk, int hq, int hk, int d,
+                             float scale, float softcap, const float* slopes, int causal, const int* kv_lens,
+                             const int* prefix, const int* spans, void* o, void* o_lo, float* lse, float* ws,
+                             void* stream) {
+  AtArgs a = {};
+  a.q = q, a.k = k, a.v = v;
+  a.q_sb = q_sb, a.q_sl = q_sl, a.q_sh = q_sh, a.k_sb = k_sb, a.k_sl = k_sl, a.k_sh = k_sh;
+  a.v_sb = v_sb, a.v_sl = v_sl, a.v_sh = v_sh;
+  a.batch = batch, a.lq = lq, a.lk = lk, a.hq = hq, a.hk = hk, a.d = d, a.group = hk > 0 ? hq / hk : 0;
+  a.scale = scale, a.cap = softcap, a.slopes = slopes, a.causal = causal, a.kv_lens = kv_lens, a.prefix = prefix;
+  a.spans = (const int2*)spans, a.o = o, a.o_lo = o_lo, a.lse = lse;
+  if (int rc = at_check("dmf_mattn_fwd", a, dtype)) return rc;
+  if (batch == 0 || lq == 0) return 0;
+  DMF_CHECK_ARG(q && o && (lk == 0 || (k && v)), "dmf_mattn_fwd: null operand");
+  DMF_CHECK_ARG((uintptr_t)o % 16 == 0 && (uintptr_t)o_lo % 16 == 0 && (uintptr_t)spans % 8 == 0,
+                "dmf_mattn_fwd: outputs must be aligned to 16 bytes");
+  const AtPlan p = at_plan(batch, lq, lk, hk, a.group);
+  a.chunk = p.chunk, a.splits = p.splits;
+  if (p.splits > 1) {
+    DMF_CHECK_ARG(ws && (uintptr_t)ws % 16 == 0, "dmf_mattn_fwd: this size needs a workspace (dmf_mattn_fwd_ws_floats)");
+    a.po = ws;
+    a.pml = ws + (long long)p.splits * batch * lq * hq * d;
+  }
+  hipStream_t s = (hipStream_t)stream;
+  return dtype == DMF_BF16 ? mattn_fwd_bf16(a, p.nw, s) : dtype == DMF_F16 ? mattn_fwd_f16(a, p.nw, s)
+                                                                          : mattn_fwd_f32(a, p.nw, s);
+}
+
+extern "C" int dmf_mattn_bwd(int dtype, const void* q, long long q_sb, long long q_sl, long long q_sh, const void* k,
+                             long long k_sb, long long k_sl, long long k_sh, const void* v, long long v_sb,
+                             long long v_sl, long long v_sh, int batch, int lq, int lk, int hq, int hk, int d,
+                             float scale, float softcap, const float* slopes, int causal, const int* kv_lens,
+                             const int* prefix, const int* spans, const void* o, const void* o_lo, const float* lse,
+                             const void* go, float* delta, void* dq, void* dk, void* dv, void* stream) {
+  AtArgs a = {};
+  a.q = q, a.k = k, a.v = v;
+  a.q_sb = q_sb, a.q_sl = q_sl, a.q_sh = q_sh, a.k_sb = k_sb, a.k_sl = k_sl, a.k_sh = k_sh;
+  a.v_sb = v_sb, a.v_sl = v_sl, a.v_sh = v_sh;
+  a.batch = batch, a.lq = lq, a.lk = lk, a.hq = hq, a.hk = hk, a.d = d, a.group = hk > 0 ? hq / hk : 0;
+  a.scale = scale, a.cap = softcap, a.slopes = slopes, a.causal = causal, a.kv_lens = kv_lens, a.prefix = prefix;
+  a.spans = (const int2*)spans, a.o = (void*)o, a.o_lo = (void*)o_lo, a.lse = (float*)lse, a.go = go, a.delta = delta;
+  a.dq = dq, a.dk = dk, a.dv = dv;
+  if (int rc = at_check("dmf_mattn_bwd", a, dtype)) return rc;
+  if (batch == 0 || (lq == 0 && lk == 0)) return 0;
+  DMF_CHECK_ARG((lq == 0 || (q && o && lse && go && delta && dq)) && (lk == 0 || (k && v && dk && dv)),
+                "dmf_mattn_bwd: null operand");
+  const uintptr_t al = (uintptr_t)o | (uintptr_t)o_lo | (uintptr_t)go | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv;
+  DMF_CHECK_ARG(al % 16 == 0 && (uintptr_t)spans % 8 == 0, "dmf_mattn_bwd: operands must be aligned to 16 bytes");
+  hipStream_t s = (hipStream_t)stream;
+  return dtype == DMF_BF16 ? mattn_bwd_bf16(a, s) : dtype == DMF_F16 ? mattn_bwd_f16(a, s) : mattn_bwd_f32(a, s);
+}

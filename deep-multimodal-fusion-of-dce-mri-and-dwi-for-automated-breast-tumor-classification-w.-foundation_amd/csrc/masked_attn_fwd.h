@@ -1,0 +1,325 @@
+// Masked attention forward (see masked_attn.h for the mathematics and the layouts).
+//
+// A workgroup of NW waves takes 32 NW packed rows of one (batch row, key head); the keys of the union of their spans
+// stream through two LDS stages of KT keys (LDS-DMA, the next tile in flight under the current one's products). A wave
+// holds its 32 queries and their output accumulators in registers and keeps a running maximum and sum per row. The
+// maximum may lag by 2^8 before the accumulators are rescaled (p <= 256 is exact enough in f32 and in range in f16), which
+// takes the rescale out of almost every tile. NW = 4, KT = 64 for rows that fill it; NW = 1, KT = 32 for up to 32 rows
+// (single tokens: one wave per workgroup, five in a CU's LDS, so that enough loads are in flight to draw on HBM).
+//
+// Splits: with few workgroups along the rows the keys are cut into chunks of a.chunk, each workgroup writes its
+// unnormalised accumulators with (max, sum), and k_mattn_join adds them. Chunks are cut at absolute keys, so a short row of a
+// long cache leaves workgroups that exit at once instead of long ones that hold the others up.
+//
+// A masked key has p = 0 exactly, but 0 * NaN is NaN: a NaN or infinity in a value that some row of the tile may not see
+// would reach that row. Keys outside the union of the workgroup's spans are zero-filled on load; for the rest, a wave whose
+// accumulators end up non-finite recomputes the rows in question key by key over their own spans (at_row_alone), which
+// costs nothing where the values are finite.
+#pragma once
+#include "masked_attn.h"
+
+namespace dmf {
+
+// one row over its own span only: each lane holds dims lane and lane + 64
+template <typename T, bool CAP, bool SLOPE>
+__device__ void at_row_alone(const AtArgs& a, const T* q, const T* k, const T* v, int lo, int hi, int at, int head,
+                             int lane, float& m, float& l, float& o0, float& o1) {
+  const AtScore sc = at_score_of<T>(a, head);
+  const float q0 = lane < a.d ? ld(q + lane) : 0.f, q1 = lane + 64 < a.d ? ld(q + lane + 64) : 0.f;
+  m = -INFINITY;
+  l = o0 = o1 = 0.f;
+  for (int j = lo; j < hi; ++j) {
+    const T* kj = k + j * a.k_sl;
+    const T* vj = v + j * a.v_sl;
+    float dot = 0.f;
+    if (lane < a.d) dot = q0 * ld(kj + lane);
+    if (lane + 64 < a.d) dot = fmaf(q1, ld(kj + lane + 64), dot);
+    dot = wave_sum(dot);
+    const float s = at_score<T, CAP, SLOPE>(sc, dot, fabsf((float)(at - j)));
+    const float mn = fmaxf(m, s), ms = mn == -INFINITY ? 0.f : mn;
+    const float alpha = at_exp<T>(m - ms), p = at_exp<T>(s - ms);
+    m = mn;
+    l = fmaf(l, alpha, p);
+    o0 = o0 * alpha;
+    o1 = o1 * alpha;
+    if (lane < a.d) o0 = fmaf(p, ld(vj + lane), o0);
+    if (lane + 64 < a.d) o1 = fmaf(p, ld(vj + lane + 64), o1);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void at_store4(T* p, const float* v) {  // p aligned to 4 elements
+  if constexpr (sizeof(T) == 4)
+    *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
+  else
+    *(uint2*)p = make_uint2(B16<T>::pack(v[0], v[1]), B16<T>::pack(v[2], v[3]));
+}
+
+template <typename T, int DF, bool CAP, bool SLOPE, int NW, int KT>
+__global__ void __launch_bounds__(64 * NW, NW == 4 ? (sizeof(T) == 4 ? 1 : 2) : 1) k_mattn_fwd(AtArgs a) {
+  constexpr int DP = AtPad<DF>::DP, KS = AtSteps<T, DF>::N, FD = DF / 32, KF = KT / 32;
+  constexpr int TILE = KT * DP * AtT<T>::E, STAGE = 2 * TILE;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ int range[2 * NW];
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int nbh = a.batch * a.hk, rows = a.lq * a.group;
+  // key heads vary fastest (their tiles of one row block go to different XCDs, each XCD keeps its heads' K / V in
+  // its L2); the last row blocks, the longest under a causal mask, start first
+  const int bh = blockIdx.x % nbh, tile = gridDim.x / nbh - 1 - blockIdx.x / nbh, split = blockIdx.y;
+  const int b = bh / a.hk, kh = bh - b * a.hk;
+  const int row = tile * 32 * NW + wid * 32 + (lane & 31);
+  const int qi = row < rows ? row / a.group : 0, head = kh * a.group + (row < rows ? row - qi * a.group : 0);
+  AtSpan sp = row < rows ? at_span(a, b, qi) : AtSpan{0, 0, 0};
+  const bool live = sp.hi > sp.lo;
+  // the wave's spans: union (w_lo, w_hi) and intersection (i_lo, i_hi) over the rows that see anything
+  const int w_lo = at_wave_min(live ? sp.lo : 0x7fffffff), w_hi = at_wave_max(live ? sp.hi : 0);
+  const int i_lo = at_wave_max(live ? sp.lo : 0), i_hi = at_wave_min(live ? sp.hi : 0x7fffffff);
+  int k_lo = w_lo, k_hi = w_hi;
+  if constexpr (NW > 1) {
+    if (lane == 0) range[wid] = w_lo, range[NW + wid] = w_hi;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) k_lo = min(k_lo, range[w]), k_hi = max(k_hi, range[NW + w]);
+    k_lo = __builtin_amdgcn_readfirstlane(k_lo);
+    k_hi = __builtin_amdgcn_readfirstlane(k_hi);
+  }
+  if (a.splits > 1) {
+    k_lo = max(k_lo, split * a.chunk);
+    k_hi = (int)min((long long)k_hi, (long long)(split + 1) * a.chunk);
+    if (k_lo >= k_hi) return;
+  }
+  const T* kb = (const T*)a.k + b * a.k_sb + kh * a.k_sh;
+  const T* vb = (const T*)a.v + b * a.v_sb + kh * a.v_sh;
+  const T* qb = (const T*)a.q + b * a.q_sb + (long long)qi * a.q_sl + head * a.q_sh;
+  const AtScore sc = at_score_of<T>(a, head);
+  const unsigned lds0 = (unsigned)(uintptr_t)((__attribute__((address_space(3))) char*)smem);
+
+  uint4 qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    const int e = (2 * ks + h) * AtT<T>::CH;
+    qf[ks] = live && e < a.d ? *(const uint4*)(qb + e) : make_uint4(0, 0, 0, 0);
+  }
+  auto issue = [&](int stage, int k0) {
+    at_load_rows<T, DP, KT, NW>(kb, a.k_sl, k0, k_lo, k_hi, a.d, lds0 + stage * STAGE, wid, lane);
+    at_load_rows<T, DP, KT, NW>(vb, a.v_sl, k0, k_lo, k_hi, a.d, lds0 + stage * STAGE + TILE, wid, lane);
+  };
+
+  at_f32x16 acc[FD];
+#pragma unroll
+  for (int f = 0; f < FD; ++f) acc[f] = at_zero();
+  float m = -INFINITY, ms = 0.f, l = 0.f;  // ms: m, or 0 while there is none
+  const int nt = k_hi > k_lo ? (k_hi - k_lo + KT - 1) / KT : 0;
+  if (nt > 0) issue(0, k_lo);
+  for (int t = 0; t < nt; ++t) {
+    const int k0 = k_lo + t * KT;
+    // this tile has landed (in every wave: the barrier); the other stage's last readers are past it too
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (t + 1 < nt) issue((t + 1) & 1, k0 + KT);
+    if (k0 >= w_hi || k0 + KT <= w_lo) continue;  // (wave-uniform) nothing here for these rows
+    const char* K = smem + (t & 1) * STAGE;
+    const char* V = K + TILE;
+    at_f32x16 s[KF];
+#pragma unroll
+    for (int f = 0; f < KF; ++f) {
+      s[f] = at_zero();
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s[f] = at_mfma<T>(at_row<T, DP>(K, 32 * f + (lane & 31), ks, h), qf[ks], s[f]);
+    }
+    const float x0 = (float)(sp.at - k0 - 4 * h);  // position minus this lane's first key
+    if constexpr (CAP || SLOPE || sizeof(T) == 4) {
+#pragma unroll
+      for (int f = 0; f < KF; ++f)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          s[f][i] = at_score<T, CAP, SLOPE>(sc, s[f][i], fabsf(x0 - (float)(32 * f + 8 * (i >> 2) + (i & 3))));
+    }
+    if (k0 < i_lo || k0 + KT > i_hi) {  // (wave-uniform) some row does not see the whole tile
+#pragma unroll
+      for (int f = 0; f < KF; ++f)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int j = k0 + 32 * f + 8 * (i >> 2) + 4 * h + (i & 3);
+          if (j < sp.lo || j >= sp.hi) s[f][i] = -INFINITY;
+        }
+    }
+    // scores in units U after at_score; plain 16-bit scores stay raw and are scaled in the exponent's FMA (scale > 0)
+    constexpr bool RAW = !(CAP || SLOPE || sizeof(T) == 4);
+    float mt = -INFINITY;
+#pragma unroll
+    for (int f = 0; f < KF; ++f)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[f][i]);
+    mt = at_half_max(mt);
+    if (RAW) mt *= sc.scale_u;
+    if (__any(mt > m + 8.f * AtUnit<T>::U / AT_LOG2E)) {
+      const float mn = fmaxf(m, mt);
+      ms = mn == -INFINITY ? 0.f : mn;
+      const float alpha = at_exp<T>(m - ms);
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int f = 0; f < FD; ++f) acc[f] *= alpha;
+    }
+#pragma unroll
+    for (int f = 0; f < KF; ++f) {
+      float p[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        p[i] = RAW ? at_exp<T>(fmaf(s[f][i], sc.scale_u, -ms)) : at_exp<T>(s[f][i] - ms);
+        l += p[i];
+      }
+      // p is rounded to the 16-bit operand type (half a step, random in sign over the keys); l sums the unrounded ones
+      at_accumulate<T, DF>(V, 32 * f, p, acc, lane);
+    }
+  }
+  l = at_half_sum(l);
+  float bad = l * 0.f;
+#pragma unroll
+  for (int f = 0; f < FD; ++f)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) bad = fmaf(acc[f][i], 0.f, bad);
+  const unsigned long long redo = __ballot(live && bad != bad);
+  const unsigned alone = (unsigned)redo | (unsigned)(redo >> 32);
+
+  const long long prow = ((long long)split * nbh + bh) * rows + row;  // partials
+  T* ob = (T*)a.o + (((long long)b * a.lq + qi) * a.hq + head) * a.d;
+  T* olo = a.o_lo ? (T*)a.o_lo + (((long long)b * a.lq + qi) * a.hq + head) * a.d : nullptr;
+  if (row < rows && !((alone >> (lane & 31)) & 1)) {
+    if (a.splits > 1) {
+      float* po = a.po + prow * a.d;
+#pragma unroll
+      for (int f = 0; f < FD; ++f)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int e = 32 * f + 8 * g + 4 * h;
+          if (e < a.d) *(float4*)(po + e) = make_float4(acc[f][4 * g], acc[f][4 * g + 1], acc[f][4 * g + 2], acc[f][4 * g + 3]);
+        }
+      if (h == 0) *(float2*)(a.pml + 2 * prow) = make_float2(m, l);
+    } else {
+      const float inv = live ? 1.f / l : 0.f;
+#pragma unroll
+      for (int f = 0; f < FD; ++f)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int e = 32 * f + 8 * g + 4 * h;
+          if (e >= a.d) continue;
+          float v[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = live ? acc[f][4 * g + r] * inv : 0.f;
+          at_store4(ob + e, v);
+          if (olo) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] -= Cvt<T>::load(Cvt<T>::store(v[r]));
+            at_store4(olo + e, v);
+          }
+        }
+      if (a.lse && h == 0) a.lse[(long long)bh * rows + row] = live ? ms + at_log<T>(l) : INFINITY;
+    }
+  }
+  for (unsigned todo = alone; todo; todo &= todo - 1) {
+    const int n = __builtin_ctz(todo);
+    const int r_lo = max(__shfl(sp.lo, n, 64), k_lo), r_hi = min(__shfl(sp.hi, n, 64), k_hi);
+    const int r_at = __shfl(sp.at, n, 64), r_qi = __shfl(qi, n, 64), r_head = __shfl(head, n, 64);
+    float rm, rl, o0, o1;
+    at_row_alone<T, CAP, SLOPE>(a, (const T*)a.q + b * a.q_sb + (long long)r_qi * a.q_sl + r_head * a.q_sh, kb, vb, r_lo,
+                                r_hi, r_at, r_head, lane, rm, rl, o0, o1);
+    const long long pr = prow - row + __shfl(row, n, 64), orow = (((long long)b * a.lq + r_qi) * a.hq + r_head) * a.d;
+    if (a.splits == 1) {
+      o0 /= rl;
+      o1 /= rl;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int e = lane + 64 * k;
+      const float o = k ? o1 : o0;
+      if (e >= a.d) continue;
+      if (a.splits > 1) {
+        a.po[pr * a.d + e] = o;
+      } else {
+        st((T*)a.o + orow + e, o);
+        if (a.o_lo) st((T*)a.o_lo + orow + e, o - Cvt<T>::load(Cvt<T>::store(o)));
+      }
+    }
+    if (lane == 0) {
+      if (a.splits > 1)
+        *(float2*)(a.pml + 2 * pr) = make_float2(rm, rl);
+      else if (a.lse)
+        a.lse[pr] = (rm == -INFINITY ? 0.f : rm) + at_log<T>(rl);
+    }
+  }
+}
+
+// o of one packed row from its splits: sum exp(m_s - m) O_s / sum exp(m_s - m) l_s over the splits its span touches.
+// One wave per row; lanes hold dims lane and lane + 64.
+template <typename T>
+__global__ void __launch_bounds__(64) k_mattn_join(AtArgs a) {
+  const int lane = threadIdx.x, nbh = a.batch * a.hk, rows = a.lq * a.group;
+  const int bh = blockIdx.x % nbh, row = blockIdx.x / nbh;
+  const int b = bh / a.hk, kh = bh - b * a.hk, qi = row / a.group, head = kh * a.group + row - qi * a.group;
+  const AtSpan sp = at_span(a, b, qi);
+  const bool live = sp.hi > sp.lo;
+  const int s0 = sp.lo / a.chunk, s1 = live ? (sp.hi - 1) / a.chunk + 1 : s0;
+  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int s = s0 + lane; s < s1; s += 64) m = fmaxf(m, a.pml[2 * (((long long)s * nbh + bh) * rows + row)]);
+  m = wave_max(m);
+  const float ms = m == -INFINITY ? 0.f : m;
+  for (int s = s0; s < s1; ++s) {
+    const long long pr = ((long long)s * nbh + bh) * rows + row;
+    const float2 ml = *(const float2*)(a.pml + 2 * pr);
+    const float w = at_exp<T>(ml.x - ms);
+    // (a split whose keys are all -inf for this row has w = 0 and finite sums)
+    l = fmaf(w, ml.y, l);
+    if (lane < a.d) o0 = fmaf(w, a.po[pr * a.d + lane], o0);
+    if (lane + 64 < a.d) o1 = fmaf(w, a.po[pr * a.d + lane + 64], o1);
+  }
+  const long long orow = (((long long)b * a.lq + qi) * a.hq + head) * a.d;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int e = lane + 64 * k;
+    const float o = live ? (k ? o1 : o0) / l : 0.f;
+    if (e >= a.d) continue;
+    st((T*)a.o + orow + e, o);
+    if (a.o_lo) st((T*)a.o_lo + orow + e, o - Cvt<T>::load(Cvt<T>::store(o)));
+  }
+  if (a.lse && lane == 0) a.lse[(long long)bh * rows + row] = live ? ms + at_log<T>(l) : INFINITY;
+}
+
+template <typename T, int DF, bool CAP, bool SLOPE>
+static int mattn_fwd_df(const AtArgs& a, int nw, hipStream_t stream) {
+  constexpr int RB = AtPad<DF>::DP * AtT<T>::E;
+  const int rows = a.lq * a.group, nbh = a.batch * a.hk;
+  const dim3 grid((unsigned)((long long)cdiv(rows, 32 * nw) * nbh), (unsigned)a.splits);
+  if (nw == 4) {
+    constexpr int KT = sizeof(T) == 4 ? 32 : 64;  // f32 rows are twice as wide: the same LDS for half the keys
+    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, 4, KT>), grid, dim3(256), 4 * KT * RB, stream, a);
+  } else {
+    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, 1, 32>), grid, dim3(64), 4 * 32 * RB, stream, a);
+  }
+  DMF_LAUNCH_CHECK("dmf_mattn_fwd");
+  return 0;
+}
+
+template <typename T>
+static int mattn_fwd_t(const AtArgs& a, int nw, hipStream_t stream) {
+  int rc = 0;
+#define DMF_AT_MODE(DF)                                                                  \
+  rc = a.cap > 0.f ? (a.slopes ? mattn_fwd_df<T, DF, true, true>(a, nw, stream)          \
+                               : mattn_fwd_df<T, DF, true, false>(a, nw, stream))        \
+                   : (a.slopes ? mattn_fwd_df<T, DF, false, true>(a, nw, stream)         \
+                               : mattn_fwd_df<T, DF, false, false>(a, nw, stream))
+  if (a.d <= 32) DMF_AT_MODE(32);
+  else if (a.d <= 64) DMF_AT_MODE(64);
+  else if (a.d <= 96) DMF_AT_MODE(96);
+  else DMF_AT_MODE(128);
+#undef DMF_AT_MODE
+  if (rc) return rc;
+  if (a.splits > 1) {
+    hipLaunchKernelGGL((k_mattn_join<T>), dim3((unsigned)((long long)a.lq * a.group * a.batch * a.hk)), dim3(64), 0,
+                       stream, a);
+    DMF_LAUNCH_CHECK("dmf_mattn_fwd (join)");
+  }
+  return 0;
+}
+
+}  // namespace dmf

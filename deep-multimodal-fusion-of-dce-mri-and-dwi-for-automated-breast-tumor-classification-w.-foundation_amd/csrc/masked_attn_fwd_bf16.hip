@@ -1,0 +1,6 @@
+// Masked attention forward for bf16 storage.
+#include "masked_attn_fwd.h"
+
+namespace dmf {
+int mattn_fwd_bf16(const AtArgs& a, int nw, hipStream_t stream) { return mattn_fwd_t<bf16_t>(a, nw, stream); }
+}  // namespace dmf

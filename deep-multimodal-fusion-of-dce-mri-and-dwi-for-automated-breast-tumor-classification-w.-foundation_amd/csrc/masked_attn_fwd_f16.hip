@@ -1,0 +1,6 @@
+// Masked attention forward for f16 storage.
+#include "masked_attn_fwd.h"
+
+namespace dmf {
+int mattn_fwd_f16(const AtArgs& a, int nw, hipStream_t stream) { return mattn_fwd_t<f16_t>(a, nw, stream); }
+}  // namespace dmf

@@ -1,0 +1,306 @@
+"""Token attention between a block's qkv projection and its output projection: the per-head norm of
+queries and keys with the position rotation (``qk_norm_rope``), and attention with capped scores, a
+distance bias and causal / prefix / document masks over shared key heads (``attention``), for training
+and for single tokens against a long cache.
+
+The reference's MultiHeadSelfAttention (transformer_model.py:83-116) is the case without any of these
+(dmf_tokens); its blocks take them as options (transformer_model.TransformerStage). Both ops run on
+csrc/qknorm.hip and csrc/masked_attn*.h through the C-ABI, on torch's current stream, with every
+workspace from torch's allocator, so they can be captured into a graph; sizes are checked on the host, and
+device-side values (positions, lengths, ids) are bounds-checked in the kernels.
+"""
+from __future__ import annotations
+
+import contextlib
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+import dmf_native as N
+
+_DTYPES = {torch.float32: N.F32, torch.bfloat16: N.BF16, torch.float16: N.F16}
+
+
+def _on(t):
+    """Launches go to the tensors' device, also where another one is current."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _heads(what, name, t, like=None):
+    if not isinstance(t, torch.Tensor) or t.dim() != 4:
+        raise ValueError(f"{what}: {name} must be [batch, length, heads, head_dim], got "
+                         f"{tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__}")
+    if not t.is_cuda:
+        N.require_cuda(t)
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"{what}: {name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{what}: {name} is {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+
+
+def _strided(t, align):
+    """(tensor, batch / token / head strides) with contiguous head dims; strides and base multiples of
+    ``align`` elements, else of a contiguous copy."""
+    for _ in range(2):
+        # the stride of a dim of length 1 says nothing
+        st = [0 if t.shape[i] == 1 else t.stride(i) for i in range(3)]
+        if ((t.shape[3] == 1 or t.stride(3) == 1) and all(s % align == 0 for s in st)
+                and t.data_ptr() % (align * t.element_size()) == 0):
+            return t, st
+        t = t.contiguous()
+        if t.data_ptr() % (align * t.element_size()):
+            t = t.clone(memory_format=torch.contiguous_format)
+    return t, st
+
+
+def _plain(t, align=1):
+    """Contiguous (and, for 16-byte loads, aligned) form of a gradient."""
+    t = t.contiguous()
+    return t if align == 1 or t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _small(what, name, t, shape, dtype, device):
+    if t is None:
+        return None
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{what}: {name} is on {t.device}, expected {device}")
+    if t.is_floating_point() != dtype.is_floating_point or t.dtype == torch.bool:
+        raise ValueError(f"{what}: {name} must be {dtype}, got {t.dtype}")
+    return t.to(dtype).contiguous()
+
+
+# -------------------------------------------------------- norm and rotation
+def rope_table(length, dims, theta=10000.0, device=None):
+    """(cos, sin), each f32 [length, dims / 2]: pair p of position t turns by t * theta^(-2 p / dims)
+    (angles in 64 bits: far positions keep their phase)."""
+    if dims < 2 or dims % 2 or length < 1:
+        raise ValueError(f"rope_table: dims {dims} must be even and positive, length {length} positive")
+    f = theta ** (-torch.arange(dims // 2, dtype=torch.float64, device=device) * 2 / dims)
+    a = torch.arange(length, dtype=torch.float64, device=device)[:, None] * f
+    return a.cos().float(), a.sin().float()
+
+
+def rope_table_2d(height, width, dims, theta=100.0, device=None):
+    """(cos, sin), each f32 [height * width, dims / 2], of a token grid in row-major order: the first half of
+    the pairs turns with the row, the rest with the column."""
+    if dims < 4 or dims % 4 or height < 1 or width < 1:
+        raise ValueError(f"rope_table_2d: dims {dims} must be a positive multiple of 4, the grid {height} x {width} not empty")
+    c, s = rope_table(max(height, width), dims // 2, theta, device)
+    y = torch.arange(height, device=device).repeat_interleave(width)
+    x = torch.arange(width, device=device).repeat(height)
+    return torch.cat([c[y], c[x]], 1).contiguous(), torch.cat([s[y], s[x]], 1).contiguous()
+
+
+def _qk_call(name, q, k, cos, sin, pos, wq, wk, norm, eps, interleaved, *rest):
+    b, n, hq, d = q.shape
+    q, qs = _strided(q, 1)
+    k, ks = _strided(k, 1)
+    rot = 0 if cos is None else 2 * cos.shape[1]
+    pos_sb = 0 if pos is None or pos.dim() == 1 else pos.stride(0)
+    with _on(q):
+        N.call(name, _DTYPES[q.dtype], q.data_ptr(), *qs, hq, k.data_ptr(), *ks, k.shape[2], b, n, d, rot,
+               int(interleaved), int(norm), eps, _p(wq), _p(wk), _p(cos), _p(sin), _p(pos), pos_sb,
+               int(pos is not None and pos.dtype == torch.int64), 0 if cos is None else cos.shape[0], *rest,
+               N.stream_ptr(q.device))
+
+
+def _qk_fwd(q, k, cos, sin, pos, wq, wk, norm, eps, interleaved):
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    _qk_call("dmf_qk_norm_rope", q, k, cos, sin, pos, wq, wk, norm, eps, interleaved, qo.data_ptr(), ko.data_ptr())
+    return qo, ko
+
+
+class _QkNormRopeFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, cos, sin, pos, norm, eps, interleaved):
+        ctx.save_for_backward(q, k, wq, wk, cos, sin, pos)
+        ctx.cfg = (norm, eps, interleaved)
+        return _qk_fwd(q, k, cos, sin, pos, wq, wk, *ctx.cfg)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gq, gk):
+        q, k, wq, wk, cos, sin, pos = ctx.saved_tensors
+        gq, gk = _plain(gq, 16), _plain(gk, 16)
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        dwq = dwk = ws = None
+        if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
+            d = q.shape[3]
+            dwq, dwk = (torch.empty(d, dtype=torch.float32, device=q.device) for _ in range(2))
+            ws = torch.empty(N.load().dmf_qk_norm_rope_bwd_ws_floats(q.shape[2], k.shape[2], d), dtype=torch.float32,
+                             device=q.device)
+        _qk_call("dmf_qk_norm_rope_bwd", q, k, cos, sin, pos, wq, wk, *ctx.cfg, gq.data_ptr(), gk.data_ptr(),
+                 dq.data_ptr(), dk.data_ptr(), _p(dwq), _p(dwk), _p(ws))
+        need = ctx.needs_input_grad
+        return (dq if need[0] else None, dk if need[1] else None, dwq if need[2] else None,
+                dwk if need[3] else None, None, None, None, None, None, None)
+
+
+def qk_norm_rope(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False):
+    """Norm and rotation of queries [b, n, hq, d] and keys [b, n, hk, d] (any strides, e.g. views of packed qkv
+    rows) in one pass: ``rot(x * rsqrt(mean(x^2) + eps) * weight)`` per head, in 32 bits, rounded once. Returns
+    contiguous (q, k); differentiable in q, k and the weights.
+
+    ``q_weight`` / ``k_weight`` f32 [d]: both given, or both None for the rotation alone (no norm).
+    ``cos`` / ``sin`` f32 [rows, rot / 2] (rope_table, rope_table_2d): the first ``rot`` dims turn, as pairs
+    (p, p + rot / 2) or, ``interleaved``, (2p, 2p + 1); None for the norm alone. ``positions`` int [b, n] or
+    [n]: each token's table row (default: its index); one outside the table makes its row NaN.
+    """
+    what = "qk_norm_rope"
+    _heads(what, "q", q)
+    _heads(what, "k", k, q)
+    b, n, hq, d = q.shape
+    if k.shape[:2] != q.shape[:2] or k.shape[3] != d or hq < 1 or k.shape[2] < 1:
+        raise ValueError(f"{what}: q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch, length or head dim")
+    if d % 2 or not 2 <= d <= 512:
+        raise ValueError(f"{what}: head dim {d} must be even and at most 512")
+    if (q_weight is None) != (k_weight is None) or (cos is None) != (sin is None):
+        raise ValueError(f"{what}: q_weight and k_weight, cos and sin are given together")
+    if q_weight is None and cos is None:
+        raise ValueError(f"{what}: neither norm weights nor a rotation table")
+    norm = q_weight is not None
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if norm and (tuple(w.shape) != (d,) or w.dtype != torch.float32 or w.device != q.device or not w.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be contiguous float32 [{d}] on {q.device}")
+    if cos is not None:
+        if (cos.dim() != 2 or cos.shape != sin.shape or not 1 <= cos.shape[1] <= d // 2 or cos.shape[0] < 1
+                or cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.device != q.device
+                or sin.device != q.device):
+            raise ValueError(f"{what}: cos and sin must be float32 [rows, up to {d // 2}] on {q.device}")
+        if cos.requires_grad or sin.requires_grad:
+            raise ValueError(f"{what}: no gradient reaches cos and sin")
+        cos, sin = cos.contiguous(), sin.contiguous()
+    if positions is not None:
+        if cos is None:
+            raise ValueError(f"{what}: positions without a rotation table")
+        if (tuple(positions.shape) not in ((b, n), (n,)) or positions.dtype not in (torch.int32, torch.int64)
+                or positions.device != q.device):
+            raise ValueError(f"{what}: positions must be int32 or int64 [{b}, {n}] or [{n}] on {q.device}")
+        if n > 1 and positions.stride(-1) != 1:
+            positions = positions.contiguous()
+    elif cos is not None and cos.shape[0] < n:
+        raise ValueError(f"{what}: the table has {cos.shape[0]} rows for {n} tokens")
+    if not (math.isfinite(eps) and eps >= 0):
+        raise ValueError(f"{what}: eps {eps}")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
+                                    or (norm and (q_weight.requires_grad or k_weight.requires_grad))):
+        return _QkNormRopeFn.apply(q, k, q_weight, k_weight, cos, sin, positions, norm, float(eps), bool(interleaved))
+    return _qk_fwd(q, k, cos, sin, positions, q_weight, k_weight, norm, float(eps), bool(interleaved))
+
+
+# ---------------------------------------------------------------- attention
+def _spans(documents, kv_lens, prefix, b, lq, lk, causal):
+    spans = torch.empty((b, lq, 2), dtype=torch.int32, device=documents.device)
+    with _on(documents):
+        N.call("dmf_mattn_spans", documents.data_ptr(), lk, _p(kv_lens), _p(prefix), b, lq, lk, int(causal),
+               spans.data_ptr(), N.stream_ptr(documents.device))
+    return spans
+
+
+def _attn_dims(q, k, v, cfg, kv_lens, prefix, slopes, spans):
+    """The leading arguments dmf_mattn_fwd and dmf_mattn_bwd share, and the tensors they point into."""
+    scale, softcap, causal = cfg
+    align = 16 // q.element_size()
+    (q, qs), (k, ks), (v, vs) = _strided(q, align), _strided(k, align), _strided(v, align)
+    args = (_DTYPES[q.dtype], q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs, q.shape[0], q.shape[1],
+            k.shape[1], q.shape[2], k.shape[2], q.shape[3], scale, softcap, _p(slopes), int(causal), _p(kv_lens),
+            None if spans is not None else _p(prefix), _p(spans))
+    return args, (q, k, v)
+
+
+def _attn_fwd(q, k, v, cfg, kv_lens, prefix, slopes, spans, train):
+    b, lq, hq, d = q.shape
+    args, keep = _attn_dims(q, k, v, cfg, kv_lens, prefix, slopes, spans)
+    o = torch.empty((b, lq, hq, d), dtype=q.dtype, device=q.device)
+    o_lo = torch.empty_like(o) if train and q.dtype != torch.float32 else None
+    lse = torch.empty(b * lq * hq, dtype=torch.float32, device=q.device) if train else None
+    n = N.load().dmf_mattn_fwd_ws_floats(b, lq, k.shape[1], hq, k.shape[2], d)
+    ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+    with _on(q):
+        N.call("dmf_mattn_fwd", *args, o.data_ptr(), _p(o_lo), _p(lse), _p(ws), N.stream_ptr(q.device))
+    del keep
+    return o, o_lo, lse
+
+
+class _AttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cfg, kv_lens, prefix, slopes, spans):
+        o, o_lo, lse = _attn_fwd(q, k, v, cfg, kv_lens, prefix, slopes, spans, True)
+        ctx.save_for_backward(q, k, v, kv_lens, prefix, slopes, spans, o, o_lo, lse)
+        ctx.cfg = cfg
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, go):
+        q, k, v, kv_lens, prefix, slopes, spans, o, o_lo, lse = ctx.saved_tensors
+        args, keep = _attn_dims(q, k, v, ctx.cfg, kv_lens, prefix, slopes, spans)
+        go = _plain(go, 16)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        delta = torch.empty_like(lse)
+        with _on(q):
+            N.call("dmf_mattn_bwd", *args, o.data_ptr(), _p(o_lo), lse.data_ptr(), go.data_ptr(), delta.data_ptr(),
+                   dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), N.stream_ptr(q.device))
+        del keep
+        need = ctx.needs_input_grad
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None, None)
+
+
+def attention(q, k, v, *, scale=None, softcap=0.0, slopes=None, causal=False, kv_lens=None, prefix=None,
+              documents=None):
+    """softmax(score) v per head, [b, lq, hq, d], of queries [b, lq, hq, d] over keys and values [b, lk, hk, d]
+    (any strides; hq a multiple of hk: query head h reads key head h // (hq // hk)). Differentiable in q, k, v.
+
+    score = softcap * tanh(z / softcap) - slopes[h] * |p - j|, z = scale * q.k (scale: d^-0.5; softcap 0 and
+    slopes None leave their term out; slopes f32 [hq] is not differentiated). Query i stands at position
+    p = kv_len - lq + i: the queries are the last lq of the kv_len tokens, so one new token against a cache of
+    capacity lk has lq = 1. It sees the keys j < kv_len (``kv_lens`` int [b], clamped to [0, lk]; default lk),
+    under ``causal`` those with j <= p and, all queries, the first ``prefix`` (int [b]) keys, and with
+    ``documents`` (int [b, lk] ids) those of its own document: the run of equal ids >= 0 it stands in (a
+    negative id belongs to none; the prefix then counts from the document's start). For a padded batch give
+    the padding a negative id. A query that sees nothing yields zeros and no gradient, and what a key or a value holds
+    does not reach the queries that do not see it.
+    """
+    what = "attention"
+    _heads(what, "q", q)
+    _heads(what, "k", k, q)
+    _heads(what, "v", v, q)
+    b, lq, hq, d = q.shape
+    lk, hk = k.shape[1], k.shape[2]
+    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+    if hk < 1 or hq < 1 or hq % hk:
+        raise ValueError(f"{what}: {hq} query heads must be a multiple of {hk} key heads")
+    if d % 8 or not 8 <= d <= 128:
+        raise ValueError(f"{what}: head dim {d} must be a multiple of 8 up to 128")
+    scale = d ** -0.5 if scale is None else float(scale)
+    softcap = float(softcap)
+    if not (0 < scale < math.inf) or not (0 <= softcap < math.inf):
+        raise ValueError(f"{what}: scale {scale} must be positive and softcap {softcap} positive or 0")
+    if prefix is not None and not causal:
+        raise ValueError(f"{what}: a prefix needs causal=True")
+    if slopes is not None and slopes.requires_grad:
+        raise ValueError(f"{what}: no gradient reaches slopes")
+    dev = q.device
+    slopes = _small(what, "slopes", slopes, (hq,), torch.float32, dev)
+    kv_lens = _small(what, "kv_lens", kv_lens, (b,), torch.int32, dev)
+    prefix = _small(what, "prefix", prefix, (b,), torch.int32, dev)
+    spans = None
+    if documents is not None:
+        documents = _small(what, "documents", documents, (b, lk), torch.int32, dev)
+        spans = _spans(documents, kv_lens, prefix, b, lq, lk, causal)
+    cfg = (scale, softcap, bool(causal))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _AttentionFn.apply(q, k, v, cfg, kv_lens, prefix, slopes, spans)
+    return _attn_fwd(q, k, v, cfg, kv_lens, prefix, slopes, spans, False)[0]

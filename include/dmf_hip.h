@@ -666,6 +666,58 @@ int dmf_affine_flip(const float* x, int N, int C, int H, int W, const float* par
 int dmf_resize_aa(const float* x, long long planes, int Hin, int Win, int Hout, int Wout, float* tmp, float* y,
                   void* stream);
 
+/* ------------------------------------------------------ token attention
+ * What stands between a token block's qkv projection and its output projection
+ * (transformer_model.py:100-116), beyond the plain softmax attention above. `dtype` is the storage type of
+ * queries, keys, values, outputs and their gradients (f32, bf16, f16); all arithmetic is f32. Element
+ * (b, l, h, i) of an operand stands at b*sb + l*sl + h*sh + i (element strides; the dims of a head are
+ * contiguous); outputs are contiguous [batch][len][heads][d].
+ *
+ * dmf_qk_norm_rope: y = rot(x * rsqrt(mean(x^2) + eps) * w) per head of the queries and keys in one launch.
+ *   norm 0: no norm (then no weights); wq / wk [d] null: ones. rot (even, <= d; 0: none): dims turned by
+ *   cos_t / sin_t [table_rows][rot/2] at the token's row, pairs (p, p + rot/2) or, interleaved, (2p, 2p + 1).
+ *   The row is pos[b*pos_sb + l] (int, or long long with pos64) or, pos null, l; a position outside the table makes the
+ *   rotated dims NaN. d even, at most 512.
+ * dmf_qk_norm_rope_bwd: dq / dk from dq_out / dk_out (contiguous), and, with the norm, dwq / dwk (both or
+ *   neither; overwritten), summed in a fixed order through ws (dmf_qk_norm_rope_bwd_ws_floats). */
+int dmf_qk_norm_rope(int dtype, const void* q, long long q_sb, long long q_sl, long long q_sh, int hq, const void* k,
+                     long long k_sb, long long k_sl, long long k_sh, int hk, int batch, int len, int d, int rot,
+                     int interleaved, int norm, float eps, const float* wq, const float* wk, const float* cos_t,
+                     const float* sin_t, const void* pos, long long pos_sb, int pos64, long long table_rows,
+                     void* q_out, void* k_out, void* stream);
+long long dmf_qk_norm_rope_bwd_ws_floats(int hq, int hk, int d);
+int dmf_qk_norm_rope_bwd(int dtype, const void* q, long long q_sb, long long q_sl, long long q_sh, int hq,
+                         const void* k, long long k_sb, long long k_sl, long long k_sh, int hk, int batch, int len,
+                         int d, int rot, int interleaved, int norm, float eps, const float* wq, const float* wk,
+                         const float* cos_t, const float* sin_t, const void* pos, long long pos_sb, int pos64,
+                         long long table_rows, const void* dq_out, const void* dk_out, void* dq, void* dk, float* dwq,
+                         float* dwk, float* ws, void* stream);
+/* dmf_mattn_fwd: o = softmax(s) v over the keys j that query i sees, s = softcap * tanh(z / softcap) (0: z) -
+ *   slopes[h] * |p - j|, z = scale * q.k; query head h reads key head h / (hq / hk). Query i stands at position
+ *   p = kv_len - lq + i (the queries are the last lq of the kv_len tokens); kv_lens [batch] (null: lk) is clamped to
+ *   [0, lk]. causal: j <= p, and the first prefix[b] keys (null: 0) are seen by all. spans [batch][lq][2]
+ *   (dmf_mattn_spans) takes the place of causal / prefix. A query that sees nothing has o = 0; keys that a query does not see
+ *   do not reach its output, whatever they hold. d a multiple of 8 up to 128, strides and bases multiples of 16 bytes.
+ *   For the backward: lse [batch][hk][lq][hq/hk] and, for 16-bit types, o_lo (what rounding o left over); both nullable.
+ *   ws: dmf_mattn_fwd_ws_floats floats (0: null allowed), where the keys are split over workgroups.
+ * dmf_mattn_bwd: dq, dk, dv from go = d o; delta: batch*lq*hq floats of scratch. No atomics: same bits every run.
+ * dmf_mattn_spans: spans of documents [batch] rows of doc_sb, lk ids each: a document is a maximal run of equal ids >= 0
+ *   within kv_len; a query sees its document, under causal up to itself or the document's first prefix[b] tokens. */
+int dmf_mattn_spans(const int* documents, long long doc_sb, const int* kv_lens, const int* prefix, int batch, int lq,
+                    int lk, int causal, int* spans, void* stream);
+long long dmf_mattn_fwd_ws_floats(int batch, int lq, int lk, int hq, int hk, int d);
+int dmf_mattn_fwd(int dtype, const void* q, long long q_sb, long long q_sl, long long q_sh, const void* k,
+                  long long k_sb, long long k_sl, long long k_sh, const void* v, long long v_sb, long long v_sl,
+                  long long v_sh, int batch, int lq, int lk, int hq, int hk, int d, float scale, float softcap,
+                  const float* slopes, int causal, const int* kv_lens, const int* prefix, const int* spans, void* o,
+                  void* o_lo, float* lse, float* ws, void* stream);
+int dmf_mattn_bwd(int dtype, const void* q, long long q_sb, long long q_sl, long long q_sh, const void* k,
+                  long long k_sb, long long k_sl, long long k_sh, const void* v, long long v_sb, long long v_sl,
+                  long long v_sh, int batch, int lq, int lk, int hq, int hk, int d, float scale, float softcap,
+                  const float* slopes, int causal, const int* kv_lens, const int* prefix, const int* spans,
+                  const void* o, const void* o_lo, const float* lse, const void* go, float* delta, void* dq, void* dk,
+                  void* dv, void* stream);
+
 /* ------------------------------------------------------------ optimizer
  * torch.optim.AdamW as built by LightningFusionOptimizerFactory
  * (selector_helpers.py:632-685, :617-629) -- multi-tensor, one launch. */
