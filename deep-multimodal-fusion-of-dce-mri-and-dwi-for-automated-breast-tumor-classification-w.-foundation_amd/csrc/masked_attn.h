@@ -21,11 +21,21 @@
 
 namespace dmf {
 
+struct AtScore {
+  float scale_u;    // scale * U (AtUnit)
+  float scale_cap;  // scale / cap
+  float cap_u;      // cap * U
+  float bend;       // -1 / cap_u^2
+  float poly[6];    // cap * U * tanh(x) = raw * poly(raw^2) for |x| = |raw| scale / cap <= 1 (16-bit types)
+};
+
 struct AtArgs {
   const void *q, *k, *v;
   long long q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh;  // element strides: batch, token, head
   int batch, lq, lk, hq, hk, d, group;
+  unsigned group_m;            // ceil(2^32 / group) (0 for 1): r / group = mulhi(r, group_m) while r * group < 2^32
   float scale, cap;            // cap 0: none
+  AtScore sc;                  // the score's constants (at_score_args)
   const float* slopes;         // [hq], null: none
   int causal;
   const int* kv_lens;          // [batch], null: lk
@@ -33,12 +43,12 @@ struct AtArgs {
   const int2* spans;           // [batch][lq] (documents), null: from the fields above
   void* o;                     // [batch][lq][hq][d]
   void* o_lo;                  // what rounding o to 16 bits left over (training: the backward's row sums), null: none
-  float* lse;                  // [batch][hk][lq * group]: log sum exp of s (log2 domain; natural for f32), null: none
+  float* lse;                  // [batch][hq][lq]: log sum exp of s (log2 domain; natural for f32), null: none
   int chunk, splits;           // keys per split, splits (1: the whole row in one workgroup)
-  float *po, *pml;             // partials [splits][batch * hk][rows][d], [..][2] (max, sum)
+  float *po, *pml;             // partials [splits][batch * hk][rows][d], [..][4] (max, o's sum, sum)
   // backward
   const void* go;              // [batch][lq][hq][d]
-  float* delta;                // [batch][hk][rows]
+  float* rowws;                // backward scratch: delta [batch][hq][lq], span lo [batch][lq], hi [batch][lq]
   void *dq, *dk, *dv;          // contiguous [batch][l][h][d]
 };
 
@@ -69,6 +79,27 @@ __device__ __forceinline__ at_f32x16 at_mfma(const uint4& a, const uint4& b, at_
 __device__ __forceinline__ at_f32x16 at_zero() {
   return at_f32x16{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 }
+
+// two floats rounded to a pair of 16-bit elements (one v_cvt_pk); sum of a pair's elements added to c (one v_dot2)
+template <typename T> struct AtPair;
+template <> struct AtPair<bf16_t> {
+  typedef __attribute__((ext_vector_type(2))) __bf16 V;
+  __device__ __forceinline__ static uint32_t pack(float l, float h) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((dmf_f2{l, h}), V));
+  }
+  __device__ __forceinline__ static float add(uint32_t w, float c) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(V, w), V{(__bf16)1.f, (__bf16)1.f}, c, false);
+  }
+};
+template <> struct AtPair<f16_t> {
+  typedef __attribute__((ext_vector_type(2))) _Float16 V;
+  __device__ __forceinline__ static uint32_t pack(float l, float h) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((dmf_f2{l, h}), V));
+  }
+  __device__ __forceinline__ static float add(uint32_t w, float c) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(V, w), V{(_Float16)1.f, (_Float16)1.f}, c, false);
+  }
+};
 
 // value of the other half wave's lane (lane ^ 32) combined with this one's
 __device__ __forceinline__ float at_half_max(float v) {
@@ -103,57 +134,108 @@ __device__ __forceinline__ int at_off(int row, int ch) {
   return row * (DP * AtT<T>::E) + ((ch ^ at_swz<T, DP>(row)) << 4);
 }
 
-// LDS-DMA of rows r0 .. r0 + ROWS - 1 of a strided matrix into a tile; rows outside [lo, hi) and the dims from d to DP
-// arrive as zeros from the buffer range check. `base` is row 0, sl the row stride in elements; all but the lane is
-// wave-uniform. NW waves share the work.
+// LDS-DMA of ROWS rows of a strided matrix into a tile, shared by NW waves. The lanes' byte offsets within a tile of rows
+// are computed once; a tile then costs scalar work only: its first row's address and, as the buffer's range, the bytes up to
+// row hi, past which rows arrive as zeros. The dims from d to DP get an offset past any range: zeros too. Needs a row stride
+// of at least d elements, and ROWS rows within 2 GiB.
 template <typename T, int DP, int ROWS, int NW>
-__device__ __forceinline__ void at_load_rows(const T* base, long long sl, int r0, int lo, int hi, int d, unsigned lds,
-                                             int wid, int lane) {
-  constexpr int NC = DP * AtT<T>::E / 16, PIECES = ROWS * NC / 64;
-  static_assert(PIECES % NW == 0, "pieces per wave");
-  const v4i_t rs = buf_rsrc(base + (long long)r0 * sl, AT_RECORDS);
+struct AtLoad {
+  static constexpr int NC = DP * AtT<T>::E / 16, PIECES = ROWS * NC / 64, PW = (PIECES + NW - 1) / NW;
+  unsigned voff[PW];
+  unsigned row_bytes;
+  __device__ __forceinline__ AtLoad(long long sl, int d, int wid, int lane) : row_bytes((unsigned)sl * AtT<T>::E) {
 #pragma unroll
-  for (int i = 0; i < PIECES / NW; ++i) {
-    const int p = wid * (PIECES / NW) + i, pos = p * 64 + lane, row = pos / NC;
-    const int ch = (pos % NC) ^ at_swz<T, DP>(row);
-    const bool ok = r0 + row >= lo && r0 + row < hi && ch * AtT<T>::CH < d;
-    dma16(rs, ok ? (unsigned)(row * (int)sl * AtT<T>::E + ch * 16) : BUF_OOB, 0, lds + p * 1024);
+    for (int i = 0; i < PW; ++i) {
+      const int pos = (wid * PW + i) * 64 + lane, row = pos / NC, ch = (pos % NC) ^ at_swz<T, DP>(row);
+      voff[i] = ch * AtT<T>::CH < d ? row * row_bytes + ch * 16 : BUF_OOB;
+    }
   }
-}
-// Bytes one wave's vmcnt counts per at_load_rows call are PIECES / NW instructions.
+  // rows r0 .. of base (row 0), valid below hi, to LDS address lds
+  __device__ __forceinline__ void issue(const T* base, int r0, int hi, unsigned lds, int wid) const {
+    const unsigned n = (unsigned)min(max(hi - r0, 0), ROWS);
+    const v4i_t rs = buf_rsrc((const char*)base + (unsigned long long)(unsigned)r0 * row_bytes,
+                              __builtin_amdgcn_readfirstlane(n * row_bytes));
+#pragma unroll
+    for (int i = 0; i < PW; ++i)
+      if (PIECES % NW == 0 || wid * PW + i < PIECES) dma16(rs, voff[i], 0, lds + (wid * PW + i) * 1024);
+  }
+};
 
-// one row operand: 8 (16-bit) or 4 (f32) consecutive dims of `row`, step ks (the steps cover DF dims)
-template <typename T, int DF>
-struct AtSteps { static constexpr int N = DF / (2 * AtT<T>::CH); };  // row-operand steps over the head dim
-template <typename T, int DP>
-__device__ __forceinline__ uint4 at_row(const char* tile, int row, int ks, int h) {
-  return *(const uint4*)(tile + at_off<T, DP>(row, 2 * ks + h));
+// one LDS-DMA wave-instruction of 4 B a lane: LDS [lds, lds + 256) (see dma16)
+__device__ __forceinline__ void at_dma4(v4i_t rsrc, unsigned voff, unsigned lds) {
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tbuffer_load_dword %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep)
+               : "v"(voff), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(lds))
+               : "memory");
 }
+
+// This lane's byte offsets into any tile of these dims: row operands (row lane & 31, step ks) and transposed operands
+// (column block fd, see at_accumulate). The XOR depends only on the row modulo 16, so other rows, tiles and stages are
+// constants added to these, which the LDS instructions take as immediates.
+template <typename T, int DF>
+struct AtOffsets {
+  static constexpr int DP = AtPad<DF>::DP, KS = DF / (2 * AtT<T>::CH), FD = DF / 32;
+  static constexpr int RB = DP * AtT<T>::E;
+  int row[KS];
+  int col[sizeof(T) == 2 ? 2 * FD : 1];
+  __device__ __forceinline__ explicit AtOffsets(int lane) {
+    const int h = lane >> 5;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) row[ks] = at_off<T, DP>(lane & 31, 2 * ks + h);
+    if constexpr (sizeof(T) == 2) {
+      const int r = 4 * h + ((lane >> 2) & 3), ch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+#pragma unroll
+      for (int fd = 0; fd < FD; ++fd) {
+        col[2 * fd] = at_off<T, DP>(r, 4 * fd + ch) + 8 * (lane & 1);
+        col[2 * fd + 1] = at_off<T, DP>(r + 8, 4 * fd + ch) + 8 * (lane & 1);
+      }
+    }
+  }
+};
+// one row operand: 8 (16-bit) or 4 (f32) consecutive dims of row r0 + (lane & 31) (r0 a multiple of 16), step ks
+template <typename T, int DF>
+__device__ __forceinline__ uint4 at_row(const char* tile, const AtOffsets<T, DF>& o, int r0, int ks) {
+  return *(const uint4*)(tile + r0 * AtOffsets<T, DF>::RB + o.row[ks]);
+}
+
+// A 32 x 32 result tile as the operand of the next product: 16-bit types rounded to pairs, f32 as it is
+template <typename T> struct AtP {
+  uint32_t w[8];
+  __device__ __forceinline__ explicit AtP(const float* p) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = AtPair<T>::pack(p[2 * i], p[2 * i + 1]);
+  }
+};
+template <> struct AtP<float> {
+  float w[16];
+  __device__ __forceinline__ explicit AtP(const float* p) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = p[i];
+  }
+};
 
 // acc[fd] += X^T P for the 32 tile rows r0 .. r0 + 31: X's column block fd (32 dims) as the row operand, read transposed
-// from its tile; P (32 rows x 32 columns) as a result tile whose registers are p[0..15]
+// from its tile
 template <typename T, int DF>
-__device__ __forceinline__ void at_accumulate(const char* tile, int r0, const float* p, at_f32x16* acc, int lane) {
-  constexpr int DP = AtPad<DF>::DP;
-  const int h = lane >> 5;
+__device__ __forceinline__ void at_accumulate(const char* tile, const AtOffsets<T, DF>& o, int r0, const AtP<T>& p,
+                                              at_f32x16* acc, int lane) {
+  constexpr int DP = AtPad<DF>::DP, RB = AtOffsets<T, DF>::RB;
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const uint4 b = make_uint4(B16<T>::pack(p[8 * c], p[8 * c + 1]), B16<T>::pack(p[8 * c + 2], p[8 * c + 3]),
-                                 B16<T>::pack(p[8 * c + 4], p[8 * c + 5]), B16<T>::pack(p[8 * c + 6], p[8 * c + 7]));
-      const int row = r0 + 16 * c + 4 * h + ((lane >> 2) & 3);
-      const int ch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+      const uint4 b = make_uint4(p.w[4 * c], p.w[4 * c + 1], p.w[4 * c + 2], p.w[4 * c + 3]);
+      const char* t = tile + (r0 + 16 * c) * RB;
 #pragma unroll
       for (int fd = 0; fd < DF / 32; ++fd) {
-        const at_v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (at_lds_v4s*)(tile + at_off<T, DP>(row, 4 * fd + ch) + 8 * (lane & 1)));
-        const at_v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (at_lds_v4s*)(tile + at_off<T, DP>(row + 8, 4 * fd + ch) + 8 * (lane & 1)));
-        const uint2 l = __builtin_bit_cast(uint2, lo), g = __builtin_bit_cast(uint2, hi);
+        const uint2 l = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_v4s*)(t + o.col[2 * fd])));
+        const uint2 g =
+            __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_v4s*)(t + o.col[2 * fd + 1])));
         acc[fd] = at_mfma<T>(make_uint4(l.x, l.y, g.x, g.y), b, acc[fd]);
       }
     }
   } else {
+    const int h = lane >> 5;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int row = r0 + 8 * (i >> 2) + 4 * h + (i & 3);
@@ -161,7 +243,7 @@ __device__ __forceinline__ void at_accumulate(const char* tile, int r0, const fl
       for (int fd = 0; fd < DF / 32; ++fd) {
         const int e = 32 * fd + (lane & 31);
         const float x = *(const float*)(tile + at_off<T, DP>(row, e >> 2) + 4 * (e & 3));
-        acc[fd] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p[i], acc[fd], 0, 0, 0);
+        acc[fd] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, p.w[i], acc[fd], 0, 0, 0);
       }
     }
   }
@@ -172,8 +254,11 @@ struct AtSpan {
   int lo, hi;  // hi <= lo: nothing
   int at;      // the query's position
 };
+__device__ __forceinline__ int at_keys(const AtArgs& a, int b) {
+  return a.kv_lens ? min(max(a.kv_lens[b], 0), a.lk) : a.lk;
+}
 __device__ __forceinline__ AtSpan at_span(const AtArgs& a, int b, int i) {
-  const int n = a.kv_lens ? min(max(a.kv_lens[b], 0), a.lk) : a.lk;
+  const int n = at_keys(a, b);
   AtSpan s;
   s.at = n - a.lq + i;
   if (a.spans) {
@@ -188,6 +273,17 @@ __device__ __forceinline__ AtSpan at_span(const AtArgs& a, int b, int i) {
   return s;
 }
 
+// packed row r of key head kh: query qi, query head
+struct AtRow {
+  int qi, head;
+};
+__device__ __forceinline__ AtRow at_packed(const AtArgs& a, int kh, int r) {
+  AtRow x;
+  x.qi = a.group_m ? (int)__umulhi((unsigned)r, a.group_m) : r;
+  x.head = kh * a.group + r - x.qi * a.group;
+  return x;
+}
+
 // wave-wide minimum / maximum of an int
 __device__ __forceinline__ int at_wave_min(int v) {
 #pragma unroll
@@ -197,26 +293,12 @@ __device__ __forceinline__ int at_wave_min(int v) {
 __device__ __forceinline__ int at_wave_max(int v) { return -at_wave_min(-v); }
 
 // ------------------------------------------------------------------ scores
-// CAP: tanh(x) = 1 - 2 / (exp(2 x) + 1): one v_exp, one v_rcp (absolute error ~1e-7, below the 16-bit rounding of the
-// probabilities); f32 calls tanhf, since cap * 1e-7 would be several f32 units of the exponent.
-template <typename T>
-__device__ __forceinline__ float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-template <typename T>
-__device__ __forceinline__ float at_tanh(float x) {  // of x = z / cap
-  if constexpr (sizeof(T) == 4)
-    return tanhf(x);
-  else
-    return fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * (2.f * AT_LOG2E)) + 1.f), 1.f);
-}
-// The exponent's unit is the log2 domain for 16-bit types (v_exp_f32 is 2^x: one multiply saved per score) and the
+// The exponent's unit U is the log2 domain for 16-bit types (v_exp_f32 is 2^x: one multiply saved per score) and the
 // natural one for f32, where scaling s before the maximum is subtracted would round it at |s| log2 e.
 template <typename T> struct AtUnit { static constexpr float U = sizeof(T) == 4 ? 1.f : AT_LOG2E; };
 template <typename T>
 __device__ __forceinline__ float at_exp(float x) {
-  if constexpr (sizeof(T) == 4)
-    return __builtin_amdgcn_exp2f(x * AT_LOG2E);
-  else
-    return __builtin_amdgcn_exp2f(x);
+  return __builtin_amdgcn_exp2f(sizeof(T) == 4 ? x * AT_LOG2E : x);
 }
 template <typename T>
 __device__ __forceinline__ float at_log(float x) {
@@ -225,30 +307,55 @@ __device__ __forceinline__ float at_log(float x) {
   else
     return __builtin_amdgcn_logf(x);  // log2
 }
-struct AtScore {
-  float scale_u;      // scale * U
-  float scale_cap;    // scale / cap
-  float cap_u;        // cap * U
-  float slope_u;      // slope * U (this lane's head)
-};
+
+// CAP. The scores are bound by the vector ALU, and there by v_exp / v_rcp (a quarter of the rate): tanh as
+// 1 - 2 / (exp(2 x) + 1) takes two of them and four more operations. While no score of a tile exceeds the cap
+// (|x| <= 1, checked per wave and tile with half an operation a score), tanh(x) / x is a polynomial of degree 5 in x^2
+// instead: minimax, relative error 5.9e-7, no transcendental, and its coefficients carry scale and cap. Either form is off by
+// less than 10 * 2^-24 * cap, below the 16-bit rounding of the probabilities; f32 calls tanhf, since that would be several
+// f32 units of the exponent.
 template <typename T>
-__device__ __forceinline__ AtScore at_score_of(const AtArgs& a, int head) {
-  AtScore s;
-  s.scale_u = a.scale * AtUnit<T>::U;
-  s.scale_cap = a.cap > 0.f ? a.scale / a.cap : 0.f;
-  s.cap_u = a.cap * AtUnit<T>::U;
-  s.slope_u = a.slopes ? a.slopes[head] * AtUnit<T>::U : 0.f;
-  return s;
+inline void at_score_args(AtArgs& a) {
+  static const double C[6] = {0.9999994039535522,    -0.3332904279232025,  0.13281433284282684,
+                              -0.051605671644210815, 0.016743114218115807, -0.0030670599082022196};
+  a.sc.scale_u = a.scale * AtUnit<T>::U;
+  a.sc.scale_cap = a.cap > 0.f ? a.scale / a.cap : 0.f;
+  a.sc.cap_u = a.cap * AtUnit<T>::U;
+  a.sc.bend = a.cap > 0.f ? -1.f / (a.sc.cap_u * a.sc.cap_u) : 0.f;
+  double x = a.sc.scale_cap;
+  for (int i = 0; i < 6; ++i) {
+    a.sc.poly[i] = (float)(C[i] * a.sc.cap_u * x);
+    x *= (double)a.sc.scale_cap * a.sc.scale_cap;
+  }
 }
-// s (in units U) of the raw product; dist = |a - j|
+template <typename T>
+__device__ __forceinline__ float at_slope(const AtArgs& a, int head) {
+  return a.slopes ? a.slopes[head] * AtUnit<T>::U : 0.f;
+}
+// cap tanh(z / cap), or z, in units U, of the raw product; SMALL: |raw| scale <= cap is known
+template <typename T, bool CAP, bool SMALL>
+__device__ __forceinline__ float at_bent(const AtScore& c, float raw) {
+  if constexpr (!CAP) {
+    return raw * c.scale_u;
+  } else if constexpr (sizeof(T) == 4) {
+    return c.cap_u * tanhf(raw * c.scale_cap);
+  } else if constexpr (SMALL) {
+    const float t = raw * raw;
+    float p = fmaf(c.poly[5], t, c.poly[4]);
+    p = fmaf(p, t, c.poly[3]);
+    p = fmaf(p, t, c.poly[2]);
+    p = fmaf(p, t, c.poly[1]);
+    return raw * fmaf(p, t, c.poly[0]);
+  } else {
+    const float e = __builtin_amdgcn_exp2f(raw * (c.scale_cap * (2.f * AT_LOG2E))) + 1.f;
+    return fmaf(-2.f * c.cap_u, __builtin_amdgcn_rcpf(e), c.cap_u);
+  }
+}
+// s (in units U) of one raw product; dist = |a - j|
 template <typename T, bool CAP, bool SLOPE>
-__device__ __forceinline__ float at_score(const AtScore& c, float raw, float dist) {
-  float s;
-  if constexpr (CAP)
-    s = c.cap_u * at_tanh<T>(raw * c.scale_cap);
-  else
-    s = raw * c.scale_u;
-  if constexpr (SLOPE) s = fmaf(-c.slope_u, dist, s);
+__device__ __forceinline__ float at_score(const AtScore& c, float slope_u, float raw, float dist) {
+  float s = at_bent<T, CAP, false>(c, raw);
+  if constexpr (SLOPE) s = fmaf(-slope_u, dist, s);
   return s;
 }
 

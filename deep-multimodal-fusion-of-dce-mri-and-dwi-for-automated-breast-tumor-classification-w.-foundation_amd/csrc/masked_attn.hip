@@ -79,7 +79,7 @@ static AtPlan at_plan(int batch, int lq, int lk, int hk, int group) {
   return p;
 }
 
-static int at_check(const char* who, const AtArgs& a, int dtype) {
+static int at_check(const char* who, AtArgs& a, int dtype) {
   DMF_CHECK_ARG(dtype == DMF_F32 || dtype == DMF_BF16 || dtype == DMF_F16, "%s: dtype %d", who, dtype);
   DMF_CHECK_ARG(a.batch >= 0 && a.lq >= 0 && a.lk >= 0 && a.hk >= 1 && a.hq >= 1 && a.hq % a.hk == 0,
                 "%s: %d query heads must be a multiple of %d key heads", who, a.hq, a.hk);
@@ -92,6 +92,8 @@ static int at_check(const char* who, const AtArgs& a, int dtype) {
                 "%s: %d queries x %d heads x %d rows exceed the launch", who, a.lq, a.hq, a.batch);
   const int e = dtype == DMF_F32 ? 4 : 2;
   const long long st[] = {a.q_sb, a.q_sl, a.q_sh, a.k_sb, a.k_sl, a.k_sh, a.v_sb, a.v_sl, a.v_sh};
+  DMF_CHECK_ARG((a.lq <= 1 || a.q_sl >= a.d) && (a.lk <= 1 || (a.k_sl >= a.d && a.v_sl >= a.d)),
+                "%s: token strides %lld / %lld / %lld must be at least the head dim", who, a.q_sl, a.k_sl, a.v_sl);
   for (long long s : st) DMF_CHECK_ARG(s >= 0 && s * e % 16 == 0, "%s: stride %lld is not a multiple of 16 bytes", who, s);
   DMF_CHECK_ARG((uintptr_t)a.q % 16 == 0 && (uintptr_t)a.k % 16 == 0 && (uintptr_t)a.v % 16 == 0,
                 "%s: q, k and v must be aligned to 16 bytes", who);
@@ -99,6 +101,8 @@ static int at_check(const char* who, const AtArgs& a, int dtype) {
                     (130 * a.q_sl + a.group * a.q_sh) * e < (1LL << 31) &&
                     (130LL * a.hq * a.d + (long long)a.hq * a.d) * e < (1LL << 31),
                 "%s: a tile of rows spans more than 2 GiB", who);
+  if (a.lq <= 1) a.q_sl = a.d;  // (a length of one: any stride says the same)
+  if (a.lk <= 1) a.k_sl = a.v_sl = a.d;
   return 0;
 }
 
@@ -120,7 +124,7 @@ extern "C" int dmf_mattn_spans(const int* documents, long long doc_sb, const int
 extern "C" long long dmf_mattn_fwd_ws_floats(int batch, int lq, int lk, int hq, int hk, int d) {
   if (batch <= 0 || lq <= 0 || lk <= 0 || hk <= 0 || hq < hk) return 0;
   const AtPlan p = at_plan(batch, lq, lk, hk, hq / hk);
-  return p.splits > 1 ? (long long)p.splits * batch * lq * hq * (d + 2) : 0;
+  return p.splits > 1 ? (long long)p.splits * batch * lq * hq * (d + 4) : 0;
 }
 
 extern "C" int dmf_mattn_fwd(int dtype, const void* q, long long q_sb, long long q_sl, long long q_sh, const void* k,
@@ -134,6 +138,7 @@ extern "C" int dmf_mattn_fwd(int dtype, const void* q, long long q_sb, long long
   a.q_sb = q_sb, a.q_sl = q_sl, a.q_sh = q_sh, a.k_sb = k_sb, a.k_sl = k_sl, a.k_sh = k_sh;
   a.v_sb = v_sb, a.v_sl = v_sl, a.v_sh = v_sh;
   a.batch = batch, a.lq = lq, a.lk = lk, a.hq = hq, a.hk = hk, a.d = d, a.group = hk > 0 ? hq / hk : 0;
+  a.group_m = a.group > 1 ? (unsigned)(((1ULL << 32) + a.group - 1) / a.group) : 0;
   a.scale = scale, a.cap = softcap, a.slopes = slopes, a.causal = causal, a.kv_lens = kv_lens, a.prefix = prefix;
   a.spans = (const int2*)spans, a.o = o, a.o_lo = o_lo, a.lse = lse;
   if (int rc = at_check("dmf_mattn_fwd", a, dtype)) return rc;
@@ -158,18 +163,19 @@ extern "C" int dmf_mattn_bwd(int dtype, const void* q, long long q_sb, long long
                              long long v_sl, long long v_sh, int batch, int lq, int lk, int hq, int hk, int d,
                              float scale, float softcap, const float* slopes, int causal, const int* kv_lens,
                              const int* prefix, const int* spans, const void* o, const void* o_lo, const float* lse,
-                             const void* go, float* delta, void* dq, void* dk, void* dv, void* stream) {
+                             const void* go, float* ws, void* dq, void* dk, void* dv, void* stream) {
   AtArgs a = {};
   a.q = q, a.k = k, a.v = v;
   a.q_sb = q_sb, a.q_sl = q_sl, a.q_sh = q_sh, a.k_sb = k_sb, a.k_sl = k_sl, a.k_sh = k_sh;
   a.v_sb = v_sb, a.v_sl = v_sl, a.v_sh = v_sh;
   a.batch = batch, a.lq = lq, a.lk = lk, a.hq = hq, a.hk = hk, a.d = d, a.group = hk > 0 ? hq / hk : 0;
+  a.group_m = a.group > 1 ? (unsigned)(((1ULL << 32) + a.group - 1) / a.group) : 0;
   a.scale = scale, a.cap = softcap, a.slopes = slopes, a.causal = causal, a.kv_lens = kv_lens, a.prefix = prefix;
-  a.spans = (const int2*)spans, a.o = (void*)o, a.o_lo = (void*)o_lo, a.lse = (float*)lse, a.go = go, a.delta = delta;
+  a.spans = (const int2*)spans, a.o = (void*)o, a.o_lo = (void*)o_lo, a.lse = (float*)lse, a.go = go, a.rowws = ws;
   a.dq = dq, a.dk = dk, a.dv = dv;
   if (int rc = at_check("dmf_mattn_bwd", a, dtype)) return rc;
   if (batch == 0 || (lq == 0 && lk == 0)) return 0;
-  DMF_CHECK_ARG((lq == 0 || (q && o && lse && go && delta && dq)) && (lk == 0 || (k && v && dk && dv)),
+  DMF_CHECK_ARG((lq == 0 || (q && o && lse && go && ws && dq)) && (lk == 0 || (k && v && dk && dv)),
                 "dmf_mattn_bwd: null operand");
   const uintptr_t al = (uintptr_t)o | (uintptr_t)o_lo | (uintptr_t)go | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv;
   DMF_CHECK_ARG(al % 16 == 0 && (uintptr_t)spans % 8 == 0, "dmf_mattn_bwd: operands must be aligned to 16 bytes");

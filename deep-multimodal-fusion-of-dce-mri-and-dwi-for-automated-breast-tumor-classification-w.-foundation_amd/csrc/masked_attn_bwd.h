@@ -1,6 +1,6 @@
 // Masked attention backward (see masked_attn.h for the mathematics and the layouts).
 //
-//   delta_i = sum_d do_i o_i          (k_mattn_delta; o with the part its 16-bit rounding left over, so that rounding does
+//   delta_i = sum_d do_i o_i          (k_mattn_rows; o with the part its 16-bit rounding left over, so that rounding does
 //                                      not enter dS through the whole row)
 //   p_ij = exp(s_ij - lse_i),  dp_ij = do_i . v_j,  ds_ij = p_ij (dp_ij - delta_i) (1 - tanh^2(z_ij / cap))
 //   dv_j = sum_i p_ij do_i,  dk_j = scale sum_i ds_ij q_i,  dq_i = scale sum_j ds_ij k_j
@@ -15,20 +15,9 @@
 
 namespace dmf {
 
-// packed row r of a (batch row, key head): query r / group, head kh * group + r % group
-struct AtRow {
-  int qi, head;
-};
-__device__ __forceinline__ AtRow at_packed(const AtArgs& a, int kh, int r) {
-  AtRow x;
-  x.qi = r / a.group;
-  x.head = kh * a.group + r - x.qi * a.group;
-  return x;
-}
-
-// delta: one lane group of 16 per packed row
+// What the backward needs of each row beside lse (a.rowws): delta, and the query's span. One lane group of 16 per row.
 template <typename T>
-__global__ void __launch_bounds__(256) k_mattn_delta(AtArgs a) {
+__global__ void __launch_bounds__(256) k_mattn_rows(AtArgs a) {
   const long long g = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4;  // (b, query, head)
   const int l16 = threadIdx.x & 15;
   const long long n = (long long)a.batch * a.lq * a.hq;
@@ -54,78 +43,85 @@ __global__ void __launch_bounds__(256) k_mattn_delta(AtArgs a) {
   if (l16 == 0) {
     const int head = (int)(g % a.hq);
     const long long bq = g / a.hq;
-    const int qi = (int)(bq % a.lq), b = (int)(bq / a.lq), kh = head / a.group;
-    a.delta[((long long)b * a.hk + kh) * a.lq * a.group + qi * a.group + head - kh * a.group] = t;
+    const int qi = (int)(bq % a.lq), b = (int)(bq / a.lq);
+    a.rowws[((long long)b * a.hq + head) * a.lq + qi] = t;
+    if (head == 0) {
+      const AtSpan sp = at_span(a, b, qi);
+      ((int*)a.rowws)[n + bq] = sp.lo;
+      ((int*)a.rowws)[n + (long long)a.batch * a.lq + bq] = sp.hi;
+    }
   }
 }
 
-// ds and p of one score (p masked to 0 by the caller)
+// p and ds of one score s = cap tanh(z / cap) (units U); dist = |a - j|
 template <typename T, bool CAP, bool SLOPE>
-__device__ __forceinline__ void at_grad(const AtScore& c, float slope_u, float raw, float dist, float lse, float dp,
+__device__ __forceinline__ void at_grad(const AtArgs& a, float slope_u, float s, float dist, float lse, float dp,
                                         float delta, float& p, float& ds) {
-  float s, bend = 1.f;
-  if constexpr (CAP) {
-    const float t = at_tanh<T>(raw * c.scale_cap);
-    s = c.cap_u * t;
-    bend = fmaf(-t, t, 1.f);
-  } else {
-    s = raw * c.scale_u;
-  }
-  if constexpr (SLOPE) s = fmaf(-slope_u, dist, s);
-  p = at_exp<T>(s - lse);
+  float e = s - lse;
+  if constexpr (SLOPE) e = fmaf(-slope_u, dist, s) - lse;
+  p = at_exp<T>(e);
   ds = p * (dp - delta);
-  if constexpr (CAP) ds *= bend;
+  if constexpr (CAP) ds *= fmaf(s * s, a.sc.bend, 1.f);  // 1 - tanh^2
+}
+// raw products of one 32 x 32 tile -> s, with the polynomial where the whole wave's tile allows it
+template <typename T, bool CAP>
+__device__ __forceinline__ void at_bend_tile(const AtArgs& a, at_f32x16& s) {
+  if constexpr (CAP && sizeof(T) == 2) {
+    float big = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(s[i]));
+    if (__any(big * a.sc.scale_cap > 1.f)) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = at_bent<T, true, false>(a.sc, s[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = at_bent<T, true, true>(a.sc, s[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = at_bent<T, CAP, false>(a.sc, s[i]);
+  }
 }
 
-// LDS of the 128-key workgroups: two stages of (Q, dO) tiles, then two stages of the per-row values
-template <int QT> struct AtRowData {
-  float lse[QT], delta[QT], at[QT], slope[QT];
-  int lo[QT], hi[QT];
-  unsigned full[4], none[4];  // bit s of [w]: every row of 32-row subtile s sees all / none of wave w's keys
+// LDS of the 128-key workgroups: their V tile, two stages of (Q, dO) tiles of 32 queries of one head, two of the rows'
+// values (one DMA instruction each, whose upper 32 lanes bring zeros). K stays in registers as the score's operand; V does
+// not fit there beside the two accumulators (192 registers) and is read from LDS for each dP.
+struct AtRowData {
+  float lse[64], delta[64];
+  int lo[64], hi[64];
+};
+constexpr int AT_QT = 32;
+template <typename T, int DF> struct AtBwdLds {
+  static constexpr int RB = AtPad<DF>::DP * AtT<T>::E;
+  static constexpr int KT = sizeof(T) == 4 ? 32 : 64;       // keys per tile of the 128-row workgroups
+  static constexpr int QTILE = AT_QT * RB, VT = 128 * RB;
+  static constexpr int KEYS = VT + 4 * QTILE + 2 * (int)sizeof(AtRowData), ROWS = 4 * KT * RB;
+  static constexpr int BYTES = (KEYS > ROWS ? KEYS : ROWS) + 8 * (int)sizeof(int);
 };
 
-template <typename T> struct AtBwdTile { static constexpr int QT = sizeof(T) == 4 ? 32 : 64, KT = QT; };
-
-// Q / dO rows r0 .. r0 + QT - 1 (packed) into a tile: as at_load_rows, with the packed row's address per lane
-template <typename T, int DP, int ROWS>
-__device__ __forceinline__ void at_load_packed(const AtArgs& a, const T* base, long long sl, long long sh, int r0, int r1,
-                                               unsigned lds, int wid, int lane) {
-  constexpr int NC = DP * AtT<T>::E / 16, PIECES = ROWS * NC / 64;
-  const int i0 = r0 / a.group;
-  const v4i_t rs = buf_rsrc(base + (long long)i0 * sl, AT_RECORDS);
-#pragma unroll
-  for (int i = 0; i < PIECES / 4; ++i) {
-    const int p = wid * (PIECES / 4) + i, pos = p * 64 + lane, row = pos / NC;
-    const int ch = (pos % NC) ^ at_swz<T, DP>(row);
-    const int r = r0 + row, qi = r / a.group, g = r - qi * a.group;
-    const bool ok = r < r1 && ch * AtT<T>::CH < a.d;
-    dma16(rs, ok ? (unsigned)(((qi - i0) * (int)sl + g * (int)sh) * AtT<T>::E + ch * 16) : BUF_OOB, 0, lds + p * 1024);
-  }
-}
-
-// dk, dv of one key over the packed rows that see it: each lane holds dims lane and lane + 64
+// dk, dv of one key over the queries in [q0, q1] that see it: each lane holds dims lane and lane + 64
 template <typename T, bool CAP, bool SLOPE>
-__device__ void at_key_alone(const AtArgs& a, int b, int kh, int j, int r0, int r1, int lane, float dk[2], float dv[2]) {
+__device__ void at_key_alone(const AtArgs& a, int b, int kh, int j, int q0, int q1, int lane, float dk[2], float dv[2]) {
   const T* kj = (const T*)a.k + b * a.k_sb + kh * a.k_sh + j * a.k_sl;
   const T* vj = (const T*)a.v + b * a.v_sb + kh * a.v_sh + j * a.v_sl;
   const bool on0 = lane < a.d, on1 = lane + 64 < a.d;
   const float k0 = on0 ? ld(kj + lane) : 0.f, k1 = on1 ? ld(kj + lane + 64) : 0.f;
   const float v0 = on0 ? ld(vj + lane) : 0.f, v1 = on1 ? ld(vj + lane + 64) : 0.f;
   dk[0] = dk[1] = dv[0] = dv[1] = 0.f;
-  const long long rows = (long long)a.lq * a.group, rb = ((long long)b * a.hk + kh) * rows;
-  for (int r = r0; r < r1; ++r) {
-    const AtRow x = at_packed(a, kh, r);
-    const AtSpan sp = at_span(a, b, x.qi);
+  for (int n = 0; n < (q1 - q0 + 1) * a.group; ++n) {
+    const int qi = q0 + n / a.group, head = kh * a.group + n % a.group;
+    const AtSpan sp = at_span(a, b, qi);
     if (j < sp.lo || j >= sp.hi) continue;
-    const T* q = (const T*)a.q + b * a.q_sb + (long long)x.qi * a.q_sl + x.head * a.q_sh;
-    const T* g = (const T*)a.go + (((long long)b * a.lq + x.qi) * a.hq + x.head) * a.d;
-    const float q0 = on0 ? ld(q + lane) : 0.f, q1 = on1 ? ld(q + lane + 64) : 0.f;
+    const T* q = (const T*)a.q + b * a.q_sb + (long long)qi * a.q_sl + head * a.q_sh;
+    const T* g = (const T*)a.go + (((long long)b * a.lq + qi) * a.hq + head) * a.d;
+    const long long rb = ((long long)b * a.hq + head) * a.lq + qi;
+    const float x0 = on0 ? ld(q + lane) : 0.f, x1 = on1 ? ld(q + lane + 64) : 0.f;
     const float g0 = on0 ? ld(g + lane) : 0.f, g1 = on1 ? ld(g + lane + 64) : 0.f;
-    const float raw = wave_sum(fmaf(q0, k0, q1 * k1)), dp = wave_sum(fmaf(g0, v0, g1 * v1));
-    const AtScore sc = at_score_of<T>(a, x.head);
+    const float raw = wave_sum(fmaf(x0, k0, x1 * k1)), dp = wave_sum(fmaf(g0, v0, g1 * v1));
     float p, ds;
-    at_grad<T, CAP, SLOPE>(sc, sc.slope_u, raw, fabsf((float)(sp.at - j)), a.lse[rb + r], dp, a.delta[rb + r], p, ds);
-    dk[0] = fmaf(ds, q0, dk[0]), dk[1] = fmaf(ds, q1, dk[1]);
+    at_grad<T, CAP, SLOPE>(a, at_slope<T>(a, head), at_bent<T, CAP, false>(a.sc, raw), fabsf((float)(sp.at - j)),
+                           a.lse[rb], dp, a.rowws[rb], p, ds);
+    dk[0] = fmaf(ds, x0, dk[0]), dk[1] = fmaf(ds, x1, dk[1]);
     dv[0] = fmaf(p, g0, dv[0]), dv[1] = fmaf(p, g1, dv[1]);
   }
 }
@@ -139,9 +135,9 @@ __device__ void at_query_alone(const AtArgs& a, int b, int kh, int r, int lo, in
   const bool on0 = lane < a.d, on1 = lane + 64 < a.d;
   const float q0 = on0 ? ld(q + lane) : 0.f, q1 = on1 ? ld(q + lane + 64) : 0.f;
   const float g0 = on0 ? ld(g + lane) : 0.f, g1 = on1 ? ld(g + lane + 64) : 0.f;
-  const long long rb = ((long long)b * a.hk + kh) * a.lq * a.group + r;
-  const float lse = a.lse[rb], delta = a.delta[rb];
-  const AtScore sc = at_score_of<T>(a, x.head);
+  const long long rb = ((long long)b * a.hq + x.head) * a.lq + x.qi;
+  const float lse = a.lse[rb], delta = a.rowws[rb];
+  const float slope = at_slope<T>(a, x.head);
   dq[0] = dq[1] = 0.f;
   for (int j = lo; j < hi; ++j) {
     const T* kj = (const T*)a.k + b * a.k_sb + kh * a.k_sh + j * a.k_sl;
@@ -150,7 +146,7 @@ __device__ void at_query_alone(const AtArgs& a, int b, int kh, int r, int lo, in
     const float v0 = on0 ? ld(vj + lane) : 0.f, v1 = on1 ? ld(vj + lane + 64) : 0.f;
     const float raw = wave_sum(fmaf(q0, k0, q1 * k1)), dp = wave_sum(fmaf(g0, v0, g1 * v1));
     float p, ds;
-    at_grad<T, CAP, SLOPE>(sc, sc.slope_u, raw, fabsf((float)(at - j)), lse, dp, delta, p, ds);
+    at_grad<T, CAP, SLOPE>(a, slope, at_bent<T, CAP, false>(a.sc, raw), fabsf((float)(at - j)), lse, dp, delta, p, ds);
     dq[0] = fmaf(ds, k0, dq[0]), dq[1] = fmaf(ds, k1, dq[1]);
   }
 }
@@ -172,26 +168,36 @@ __device__ __forceinline__ void at_store_row(T* out, const at_f32x16* acc, int d
 
 template <typename T, int DF, bool CAP, bool SLOPE>
 __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, char* smem) {
-  constexpr int DP = AtPad<DF>::DP, KS = AtSteps<T, DF>::N, FD = DF / 32, QT = AtBwdTile<T>::QT;
-  constexpr int TILE = QT * DP * AtT<T>::E, STAGE = 2 * TILE;
-  AtRowData<QT>* rd = (AtRowData<QT>*)(smem + 2 * STAGE);
-  int* range = (int*)(rd + 2);  // [8]
+  typedef AtBwdLds<T, DF> L;
+  constexpr int DP = AtPad<DF>::DP, KS = AtOffsets<T, DF>::KS, FD = DF / 32;
+  constexpr int TILE = L::QTILE, STAGE = 2 * TILE;
+  int* range = (int*)(smem + L::BYTES) - 8;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
-  const int b = bh / a.hk, kh = bh - b * a.hk, rows = a.lq * a.group;
+  const int b = bh / a.hk, kh = bh - b * a.hk;
   const int kb0 = ktile * 128, kw0 = kb0 + 32 * wid, key = kw0 + (lane & 31);
   const unsigned lds0 = (unsigned)(uintptr_t)((__attribute__((address_space(3))) char*)smem);
-  const T* qb = (const T*)a.q + b * a.q_sb + kh * a.group * a.q_sh;
-  const T* gb = (const T*)a.go + ((long long)b * a.lq * a.hq + kh * a.group) * a.d;
-  const long long rb = (long long)bh * rows;
+  const T* kb = (const T*)a.k + b * a.k_sb + kh * a.k_sh;
+  const T* vb = (const T*)a.v + b * a.v_sb + kh * a.v_sh;
 
   // the queries that see any of the 128 keys lie in [q0, q1]
+  const long long nrows = (long long)a.batch * a.hq * a.lq, nq = (long long)a.batch * a.lq;
+  const int* w_lo = (const int*)a.rowws + nrows + (long long)b * a.lq;
+  const int* w_hi = w_lo + nq;
   int q0 = 0x7fffffff, q1 = -1;
-  for (int i = threadIdx.x; i < a.lq; i += 256) {
-    const AtSpan sp = at_span(a, b, i);
-    if (sp.hi > kb0 && sp.lo < kb0 + 128 && sp.hi > sp.lo) {
-      q0 = min(q0, i);
-      q1 = max(q1, i);
+  for (int i = threadIdx.x; i < a.lq; i += 1024) {
+    int lo[4], hi[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = min(i + 256 * u, a.lq - 1);
+      lo[u] = w_lo[r];
+      hi[u] = w_hi[r];
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i + 256 * u < a.lq && hi[u] > kb0 && lo[u] < kb0 + 128) {
+        q0 = min(q0, i + 256 * u);
+        q1 = max(q1, i + 256 * u);
+      }
   }
   q0 = at_wave_min(q0), q1 = at_wave_max(q1);
   if (lane == 0) range[wid] = q0, range[4 + wid] = q1;
@@ -200,110 +206,93 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
   for (int w = 0; w < 4; ++w) q0 = min(q0, range[w]), q1 = max(q1, range[4 + w]);
   q0 = __builtin_amdgcn_readfirstlane(q0);
   q1 = __builtin_amdgcn_readfirstlane(q1);
-  const int r0 = q1 >= 0 ? q0 * a.group : 0, r1 = (q1 + 1) * a.group;
 
-  uint4 kf[KS], vf[KS];
+  uint4 kf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
     const int e = (2 * ks + h) * AtT<T>::CH;
-    const bool ok = key < a.lk && e < a.d;
-    kf[ks] = ok ? *(const uint4*)((const T*)a.k + b * a.k_sb + kh * a.k_sh + key * a.k_sl + e) : make_uint4(0, 0, 0, 0);
-    vf[ks] = ok ? *(const uint4*)((const T*)a.v + b * a.v_sb + kh * a.v_sh + key * a.v_sl + e) : make_uint4(0, 0, 0, 0);
+    kf[ks] = key < a.lk && e < a.d ? *(const uint4*)(kb + key * a.k_sl + e) : make_uint4(0, 0, 0, 0);
   }
-  auto issue = [&](int stage, int r) {
-    at_load_packed<T, DP, QT>(a, qb, a.q_sl, a.q_sh, r, r1, lds0 + stage * STAGE, wid, lane);
-    at_load_packed<T, DP, QT>(a, gb, (long long)a.hq * a.d, a.d, r, r1, lds0 + stage * STAGE + TILE, wid, lane);
-  };
-  // the rows' values for one tile, by the first QT threads (wave 0)
-  auto row_data = [&](int stage, int r) {
-    if (wid != 0) return;
-    AtRowData<QT>& x = rd[stage];
-    const int rr = r + lane;
-    const bool in = lane < QT && rr < r1;
-    AtSpan sp = {0, 0, 0};
-    float lse = INFINITY, delta = 0.f, slope = 0.f;
-    if (in) {
-      const AtRow pr = at_packed(a, kh, rr);
-      sp = at_span(a, b, pr.qi);
-      lse = a.lse[rb + rr];
-      delta = a.delta[rb + rr];
-      if (SLOPE) slope = a.slopes[pr.head] * AtUnit<T>::U;
-    }
-    const bool live = sp.hi > sp.lo;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const int kw = kb0 + 32 * w;
-      const unsigned long long f = __ballot(live && sp.lo <= kw && sp.hi >= kw + 32);
-      const unsigned long long n = __ballot(!live || sp.hi <= kw || sp.lo >= kw + 32);
-      if (lane == 0) {
-        x.full[w] = ((unsigned)f == ~0u ? 1 : 0) | ((unsigned)(f >> 32) == ~0u ? 2 : 0);
-        x.none[w] = ((unsigned)n == ~0u ? 1 : 0) | ((unsigned)(n >> 32) == ~0u ? 2 : 0);
-      }
-    }
-    if (lane < QT) {
-      x.lse[lane] = lse;
-      x.delta[lane] = delta;
-      x.at[lane] = (float)sp.at;
-      x.slope[lane] = slope;
-      x.lo[lane] = sp.lo;
-      x.hi[lane] = sp.hi;
-    }
+  const AtLoad<T, DP, AT_QT, 4> ql(a.q_sl, a.d, wid, lane), gl((long long)a.hq * a.d, a.d, wid, lane);
+  // wave w brings the tile's lse / delta / lo / hi
+  const float* rv = wid == 0 ? a.lse : wid == 1 ? a.rowws : (const float*)(wid == 2 ? w_lo : w_hi);
+  const long long rv0 = wid < 2 ? ((long long)b * a.hq + kh * a.group) * a.lq : 0, rvh = wid < 2 ? a.lq : 0;
+  const unsigned rvo = lane < AT_QT ? (unsigned)lane * 4 : BUF_OOB;
+  auto issue = [&](int stage, int g, int i0) {
+    const unsigned S = lds0 + L::VT + stage * STAGE;
+    const int head = kh * a.group + g;
+    ql.issue((const T*)a.q + b * a.q_sb + head * a.q_sh, i0, q1 + 1, S, wid);
+    gl.issue((const T*)a.go + ((long long)b * a.lq * a.hq + head) * a.d, i0, q1 + 1, S + TILE, wid);
+    // queries past the last arrive as zeros: an empty span
+    at_dma4(buf_rsrc(rv + rv0 + g * rvh + i0, __builtin_amdgcn_readfirstlane(min(q1 + 1 - i0, AT_QT) * 4)), rvo,
+            lds0 + L::VT + 2 * STAGE + stage * (unsigned)sizeof(AtRowData) + wid * 256);
   };
 
-  const AtScore sc = at_score_of<T>(a, kh * a.group);
   at_f32x16 dk[FD], dv[FD];
 #pragma unroll
   for (int f = 0; f < FD; ++f) dk[f] = at_zero(), dv[f] = at_zero();
-  const int nt = r1 > r0 ? (r1 - r0 + QT - 1) / QT : 0;
-  if (nt > 0) {
-    row_data(0, r0);
-    issue(0, r0);
-  }
-  for (int t = 0; t < nt; ++t) {
+  const AtOffsets<T, DF> off(lane);
+  const char* V = smem + wid * 32 * L::RB;
+  const int n0 = (at_keys(a, b)) - a.lq;  // position of query 0
+  int g = 0, i0 = q0;                          // the tile in hand: head, first query
+  auto step = [&](auto stage) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (t + 1 < nt) {
-      row_data((t + 1) & 1, r0 + (t + 1) * QT);
-      issue((t + 1) & 1, r0 + (t + 1) * QT);
-    }
-    const char* Q = smem + (t & 1) * STAGE;
+    int g1 = g, i1 = i0 + AT_QT;  // the next one
+    if (i1 > q1) i1 = q0, ++g1;
+    if (g1 < a.group) issue(1 - stage.value, g1, i1);
+    const char* Q = smem + L::VT + stage.value * STAGE;
     const char* G = Q + TILE;
-    const AtRowData<QT>& x = rd[t & 1];
-    const unsigned full = __builtin_amdgcn_readfirstlane(x.full[wid]), none = __builtin_amdgcn_readfirstlane(x.none[wid]);
-#pragma unroll
-    for (int f = 0; f < QT / 32; ++f) {
-      if ((none >> f) & 1) continue;
+    const AtRowData& x = *(const AtRowData*)(smem + L::VT + 2 * STAGE + stage.value * (int)sizeof(AtRowData));
+    const int f_lo = x.lo[lane & 31], f_hi = x.hi[lane & 31];
+    if (__any(f_hi > kw0 && f_lo < kw0 + 32)) {                     // some row sees some of this wave's keys
+      const bool full = __all(f_lo <= kw0 && f_hi >= kw0 + 32);     // every row sees all of them
       at_f32x16 s = at_zero(), dp = at_zero();
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        s = at_mfma<T>(at_row<T, DP>(Q, 32 * f + (lane & 31), ks, h), kf[ks], s);
-        dp = at_mfma<T>(at_row<T, DP>(G, 32 * f + (lane & 31), ks, h), vf[ks], dp);
-      }
+      for (int ks = 0; ks < KS; ++ks) s = at_mfma<T>(at_row<T, DF>(Q, off, 0, ks), kf[ks], s);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) dp = at_mfma<T>(at_row<T, DF>(G, off, 0, ks), at_row<T, DF>(V, off, 0, ks), dp);
+      at_bend_tile<T, CAP>(a, s);
+      const float slope = SLOPE ? at_slope<T>(a, kh * a.group + g) : 0.f;
+      const float x0 = (float)(n0 + i0 + 4 * h - key);  // position of this lane's first row minus its key
       float p[16], ds[16];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int rr = 32 * f + 8 * g + 4 * h;
-        const float4 lse = *(const float4*)(x.lse + rr), delta = *(const float4*)(x.delta + rr);
-        float4 at = make_float4(0.f, 0.f, 0.f, 0.f), slope = at;
-        if constexpr (SLOPE) at = *(const float4*)(x.at + rr), slope = *(const float4*)(x.slope + rr);
-        const float* lp = &lse.x;
-        const float* dl = &delta.x;
-        const float* ap = &at.x;
-        const float* sp = &slope.x;
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const float4 lse = *(const float4*)(x.lse + 8 * r4 + 4 * h), delta = *(const float4*)(x.delta + 8 * r4 + 4 * h);
+        const float lp[4] = {lse.x, lse.y, lse.z, lse.w}, dl[4] = {delta.x, delta.y, delta.z, delta.w};
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          at_grad<T, CAP, SLOPE>(sc, sp[r], s[4 * g + r], fabsf(ap[r] - (float)key), lp[r], dp[4 * g + r], dl[r],
-                                 p[4 * g + r], ds[4 * g + r]);
+        for (int r = 0; r < 4; ++r) {
+          const int i = 4 * r4 + r;
+          at_grad<T, CAP, SLOPE>(a, slope, s[i], fabsf(x0 + (float)(8 * r4 + r)), lp[r], dp[i], dl[r], p[i], ds[i]);
+        }
       }
-      if (!((full >> f) & 1)) {
+      if (!full) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int rr = 32 * f + 8 * (i >> 2) + 4 * h + (i & 3);
-          if (key < x.lo[rr] || key >= x.hi[rr]) p[i] = ds[i] = 0.f;
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const int4 lo = *(const int4*)(x.lo + 8 * r4 + 4 * h), hi = *(const int4*)(x.hi + 8 * r4 + 4 * h);
+          const int out[4] = {(key < lo.x) | (key >= hi.x), (key < lo.y) | (key >= hi.y), (key < lo.z) | (key >= hi.z),
+                              (key < lo.w) | (key >= hi.w)};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            p[4 * r4 + r] = out[r] ? 0.f : p[4 * r4 + r];
+            ds[4 * r4 + r] = out[r] ? 0.f : ds[4 * r4 + r];
+          }
         }
       }
       // p and ds are rounded to the 16-bit operand type (half a step each)
-      at_accumulate<T, DF>(G, 32 * f, p, dv, lane);
-      at_accumulate<T, DF>(Q, 32 * f, ds, dk, lane);
+      at_accumulate<T, DF>(G, off, 0, AtP<T>(p), dv, lane);
+      at_accumulate<T, DF>(Q, off, 0, AtP<T>(ds), dk, lane);
+    }
+    g = g1, i0 = i1;
+  };
+  if (q1 >= 0) {
+    const AtLoad<T, DP, 128, 4> vl(a.v_sl, a.d, wid, lane);
+    vl.issue(vb, kb0, a.lk, lds0, wid);
+    issue(0, 0, q0);
+    while (true) {
+      step(std::integral_constant<int, 0>{});
+      if (g >= a.group) break;
+      step(std::integral_constant<int, 1>{});
+      if (g >= a.group) break;
     }
   }
   float bad = 0.f;
@@ -321,7 +310,7 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
   for (unsigned todo = alone; todo; todo &= todo - 1) {
     const int j = kw0 + __builtin_ctz(todo);
     float gk[2], gv[2];
-    at_key_alone<T, CAP, SLOPE>(a, b, kh, j, r0, r1, lane, gk, gv);
+    at_key_alone<T, CAP, SLOPE>(a, b, kh, j, q0, q1, lane, gk, gv);
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       if (lane + 64 * e < a.d) {
@@ -333,9 +322,10 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
 
 template <typename T, int DF, bool CAP, bool SLOPE>
 __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, char* smem) {
-  constexpr int DP = AtPad<DF>::DP, KS = AtSteps<T, DF>::N, FD = DF / 32, KT = AtBwdTile<T>::KT;
-  constexpr int TILE = KT * DP * AtT<T>::E, STAGE = 2 * TILE;
-  int* range = (int*)(smem + 2 * STAGE);
+  typedef AtBwdLds<T, DF> L;
+  constexpr int DP = AtPad<DF>::DP, KS = AtOffsets<T, DF>::KS, FD = DF / 32, KT = L::KT;
+  constexpr int TILE = KT * L::RB, STAGE = 2 * TILE;
+  int* range = (int*)(smem + L::BYTES) - 8;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int b = bh / a.hk, kh = bh - b * a.hk, rows = a.lq * a.group;
   const int row = tile * 128 + wid * 32 + (lane & 31);
@@ -344,8 +334,9 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
   float lse = INFINITY, delta = 0.f;
   if (row < rows) {
     sp = at_span(a, b, pr.qi);
-    lse = a.lse[(long long)bh * rows + row];
-    delta = a.delta[(long long)bh * rows + row];
+    const long long r = ((long long)b * a.hq + pr.head) * a.lq + pr.qi;
+    lse = a.lse[r];
+    delta = a.rowws[r];
   }
   const bool live = sp.hi > sp.lo;
   const int w_lo = at_wave_min(live ? sp.lo : 0x7fffffff), w_hi = at_wave_max(live ? sp.hi : 0);
@@ -370,43 +361,53 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
     qf[ks] = live && e < a.d ? *(const uint4*)(qp + e) : make_uint4(0, 0, 0, 0);
     gf[ks] = live && e < a.d ? *(const uint4*)(gp + e) : make_uint4(0, 0, 0, 0);
   }
+  const AtLoad<T, DP, KT, 4> kl(a.k_sl, a.d, wid, lane), vl(a.v_sl, a.d, wid, lane);
   auto issue = [&](int stage, int k0) {
-    at_load_rows<T, DP, KT, 4>(kb, a.k_sl, k0, k_lo, k_hi, a.d, lds0 + stage * STAGE, wid, lane);
-    at_load_rows<T, DP, KT, 4>(vb, a.v_sl, k0, k_lo, k_hi, a.d, lds0 + stage * STAGE + TILE, wid, lane);
+    kl.issue(kb, k0, k_hi, lds0 + stage * STAGE, wid);
+    vl.issue(vb, k0, k_hi, lds0 + stage * STAGE + TILE, wid);
   };
-  const AtScore sc = at_score_of<T>(a, pr.head);
+  const float slope = SLOPE ? at_slope<T>(a, pr.head) : 0.f;
+  const AtOffsets<T, DF> off(lane);
   at_f32x16 dq[FD];
 #pragma unroll
   for (int f = 0; f < FD; ++f) dq[f] = at_zero();
   const int nt = k_hi > k_lo ? (k_hi - k_lo + KT - 1) / KT : 0;
-  if (nt > 0) issue(0, k_lo);
-  for (int t = 0; t < nt; ++t) {
+  auto step = [&](auto stage, int t) {
     const int k0 = k_lo + t * KT;
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (t + 1 < nt) issue((t + 1) & 1, k0 + KT);
-    if (k0 >= w_hi || k0 + KT <= w_lo) continue;
-    const char* K = smem + (t & 1) * STAGE;
+    if (t + 1 < nt) issue(1 - stage.value, k0 + KT);
+    if (k0 >= w_hi || k0 + KT <= w_lo) return;
+    const char* K = smem + stage.value * STAGE;
     const char* V = K + TILE;
     const bool part = k0 < i_lo || k0 + KT > i_hi;
-    const float x0 = (float)(sp.at - k0 - 4 * h);
 #pragma unroll
     for (int f = 0; f < KT / 32; ++f) {
       at_f32x16 s = at_zero(), dp = at_zero();
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        s = at_mfma<T>(at_row<T, DP>(K, 32 * f + (lane & 31), ks, h), qf[ks], s);
-        dp = at_mfma<T>(at_row<T, DP>(V, 32 * f + (lane & 31), ks, h), gf[ks], dp);
-      }
+      for (int ks = 0; ks < KS; ++ks) s = at_mfma<T>(at_row<T, DF>(K, off, 32 * f, ks), qf[ks], s);
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) dp = at_mfma<T>(at_row<T, DF>(V, off, 32 * f, ks), gf[ks], dp);
+      at_bend_tile<T, CAP>(a, s);
+      const float x0 = (float)(sp.at - k0 - 32 * f - 4 * h);
       float ds[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int c = 32 * f + 8 * (i >> 2) + (i & 3);
         float p;
-        at_grad<T, CAP, SLOPE>(sc, sc.slope_u, s[i], fabsf(x0 - (float)c), lse, dp[i], delta, p, ds[i]);
-        if (part && (k0 + c + 4 * h < sp.lo || k0 + c + 4 * h >= sp.hi)) ds[i] = 0.f;
+        at_grad<T, CAP, SLOPE>(a, slope, s[i], fabsf(x0 - (float)(8 * (i >> 2) + (i & 3))), lse, dp[i], delta, p, ds[i]);
       }
-      at_accumulate<T, DF>(K, 32 * f, ds, dq, lane);
+      if (part) {
+        const int lo = sp.lo - k0 - 32 * f - 4 * h, hi = sp.hi - k0 - 32 * f - 4 * h;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (8 * (i >> 2) + (i & 3) < lo || 8 * (i >> 2) + (i & 3) >= hi) ds[i] = 0.f;
+      }
+      at_accumulate<T, DF>(K, off, 32 * f, AtP<T>(ds), dq, lane);
     }
+  };
+  if (nt > 0) issue(0, k_lo);
+  for (int t = 0; t < nt; t += 2) {
+    step(std::integral_constant<int, 0>{}, t);
+    if (t + 1 < nt) step(std::integral_constant<int, 1>{}, t + 1);
   }
   float bad = 0.f;
 #pragma unroll
@@ -450,8 +451,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) k_mattn_bwd(AtArg
 
 template <typename T, int DF, bool CAP, bool SLOPE>
 static int mattn_bwd_df(const AtArgs& a, hipStream_t stream) {
-  constexpr int QT = AtBwdTile<T>::QT;
-  constexpr size_t LDS = 4 * QT * AtPad<DF>::DP * AtT<T>::E + 2 * sizeof(AtRowData<QT>) + 8 * sizeof(int);
+  constexpr size_t LDS = AtBwdLds<T, DF>::BYTES;
   const long long nbh = (long long)a.batch * a.hk;
   const long long blocks = nbh * (cdiv(a.lk, 128) + cdiv((long long)a.lq * a.group, 128));
   hipLaunchKernelGGL((k_mattn_bwd<T, DF, CAP, SLOPE>), dim3((unsigned)blocks), dim3(256), LDS, stream, a);
@@ -460,11 +460,12 @@ static int mattn_bwd_df(const AtArgs& a, hipStream_t stream) {
 }
 
 template <typename T>
-static int mattn_bwd_t(const AtArgs& a, hipStream_t stream) {
+static int mattn_bwd_t(AtArgs a, hipStream_t stream) {
+  at_score_args<T>(a);
   const long long n = (long long)a.batch * a.lq * a.hq;
   if (n > 0) {
-    hipLaunchKernelGGL((k_mattn_delta<T>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, stream, a);
-    DMF_LAUNCH_CHECK("dmf_mattn_bwd (delta)");
+    hipLaunchKernelGGL((k_mattn_rows<T>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, stream, a);
+    DMF_LAUNCH_CHECK("dmf_mattn_bwd (rows)");
   }
 #define DMF_AT_MODE(DF)                                                                                 \
   return a.cap > 0.f ? (a.slopes ? mattn_bwd_df<T, DF, true, true>(a, stream)                           \

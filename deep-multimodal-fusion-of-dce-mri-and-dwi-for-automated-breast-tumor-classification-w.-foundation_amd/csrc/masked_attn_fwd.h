@@ -17,6 +17,7 @@
 // costs nothing where the values are finite.
 #pragma once
 #include "masked_attn.h"
+#include <type_traits>
 
 namespace dmf {
 
@@ -24,7 +25,7 @@ namespace dmf {
 template <typename T, bool CAP, bool SLOPE>
 __device__ void at_row_alone(const AtArgs& a, const T* q, const T* k, const T* v, int lo, int hi, int at, int head,
                              int lane, float& m, float& l, float& o0, float& o1) {
-  const AtScore sc = at_score_of<T>(a, head);
+  const float slope = at_slope<T>(a, head);
   const float q0 = lane < a.d ? ld(q + lane) : 0.f, q1 = lane + 64 < a.d ? ld(q + lane + 64) : 0.f;
   m = -INFINITY;
   l = o0 = o1 = 0.f;
@@ -35,7 +36,7 @@ __device__ void at_row_alone(const AtArgs& a, const T* q, const T* k, const T* v
     if (lane < a.d) dot = q0 * ld(kj + lane);
     if (lane + 64 < a.d) dot = fmaf(q1, ld(kj + lane + 64), dot);
     dot = wave_sum(dot);
-    const float s = at_score<T, CAP, SLOPE>(sc, dot, fabsf((float)(at - j)));
+    const float s = at_score<T, CAP, SLOPE>(a.sc, slope, dot, fabsf((float)(at - j)));
     const float mn = fmaxf(m, s), ms = mn == -INFINITY ? 0.f : mn;
     const float alpha = at_exp<T>(m - ms), p = at_exp<T>(s - ms);
     m = mn;
@@ -52,12 +53,12 @@ __device__ __forceinline__ void at_store4(T* p, const float* v) {  // p aligned 
   if constexpr (sizeof(T) == 4)
     *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
   else
-    *(uint2*)p = make_uint2(B16<T>::pack(v[0], v[1]), B16<T>::pack(v[2], v[3]));
+    *(uint2*)p = make_uint2(AtPair<T>::pack(v[0], v[1]), AtPair<T>::pack(v[2], v[3]));
 }
 
 template <typename T, int DF, bool CAP, bool SLOPE, int NW, int KT>
-__global__ void __launch_bounds__(64 * NW, NW == 4 ? (sizeof(T) == 4 ? 1 : 2) : 1) k_mattn_fwd(AtArgs a) {
-  constexpr int DP = AtPad<DF>::DP, KS = AtSteps<T, DF>::N, FD = DF / 32, KF = KT / 32;
+__global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) k_mattn_fwd(AtArgs a) {
+  constexpr int DP = AtPad<DF>::DP, KS = AtOffsets<T, DF>::KS, FD = DF / 32, KF = KT / 32;
   constexpr int TILE = KT * DP * AtT<T>::E, STAGE = 2 * TILE;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ int range[2 * NW];
@@ -68,7 +69,8 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? (sizeof(T) == 4 ? 1 : 2) : 
   const int bh = blockIdx.x % nbh, tile = gridDim.x / nbh - 1 - blockIdx.x / nbh, split = blockIdx.y;
   const int b = bh / a.hk, kh = bh - b * a.hk;
   const int row = tile * 32 * NW + wid * 32 + (lane & 31);
-  const int qi = row < rows ? row / a.group : 0, head = kh * a.group + (row < rows ? row - qi * a.group : 0);
+  const AtRow pr = at_packed(a, kh, row < rows ? row : 0);
+  const int qi = pr.qi, head = pr.head;
   AtSpan sp = row < rows ? at_span(a, b, qi) : AtSpan{0, 0, 0};
   const bool live = sp.hi > sp.lo;
   // the wave's spans: union (w_lo, w_hi) and intersection (i_lo, i_hi) over the rows that see anything
@@ -91,7 +93,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? (sizeof(T) == 4 ? 1 : 2) : 
   const T* kb = (const T*)a.k + b * a.k_sb + kh * a.k_sh;
   const T* vb = (const T*)a.v + b * a.v_sb + kh * a.v_sh;
   const T* qb = (const T*)a.q + b * a.q_sb + (long long)qi * a.q_sl + head * a.q_sh;
-  const AtScore sc = at_score_of<T>(a, head);
+  const float slope = SLOPE ? at_slope<T>(a, head) : 0.f;
   const unsigned lds0 = (unsigned)(uintptr_t)((__attribute__((address_space(3))) char*)smem);
 
   uint4 qf[KS];
@@ -100,64 +102,92 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? (sizeof(T) == 4 ? 1 : 2) : 
     const int e = (2 * ks + h) * AtT<T>::CH;
     qf[ks] = live && e < a.d ? *(const uint4*)(qb + e) : make_uint4(0, 0, 0, 0);
   }
+  const AtLoad<T, DP, KT, NW> kl(a.k_sl, a.d, wid, lane), vl(a.v_sl, a.d, wid, lane);
   auto issue = [&](int stage, int k0) {
-    at_load_rows<T, DP, KT, NW>(kb, a.k_sl, k0, k_lo, k_hi, a.d, lds0 + stage * STAGE, wid, lane);
-    at_load_rows<T, DP, KT, NW>(vb, a.v_sl, k0, k_lo, k_hi, a.d, lds0 + stage * STAGE + TILE, wid, lane);
+    kl.issue(kb, k0, k_hi, lds0 + stage * STAGE, wid);
+    vl.issue(vb, k0, k_hi, lds0 + stage * STAGE + TILE, wid);
   };
 
   at_f32x16 acc[FD];
 #pragma unroll
   for (int f = 0; f < FD; ++f) acc[f] = at_zero();
-  float m = -INFINITY, ms = 0.f, l = 0.f;  // ms: m, or 0 while there is none
+  // ms: m, or 0 while there is none; l: the sum that o is divided by, of the probabilities as the products take them
+  // (rounded: then the rounding of a dominant key cancels); lx: the unrounded sum, for lse
+  float m = -INFINITY, ms = 0.f, l = 0.f, lx = 0.f;
   const int nt = k_hi > k_lo ? (k_hi - k_lo + KT - 1) / KT : 0;
-  if (nt > 0) issue(0, k_lo);
-  for (int t = 0; t < nt; ++t) {
+  const AtOffsets<T, DF> off(lane);
+  // plain 16-bit scores stay raw and are scaled in the exponent's FMA (scale > 0); others become s in units U in place
+  constexpr bool RAW = !(CAP || SLOPE || sizeof(T) == 4);
+  auto step = [&](auto stage, int t) {
     const int k0 = k_lo + t * KT;
     // this tile has landed (in every wave: the barrier); the other stage's last readers are past it too
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (t + 1 < nt) issue((t + 1) & 1, k0 + KT);
-    if (k0 >= w_hi || k0 + KT <= w_lo) continue;  // (wave-uniform) nothing here for these rows
-    const char* K = smem + (t & 1) * STAGE;
+    if (t + 1 < nt) issue(1 - stage.value, k0 + KT);
+    if (k0 >= w_hi || k0 + KT <= w_lo) return;  // (wave-uniform) nothing here for these rows
+    const char* K = smem + stage.value * STAGE;
     const char* V = K + TILE;
     at_f32x16 s[KF];
 #pragma unroll
     for (int f = 0; f < KF; ++f) {
       s[f] = at_zero();
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s[f] = at_mfma<T>(at_row<T, DP>(K, 32 * f + (lane & 31), ks, h), qf[ks], s[f]);
+      for (int ks = 0; ks < KS; ++ks) s[f] = at_mfma<T>(at_row<T, DF>(K, off, 32 * f, ks), qf[ks], s[f]);
     }
-    const float x0 = (float)(sp.at - k0 - 4 * h);  // position minus this lane's first key
-    if constexpr (CAP || SLOPE || sizeof(T) == 4) {
+    if constexpr (CAP && sizeof(T) == 2) {
+      float big = 0.f;
+#pragma unroll
+      for (int f = 0; f < KF; ++f)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(s[f][i]));
+      if (__any(big * a.sc.scale_cap > 1.f)) {
+#pragma unroll
+        for (int f = 0; f < KF; ++f)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[f][i] = at_bent<T, true, false>(a.sc, s[f][i]);
+      } else {
+#pragma unroll
+        for (int f = 0; f < KF; ++f)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[f][i] = at_bent<T, true, true>(a.sc, s[f][i]);
+      }
+    } else if constexpr (!RAW) {
+#pragma unroll
+      for (int f = 0; f < KF; ++f)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[f][i] = at_bent<T, CAP, false>(a.sc, s[f][i]);
+    }
+    if constexpr (SLOPE) {
+      const float x0 = (float)(sp.at - k0 - 4 * h);  // position minus this lane's first key
 #pragma unroll
       for (int f = 0; f < KF; ++f)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          s[f][i] = at_score<T, CAP, SLOPE>(sc, s[f][i], fabsf(x0 - (float)(32 * f + 8 * (i >> 2) + (i & 3))));
+          s[f][i] = fmaf(-slope, fabsf(x0 - (float)(32 * f + 8 * (i >> 2) + (i & 3))), s[f][i]);
     }
     if (k0 < i_lo || k0 + KT > i_hi) {  // (wave-uniform) some row does not see the whole tile
+      const int lo = sp.lo - k0 - 4 * h, hi = sp.hi - k0 - 4 * h;
 #pragma unroll
       for (int f = 0; f < KF; ++f)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int j = k0 + 32 * f + 8 * (i >> 2) + 4 * h + (i & 3);
-          if (j < sp.lo || j >= sp.hi) s[f][i] = -INFINITY;
+          const int j = 32 * f + 8 * (i >> 2) + (i & 3);
+          if (j < lo || j >= hi) s[f][i] = -INFINITY;
         }
     }
-    // scores in units U after at_score; plain 16-bit scores stay raw and are scaled in the exponent's FMA (scale > 0)
-    constexpr bool RAW = !(CAP || SLOPE || sizeof(T) == 4);
     float mt = -INFINITY;
 #pragma unroll
     for (int f = 0; f < KF; ++f)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[f][i]);
     mt = at_half_max(mt);
-    if (RAW) mt *= sc.scale_u;
+    if (RAW) mt *= a.sc.scale_u;
     if (__any(mt > m + 8.f * AtUnit<T>::U / AT_LOG2E)) {
       const float mn = fmaxf(m, mt);
       ms = mn == -INFINITY ? 0.f : mn;
       const float alpha = at_exp<T>(m - ms);
       m = mn;
       l *= alpha;
+      lx *= alpha;
 #pragma unroll
       for (int f = 0; f < FD; ++f) acc[f] *= alpha;
     }
@@ -165,15 +195,27 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? (sizeof(T) == 4 ? 1 : 2) : 
     for (int f = 0; f < KF; ++f) {
       float p[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        p[i] = RAW ? at_exp<T>(fmaf(s[f][i], sc.scale_u, -ms)) : at_exp<T>(s[f][i] - ms);
-        l += p[i];
+      for (int i = 0; i < 16; ++i) p[i] = at_exp<T>(RAW ? fmaf(s[f][i], a.sc.scale_u, -ms) : s[f][i] - ms);
+      // p is rounded to the 16-bit operand type: half a step, random in sign over the keys
+      const AtP<T> pk(p);
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) l = AtPair<T>::add(pk.w[i], l);
       }
-      // p is rounded to the 16-bit operand type (half a step, random in sign over the keys); l sums the unrounded ones
-      at_accumulate<T, DF>(V, 32 * f, p, acc, lane);
+      if (sizeof(T) == 4 || a.lse) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) lx += p[i];
+      }
+      at_accumulate<T, DF>(V, off, 32 * f, pk, acc, lane);
     }
+  };
+  if (nt > 0) issue(0, k_lo);
+  for (int t = 0; t < nt; t += 2) {
+    step(std::integral_constant<int, 0>{}, t);
+    if (t + 1 < nt) step(std::integral_constant<int, 1>{}, t + 1);
   }
-  l = at_half_sum(l);
+  lx = at_half_sum(lx);
+  l = sizeof(T) == 4 ? lx : at_half_sum(l);
   float bad = l * 0.f;
 #pragma unroll
   for (int f = 0; f < FD; ++f)
@@ -195,7 +237,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? (sizeof(T) == 4 ? 1 : 2) : 
           const int e = 32 * f + 8 * g + 4 * h;
           if (e < a.d) *(float4*)(po + e) = make_float4(acc[f][4 * g], acc[f][4 * g + 1], acc[f][4 * g + 2], acc[f][4 * g + 3]);
         }
-      if (h == 0) *(float2*)(a.pml + 2 * prow) = make_float2(m, l);
+      if (h == 0) *(float4*)(a.pml + 4 * prow) = make_float4(m, l, lx, 0.f);
     } else {
       const float inv = live ? 1.f / l : 0.f;
 #pragma unroll
@@ -214,7 +256,7 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? (sizeof(T) == 4 ? 1 : 2) : 
             at_store4(olo + e, v);
           }
         }
-      if (a.lse && h == 0) a.lse[(long long)bh * rows + row] = live ? ms + at_log<T>(l) : INFINITY;
+      if (a.lse && h == 0) a.lse[((long long)b * a.hq + head) * a.lq + qi] = live ? ms + at_log<T>(lx) : INFINITY;
     }
   }
   for (unsigned todo = alone; todo; todo &= todo - 1) {
@@ -243,46 +285,73 @@ __global__ void __launch_bounds__(64 * NW, NW == 4 ? (sizeof(T) == 4 ? 1 : 2) : 
     }
     if (lane == 0) {
       if (a.splits > 1)
-        *(float2*)(a.pml + 2 * pr) = make_float2(rm, rl);
+        *(float4*)(a.pml + 4 * pr) = make_float4(rm, rl, rl, 0.f);
       else if (a.lse)
-        a.lse[pr] = (rm == -INFINITY ? 0.f : rm) + at_log<T>(rl);
+        a.lse[((long long)b * a.hq + r_head) * a.lq + r_qi] = (rm == -INFINITY ? 0.f : rm) + at_log<T>(rl);
     }
   }
 }
 
 // o of one packed row from its splits: sum exp(m_s - m) O_s / sum exp(m_s - m) l_s over the splits its span touches.
-// One wave per row; lanes hold dims lane and lane + 64.
+// One workgroup per row: 8 groups of 32 lanes take every eighth split (four of its dims a lane), added up through LDS
+// in a fixed order.
 template <typename T>
-__global__ void __launch_bounds__(64) k_mattn_join(AtArgs a) {
-  const int lane = threadIdx.x, nbh = a.batch * a.hk, rows = a.lq * a.group;
+__global__ void __launch_bounds__(256) k_mattn_join(AtArgs a) {
+  __shared__ float4 part[8][32];
+  __shared__ float sums[8][2], red[4];
+  const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5, nbh = a.batch * a.hk, rows = a.lq * a.group;
   const int bh = blockIdx.x % nbh, row = blockIdx.x / nbh;
-  const int b = bh / a.hk, kh = bh - b * a.hk, qi = row / a.group, head = kh * a.group + row - qi * a.group;
+  const int b = bh / a.hk, kh = bh - b * a.hk;
+  const AtRow pr = at_packed(a, kh, row);
+  const int qi = pr.qi, head = pr.head;
   const AtSpan sp = at_span(a, b, qi);
   const bool live = sp.hi > sp.lo;
   const int s0 = sp.lo / a.chunk, s1 = live ? (sp.hi - 1) / a.chunk + 1 : s0;
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int s = s0 + lane; s < s1; s += 64) m = fmaxf(m, a.pml[2 * (((long long)s * nbh + bh) * rows + row)]);
+  const long long r0 = (long long)bh * rows + row, step = (long long)nbh * rows;
+  float m = -INFINITY;
+  for (int s = s0 + threadIdx.x; s < s1; s += 256) m = fmaxf(m, a.pml[4 * (s * step + r0)]);
   m = wave_max(m);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   const float ms = m == -INFINITY ? 0.f : m;
-  for (int s = s0; s < s1; ++s) {
-    const long long pr = ((long long)s * nbh + bh) * rows + row;
-    const float2 ml = *(const float2*)(a.pml + 2 * pr);
-    const float w = at_exp<T>(ml.x - ms);
+  const bool on = 4 * lane < a.d;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f, lx = 0.f;
+#pragma unroll 4
+  for (int s = s0 + grp; s < s1; s += 8) {
+    const long long pr = s * step + r0;
+    const float4 ml = *(const float4*)(a.pml + 4 * pr);
+    const float4 x = on ? *(const float4*)(a.po + pr * a.d + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
     // (a split whose keys are all -inf for this row has w = 0 and finite sums)
+    const float w = at_exp<T>(ml.x - ms);
     l = fmaf(w, ml.y, l);
-    if (lane < a.d) o0 = fmaf(w, a.po[pr * a.d + lane], o0);
-    if (lane + 64 < a.d) o1 = fmaf(w, a.po[pr * a.d + lane + 64], o1);
+    lx = fmaf(w, ml.z, lx);
+    o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
   }
-  const long long orow = (((long long)b * a.lq + qi) * a.hq + head) * a.d;
+  part[grp][lane] = o;
+  if (lane == 0) sums[grp][0] = l, sums[grp][1] = lx;
+  __syncthreads();
+  if (grp != 0) return;
+  l = lx = 0.f;
+  o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int e = lane + 64 * k;
-    const float o = live ? (k ? o1 : o0) / l : 0.f;
-    if (e >= a.d) continue;
-    st((T*)a.o + orow + e, o);
-    if (a.o_lo) st((T*)a.o_lo + orow + e, o - Cvt<T>::load(Cvt<T>::store(o)));
+  for (int g = 0; g < 8; ++g) {
+    const float4 x = part[g][lane];
+    o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+    l += sums[g][0], lx += sums[g][1];
   }
-  if (a.lse && lane == 0) a.lse[(long long)bh * rows + row] = live ? ms + at_log<T>(l) : INFINITY;
+  if (a.lse && lane == 0) a.lse[((long long)b * a.hq + head) * a.lq + qi] = live ? ms + at_log<T>(lx) : INFINITY;
+  if (!on) return;
+  const long long orow = (((long long)b * a.lq + qi) * a.hq + head) * a.d + 4 * lane;
+  const float inv = live ? 1.f / l : 0.f;
+  float v[4] = {live ? o.x * inv : 0.f, live ? o.y * inv : 0.f, live ? o.z * inv : 0.f, live ? o.w * inv : 0.f};
+  at_store4((T*)a.o + orow, v);
+  if (a.o_lo) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] -= Cvt<T>::load(Cvt<T>::store(v[r]));
+    at_store4((T*)a.o_lo + orow, v);
+  }
 }
 
 template <typename T, int DF, bool CAP, bool SLOPE>
@@ -301,7 +370,8 @@ static int mattn_fwd_df(const AtArgs& a, int nw, hipStream_t stream) {
 }
 
 template <typename T>
-static int mattn_fwd_t(const AtArgs& a, int nw, hipStream_t stream) {
+static int mattn_fwd_t(AtArgs a, int nw, hipStream_t stream) {
+  at_score_args<T>(a);
   int rc = 0;
 #define DMF_AT_MODE(DF)                                                                  \
   rc = a.cap > 0.f ? (a.slopes ? mattn_fwd_df<T, DF, true, true>(a, nw, stream)          \
@@ -315,7 +385,7 @@ static int mattn_fwd_t(const AtArgs& a, int nw, hipStream_t stream) {
 #undef DMF_AT_MODE
   if (rc) return rc;
   if (a.splits > 1) {
-    hipLaunchKernelGGL((k_mattn_join<T>), dim3((unsigned)((long long)a.lq * a.group * a.batch * a.hk)), dim3(64), 0,
+    hipLaunchKernelGGL((k_mattn_join<T>), dim3((unsigned)((long long)a.lq * a.group * a.batch * a.hk)), dim3(256), 0,
                        stream, a);
     DMF_LAUNCH_CHECK("dmf_mattn_fwd (join)");
   }

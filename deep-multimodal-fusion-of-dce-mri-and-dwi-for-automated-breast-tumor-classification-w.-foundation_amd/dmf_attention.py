@@ -248,9 +248,9 @@ class _AttentionFn(torch.autograd.Function):
         args, keep = _attn_dims(q, k, v, ctx.cfg, kv_lens, prefix, slopes, spans)
         go = _plain(go, 16)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        delta = torch.empty_like(lse)
+        ws = torch.empty(q.shape[0] * q.shape[1] * (q.shape[2] + 2), dtype=torch.float32, device=q.device)
         with _on(q):
-            N.call("dmf_mattn_bwd", *args, o.data_ptr(), _p(o_lo), lse.data_ptr(), go.data_ptr(), delta.data_ptr(),
+            N.call("dmf_mattn_bwd", *args, o.data_ptr(), _p(o_lo), lse.data_ptr(), go.data_ptr(), ws.data_ptr(),
                    dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), N.stream_ptr(q.device))
         del keep
         need = ctx.needs_input_grad

@@ -697,10 +697,11 @@ int dmf_qk_norm_rope_bwd(int dtype, const void* q, long long q_sb, long long q_s
  *   p = kv_len - lq + i (the queries are the last lq of the kv_len tokens); kv_lens [batch] (null: lk) is clamped to
  *   [0, lk]. causal: j <= p, and the first prefix[b] keys (null: 0) are seen by all. spans [batch][lq][2]
  *   (dmf_mattn_spans) takes the place of causal / prefix. A query that sees nothing has o = 0; keys that a query does not see
- *   do not reach its output, whatever they hold. d a multiple of 8 up to 128, strides and bases multiples of 16 bytes.
- *   For the backward: lse [batch][hk][lq][hq/hk] and, for 16-bit types, o_lo (what rounding o left over); both nullable.
+ *   do not reach its output, whatever they hold. d a multiple of 8 up to 128, strides and bases multiples of 16 bytes,
+ *   token strides at least d.
+ *   For the backward: lse [batch][hq][lq] and, for 16-bit types, o_lo (what rounding o left over); both nullable.
  *   ws: dmf_mattn_fwd_ws_floats floats (0: null allowed), where the keys are split over workgroups.
- * dmf_mattn_bwd: dq, dk, dv from go = d o; delta: batch*lq*hq floats of scratch. No atomics: same bits every run.
+ * dmf_mattn_bwd: dq, dk, dv from go = d o; ws: batch*lq*(hq + 2) floats of scratch. No atomics: same bits every run.
  * dmf_mattn_spans: spans of documents [batch] rows of doc_sb, lk ids each: a document is a maximal run of equal ids >= 0
  *   within kv_len; a query sees its document, under causal up to itself or the document's first prefix[b] tokens. */
 int dmf_mattn_spans(const int* documents, long long doc_sb, const int* kv_lens, const int* prefix, int batch, int lq,
@@ -715,7 +716,7 @@ int dmf_mattn_bwd(int dtype, const void* q, long long q_sb, long long q_sl, long
                   long long k_sb, long long k_sl, long long k_sh, const void* v, long long v_sb, long long v_sl,
                   long long v_sh, int batch, int lq, int lk, int hq, int hk, int d, float scale, float softcap,
                   const float* slopes, int causal, const int* kv_lens, const int* prefix, const int* spans,
-                  const void* o, const void* o_lo, const float* lse, const void* go, float* delta, void* dq, void* dk,
+                  const void* o, const void* o_lo, const float* lse, const void* go, float* ws, void* dq, void* dk,
                   void* dv, void* stream);
 
 /* ------------------------------------------------------------ optimizer

@@ -9,8 +9,8 @@ value, finfo.eps / 2; e = 2^-24: half a step of f32) and computed from the 64-bi
   what is below 2^-126, the smallest normal number of f32 and bf16: the same term with that value.
 * qk_norm_rope rounds once. y = rot(x r w): three products and one rotation sum in f32 (<= 8 e of
   |a cos| + |b sin|), r from a sum of d squares (its relative error <= (d + 4) e / 2 + 4 e), then u |y|.
-* attention. A score errs by D = (d + 4) e scale sum|q k| (an f32 sum of d products, scaled) plus, capped, 4 e cap for the
-  tanh of a 16-bit type (1 - 2 / (exp + 1): absolute) and plus 8 e |s| for its additions and the scaled exponent; p then
+* attention. A score errs by D = (d + 4) e scale sum|q k| (an f32 sum of d products, scaled) plus, capped, 10 e cap for the
+  tanh of a 16-bit type (its polynomial's minimax error is 5.9e-7 < 10 e; 1 - 2 / (exp + 1) is closer) and plus 8 e |s| for its additions and the scaled exponent; p then
   errs by a factor of 1 +- 2 max D (its own score's and the normaliser's) and 16-bit types round it by u for the
   products. So |o - ref| <= (2 max D + u + (n + 8) e) sum_j p|v| + u|o|, n the number of keys summed; the same for dv
   with do in place of v. ds = p (dp - delta) bend: dp and delta err by E = (d + 4) e sum|do||v| (max over the keys),
@@ -252,7 +252,7 @@ def _attn_ref(q, k, v, see, at, scale, cap, slopes, go):
     if cap:
         t = torch.tanh(z / cap)
         s, bend = cap * t, 1 - t * t
-        D = D + 4 * E * cap
+        D = D + 10 * E * cap
     if slopes is not None:
         far = (at.to(DEV)[:, None, :, None] - torch.arange(lk, device=DEV)).abs()
         s = s - slopes.double()[None, :, None, None] * far
