@@ -17,6 +17,8 @@
 // from LDS (ds_read_b64_tr_b16), takes the order 4 h + {0..3}, 8 + 4 h + {0..3} that the registers have. No shuffle and
 // no LDS round trip moves the probabilities.
 #pragma once
+#include <type_traits>
+
 #include "dmf_common.h"
 
 namespace dmf {
@@ -27,6 +29,7 @@ struct AtScore {
   float cap_u;      // cap * U
   float bend;       // -1 / cap_u^2
   float poly[6];    // cap * U * tanh(x) = raw * poly(raw^2) for |x| = |raw| scale / cap <= 1 (16-bit types)
+  float half[4];    // the same for |x| <= 0.5
 };
 
 struct AtArgs {
@@ -153,8 +156,10 @@ struct AtLoad {
   // rows r0 .. of base (row 0), valid below hi, to LDS address lds
   __device__ __forceinline__ void issue(const T* base, int r0, int hi, unsigned lds, int wid) const {
     const unsigned n = (unsigned)min(max(hi - r0, 0), ROWS);
-    const v4i_t rs = buf_rsrc((const char*)base + (unsigned long long)(unsigned)r0 * row_bytes,
-                              __builtin_amdgcn_readfirstlane(n * row_bytes));
+    const unsigned long long at = (unsigned long long)base + (unsigned long long)(unsigned)r0 * row_bytes;
+    // (wave-uniform by contract: readfirstlane keeps the descriptor in SGPRs where the compiler cannot prove it)
+    const v4i_t rs = {__builtin_amdgcn_readfirstlane((int)at), __builtin_amdgcn_readfirstlane((int)(at >> 32)),
+                      __builtin_amdgcn_readfirstlane((int)(n * row_bytes)), BUF_FLAGS};
 #pragma unroll
     for (int i = 0; i < PW; ++i)
       if (PIECES % NW == 0 || wid * PW + i < PIECES) dma16(rs, voff[i], 0, lds + (wid * PW + i) * 1024);
@@ -284,6 +289,33 @@ __device__ __forceinline__ AtRow at_packed(const AtArgs& a, int kh, int r) {
   return x;
 }
 
+// Union and intersection of the spans of packed rows r0 .. r0 + 31 that see anything, one lane pair per row (`sp`; dead
+// rows excluded), uniform over the wave. Spans by position only widen with the row, so the first and last row tell; document
+// spans are reduced over the lanes.
+struct AtBounds {
+  int lo, hi;      // union; hi 0: nothing
+  int i_lo, i_hi;  // intersection (by position: or less of it)
+};
+__device__ __forceinline__ int at_wave_min(int v);
+__device__ __forceinline__ int at_wave_max(int v);
+__device__ __forceinline__ AtBounds at_bounds(const AtArgs& a, int b, int kh, int r0, int rows, const AtSpan& sp) {
+  AtBounds w;
+  if (a.spans) {
+    const bool live = sp.hi > sp.lo;
+    w.lo = at_wave_min(live ? sp.lo : 0x7fffffff), w.hi = at_wave_max(live ? sp.hi : 0);
+    w.i_lo = at_wave_max(live ? sp.lo : 0), w.i_hi = at_wave_min(live ? sp.hi : 0x7fffffff);
+  } else if (r0 >= rows) {
+    w.lo = w.hi = w.i_lo = 0;
+    w.i_hi = 0x7fffffff;
+  } else {
+    const AtSpan first = at_span(a, b, at_packed(a, kh, r0).qi), last = at_span(a, b, at_packed(a, kh, min(r0 + 31, rows - 1)).qi);
+    w.lo = w.i_lo = 0;
+    w.hi = __builtin_amdgcn_readfirstlane(last.hi);
+    w.i_hi = __builtin_amdgcn_readfirstlane(max(first.hi, 1));  // (rows that see nothing come first, then 1, 2, .. keys)
+  }
+  return w;
+}
+
 // wave-wide minimum / maximum of an int
 __device__ __forceinline__ int at_wave_min(int v) {
 #pragma unroll
@@ -311,13 +343,15 @@ __device__ __forceinline__ float at_log(float x) {
 // CAP. The scores are bound by the vector ALU, and there by v_exp / v_rcp (a quarter of the rate): tanh as
 // 1 - 2 / (exp(2 x) + 1) takes two of them and four more operations. While no score of a tile exceeds the cap
 // (|x| <= 1, checked per wave and tile with half an operation a score), tanh(x) / x is a polynomial of degree 5 in x^2
-// instead: minimax, relative error 5.9e-7, no transcendental, and its coefficients carry scale and cap. Either form is off by
-// less than 10 * 2^-24 * cap, below the 16-bit rounding of the probabilities; f32 calls tanhf, since that would be several
-// f32 units of the exponent.
+// instead: minimax, relative error 5.9e-7, no transcendental, and its coefficients carry scale and cap; within half the
+// cap (|x| <= 0.5, where trained scores mostly are) degree 3 does, with 5.4e-07. Every form is off by less than
+// 10 * 2^-24 * cap, below the 16-bit rounding of the probabilities; f32 calls tanhf, since that would be several f32 units of
+// the exponent.
 template <typename T>
 inline void at_score_args(AtArgs& a) {
   static const double C[6] = {0.9999994039535522,    -0.3332904279232025,  0.13281433284282684,
                               -0.051605671644210815, 0.016743114218115807, -0.0030670599082022196};
+  static const double H[4] = {0.9999994557707791, -0.3332631793480118, 0.131902965910994, -0.0444022258055833};
   a.sc.scale_u = a.scale * AtUnit<T>::U;
   a.sc.scale_cap = a.cap > 0.f ? a.scale / a.cap : 0.f;
   a.sc.cap_u = a.cap * AtUnit<T>::U;
@@ -325,6 +359,7 @@ inline void at_score_args(AtArgs& a) {
   double x = a.sc.scale_cap;
   for (int i = 0; i < 6; ++i) {
     a.sc.poly[i] = (float)(C[i] * a.sc.cap_u * x);
+    if (i < 4) a.sc.half[i] = (float)(H[i] * a.sc.cap_u * x);
     x *= (double)a.sc.scale_cap * a.sc.scale_cap;
   }
 }
@@ -332,29 +367,65 @@ template <typename T>
 __device__ __forceinline__ float at_slope(const AtArgs& a, int head) {
   return a.slopes ? a.slopes[head] * AtUnit<T>::U : 0.f;
 }
-// cap tanh(z / cap), or z, in units U, of the raw product; SMALL: |raw| scale <= cap is known
-template <typename T, bool CAP, bool SMALL>
+// cap tanh(z / cap), or z, in units U, of the raw product; FORM: what is known of |x| = |raw| scale / cap
+enum { AT_ANY = 0, AT_ONE = 1, AT_HALF = 2 };
+template <int FORM>
+__device__ __forceinline__ float at_poly(const AtScore& c, float t) {  // of t = raw^2
+  if constexpr (FORM == AT_HALF) return fmaf(fmaf(fmaf(c.half[3], t, c.half[2]), t, c.half[1]), t, c.half[0]);
+  float p = fmaf(c.poly[5], t, c.poly[4]);
+  p = fmaf(p, t, c.poly[3]);
+  p = fmaf(p, t, c.poly[2]);
+  p = fmaf(p, t, c.poly[1]);
+  return fmaf(p, t, c.poly[0]);
+}
+template <typename T, bool CAP, int FORM>
 __device__ __forceinline__ float at_bent(const AtScore& c, float raw) {
   if constexpr (!CAP) {
     return raw * c.scale_u;
   } else if constexpr (sizeof(T) == 4) {
     return c.cap_u * tanhf(raw * c.scale_cap);
-  } else if constexpr (SMALL) {
-    const float t = raw * raw;
-    float p = fmaf(c.poly[5], t, c.poly[4]);
-    p = fmaf(p, t, c.poly[3]);
-    p = fmaf(p, t, c.poly[2]);
-    p = fmaf(p, t, c.poly[1]);
-    return raw * fmaf(p, t, c.poly[0]);
+  } else if constexpr (FORM != AT_ANY) {
+    return raw * at_poly<FORM>(c, raw * raw);
   } else {
     const float e = __builtin_amdgcn_exp2f(raw * (c.scale_cap * (2.f * AT_LOG2E))) + 1.f;
     return fmaf(-2.f * c.cap_u, __builtin_amdgcn_rcpf(e), c.cap_u);
   }
 }
+// calls f with the form that the wave's largest |x| allows (a NaN among them: it is NaN in every form)
+template <typename F>
+__device__ __forceinline__ void at_by_form(float x, F&& f) {
+  if (!__any(!(x <= 0.5f)))
+    f(std::integral_constant<int, AT_HALF>{});
+  else if (!__any(!(x <= 1.f)))
+    f(std::integral_constant<int, AT_ONE>{});
+  else
+    f(std::integral_constant<int, AT_ANY>{});
+}
+// raw products of N result tiles -> cap tanh(z / cap) or z in units U, in place, by the form that the whole wave's tile
+// allows
+template <typename T, bool CAP, int N>
+__device__ __forceinline__ void at_bend_tiles(const AtScore& c, at_f32x16* s) {
+  auto all = [&](auto form) {
+#pragma unroll
+    for (int f = 0; f < N; ++f)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[f][i] = at_bent<T, CAP, form.value>(c, s[f][i]);
+  };
+  if constexpr (CAP && sizeof(T) == 2) {
+    float big = 0.f;
+#pragma unroll
+    for (int f = 0; f < N; ++f)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(s[f][i]));
+    at_by_form(big * c.scale_cap, all);
+  } else {
+    all(std::integral_constant<int, AT_ANY>{});
+  }
+}
 // s (in units U) of one raw product; dist = |a - j|
 template <typename T, bool CAP, bool SLOPE>
 __device__ __forceinline__ float at_score(const AtScore& c, float slope_u, float raw, float dist) {
-  float s = at_bent<T, CAP, false>(c, raw);
+  float s = at_bent<T, CAP, AT_ANY>(c, raw);
   if constexpr (SLOPE) s = fmaf(-slope_u, dist, s);
   return s;
 }

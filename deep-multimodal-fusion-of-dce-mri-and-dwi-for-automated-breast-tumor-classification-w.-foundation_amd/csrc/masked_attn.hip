@@ -13,48 +13,69 @@ int mattn_bwd_f32(const AtArgs& a, hipStream_t stream);
 
 // Spans of a document mask: a document is a maximal run of equal ids >= 0 in the first kv_len positions; query i stands
 // at position p = kv_len - lq + i and sees its document, under `causal` only up to itself or the document's first
-// `prefix` tokens. One workgroup per batch row: each thread owns a stretch of positions, the run that enters it from
-// the left and the end that follows it on the right come from a scan of the threads' last / first run starts.
+// `prefix` tokens. One workgroup per 1024 positions and batch row: the run starts among them are bit masks (one ballot a
+// wave), a run that enters from the left or leaves to the right is followed 1024 positions at a time.
 __global__ void __launch_bounds__(1024) k_mattn_spans(const int* __restrict__ docs, long long doc_sb,
                                                       const int* kv_lens, const int* prefix, int lq, int lk, int causal,
                                                       int2* __restrict__ spans) {
-  __shared__ int left[1024], right[1024];
-  const int b = blockIdx.x, t = threadIdx.x;
+  __shared__ unsigned long long starts[16];
+  __shared__ int found[16];
+  const int b = blockIdx.y, t = threadIdx.x, lane = t & 63, wv = t >> 6;
   const int n = kv_lens ? min(max(kv_lens[b], 0), lk) : lk;
-  const int pre = prefix ? prefix[b] : 0, q0 = n - lq;  // position of query 0
+  const int q0 = n - lq;  // position of query 0
   const int* id = docs + b * doc_sb;
   int2* out = spans + (long long)b * lq;
-  const int per = (n + 1023) / 1024, j0 = min(n, t * per), j1 = min(n, j0 + per);
-  int first = n, last = -1;  // run starts within [j0, j1)
-  for (int j = j0; j < j1; ++j)
-    if (j == 0 || id[j] != id[j - 1]) {
-      if (last < 0) first = j;
-      last = j;
-    }
-  left[t] = last;
-  right[t] = first;
+  if (blockIdx.x == 0)  // queries before the first position
+    for (int i = t; i < min(lq, -q0); i += 1024) out[i] = make_int2(0, 0);
+  const long long base = (long long)blockIdx.x * 1024;
+  if (base >= n) return;
+  auto starts_at = [&](long long j) { return j == 0 || id[j] != id[j - 1]; };
+  // largest (sign 1) or smallest (sign -1) v * sign over the workgroup
+  auto most = [&](int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+    __syncthreads();
+    if (lane == 0) found[wv] = v;
+    __syncthreads();
+    int r = found[0];
+    for (int w = 1; w < 16; ++w) r = max(r, found[w]);
+    return r;
+  };
+  const int j = (int)base + t;
+  const bool in = j < n;
+  const unsigned long long mask = __ballot(in && starts_at(j));
+  if (lane == 0) starts[wv] = mask;
   __syncthreads();
-  for (int s = 1; s < 1024; s <<= 1) {
-    const int l = t >= s ? left[t - s] : -1, r = t + s < 1024 ? right[t + s] : n;
-    __syncthreads();
-    left[t] = max(left[t], l);
-    right[t] = min(right[t], r);
-    __syncthreads();
-  }
-  int start = t > 0 ? left[t - 1] : -1, end = t < 1023 ? right[t + 1] : n;
-  for (int j = j0; j < j1; ++j) {
-    if (j == 0 || id[j] != id[j - 1]) start = j;
-    if (j >= q0) out[j - q0].x = start;
-  }
-  for (int j = j1 - 1; j >= j0; --j) {
-    if (j >= q0) {
-      const int lo = out[j - q0].x;
-      const int hi = causal ? (int)min((long long)end, max((long long)j + 1, (long long)lo + max(pre, 0))) : end;
-      out[j - q0] = id[j] < 0 ? make_int2(0, 0) : make_int2(lo, hi);
+  int enter = -1, leave = 0x7fffffff;  // start of the run that enters the stretch; end of the one that leaves it
+  if (!(starts[0] & 1))
+    for (long long x = base - 1; x >= 0 && enter < 0; x -= 1024) enter = most(x - t >= 0 && starts_at(x - t) ? (int)(x - t) : -1);
+  const long long past = base + 1024;
+  if (past >= n)
+    leave = n;
+  else
+    for (long long x = past; leave == 0x7fffffff; x += 1024) {
+      const long long y = x + t;
+      leave = -most(y >= n ? -n : starts_at(y) ? -(int)y : (int)0x80000001);
     }
-    if (j == 0 || id[j] != id[j - 1]) end = j;
+  if (!in || j < q0) return;
+  int start = enter, end = leave;
+  for (int w = wv; w >= 0; --w) {
+    const unsigned long long m = w == wv ? starts[w] & (~0ull >> (63 - lane)) : starts[w];
+    if (m) {
+      start = (int)base + w * 64 + 63 - __builtin_clzll(m);
+      break;
+    }
   }
-  for (int i = t; i < min(lq, -q0); i += 1024) out[i] = make_int2(0, 0);  // queries before the first position
+  for (int w = wv; w < 16; ++w) {
+    const unsigned long long m = w == wv ? (lane == 63 ? 0ull : starts[w] & (~0ull << (lane + 1))) : starts[w];
+    if (m) {
+      end = (int)base + w * 64 + __builtin_ctzll(m);
+      break;
+    }
+  }
+  end = min(end, n);
+  if (causal) end = (int)min((long long)end, max((long long)j + 1, (long long)start + max(prefix ? prefix[b] : 0, 0)));
+  out[j - q0] = id[j] < 0 ? make_int2(0, 0) : make_int2(start, end);
 }
 
 struct AtPlan {
@@ -66,7 +87,10 @@ constexpr long long AT_FEW_BLOCKS = 4096, AT_BLOCKS = 512;
 static AtPlan at_plan(int batch, int lq, int lk, int hk, int group) {
   const long long rows = (long long)lq * group, nbh = (long long)batch * hk;
   AtPlan p;
-  p.nw = rows <= 32 ? 1 : 4;
+#ifndef X_NW8
+#define X_NW8 1024
+#endif
+  p.nw = rows <= 32 ? 1 : (rows + 255) / 256 * nbh >= X_NW8 ? 8 : 4;
   const long long blocks = ((rows + 32 * p.nw - 1) / (32 * p.nw)) * nbh;
   const long long want = p.nw == 1 ? AT_FEW_BLOCKS : AT_BLOCKS, least = p.nw == 1 ? 64 : 256;
   long long chunk = ((long long)lk * blocks + want - 1) / want;
@@ -74,6 +98,7 @@ static AtPlan at_plan(int batch, int lq, int lk, int hk, int group) {
   if (chunk < least) chunk = least;
   if (chunk * 32768 < lk) chunk = ((long long)lk / 32768 + 64) / 64 * 64;
   p.splits = (int)((lk + chunk - 1) / chunk);
+  if (nbh * p.splits >= (1LL << 31)) p.splits = 1;
   if (p.splits < 1 || blocks * 2 > want) p.splits = 1;
   p.chunk = p.splits > 1 ? (int)chunk : (lk > 0 ? lk : 1);
   return p;
@@ -88,7 +113,7 @@ static int at_check(const char* who, AtArgs& a, int dtype) {
   DMF_CHECK_ARG(a.cap >= 0.f && a.cap < INFINITY, "%s: softcap %g must be 0 (none) or positive", who, a.cap);
   DMF_CHECK_ARG(a.causal || !a.prefix, "%s: a prefix needs causal", who);
   const long long rows = (long long)a.lq * a.group, nbh = (long long)a.batch * a.hk;
-  DMF_CHECK_ARG(rows * a.group < (1LL << 31) && ((rows + 31) / 32 + (a.lk + 127) / 128 + 1) * (nbh + 1) < (1LL << 31),
+  DMF_CHECK_ARG(rows * a.group < (1LL << 31) && nbh < (1LL << 31) && (rows + 127) / 128 + (a.lk + 127LL) / 128 < 65536,
                 "%s: %d queries x %d heads x %d rows exceed the launch", who, a.lq, a.hq, a.batch);
   const int e = dtype == DMF_F32 ? 4 : 2;
   const long long st[] = {a.q_sb, a.q_sl, a.q_sh, a.k_sb, a.k_sl, a.k_sh, a.v_sb, a.v_sl, a.v_sh};
@@ -112,10 +137,10 @@ using namespace dmf;
 
 extern "C" int dmf_mattn_spans(const int* documents, long long doc_sb, const int* kv_lens, const int* prefix, int batch,
                                int lq, int lk, int causal, int* spans, void* stream) {
-  DMF_CHECK_ARG(batch >= 0 && lq >= 0 && lk >= 0, "dmf_mattn_spans: batch %d, lengths %d / %d", batch, lq, lk);
+  DMF_CHECK_ARG(batch >= 0 && batch < 65536 && lq >= 0 && lk >= 0, "dmf_mattn_spans: batch %d, lengths %d / %d", batch, lq, lk);
   if (batch == 0 || lq == 0) return 0;
   DMF_CHECK_ARG((documents || lk == 0) && spans && (uintptr_t)spans % 8 == 0, "dmf_mattn_spans: null operand");
-  hipLaunchKernelGGL(k_mattn_spans, dim3((unsigned)batch), dim3(1024), 0, (hipStream_t)stream, documents, doc_sb,
+  hipLaunchKernelGGL(k_mattn_spans, dim3((unsigned)cdiv(lk > 0 ? lk : 1, 1024), (unsigned)batch), dim3(1024), 0, (hipStream_t)stream, documents, doc_sb,
                      kv_lens, prefix, lq, lk, causal, (int2*)spans);
   DMF_LAUNCH_CHECK("dmf_mattn_spans");
   return 0;

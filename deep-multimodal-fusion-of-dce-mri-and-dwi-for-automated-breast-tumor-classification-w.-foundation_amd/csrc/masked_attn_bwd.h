@@ -5,8 +5,10 @@
 //   p_ij = exp(s_ij - lse_i),  dp_ij = do_i . v_j,  ds_ij = p_ij (dp_ij - delta_i) (1 - tanh^2(z_ij / cap))
 //   dv_j = sum_i p_ij do_i,  dk_j = scale sum_i ds_ij q_i,  dq_i = scale sum_j ds_ij k_j
 //
-// One launch holds two kinds of workgroups: those of 128 keys, which walk the packed query rows that see them and keep
-// dK and dV in registers, and those of 128 packed rows, which walk their keys and keep dQ. The scores are computed in
+// One launch holds two kinds of workgroups: those of 128 keys, which walk the queries that see them and keep dK and dV in
+// registers, and those of 128 (f32) or 256 packed rows, which walk their keys and keep dQ. The key workgroups' longest walk
+// (all queries of all heads of a group) decides how evenly a launch ends, so 16-bit types give each 128 keys two groups of
+// four waves that take the query tiles in turn and add up at the end. The scores are computed in
 // both (7 products for the 5 that one pass with dQ in atomics would take): no atomics, so the same bits every run, no
 // f32 dQ in HBM, and the sum over a group's query heads happens inside the dK / dV accumulators.
 #pragma once
@@ -63,26 +65,6 @@ __device__ __forceinline__ void at_grad(const AtArgs& a, float slope_u, float s,
   ds = p * (dp - delta);
   if constexpr (CAP) ds *= fmaf(s * s, a.sc.bend, 1.f);  // 1 - tanh^2
 }
-// raw products of one 32 x 32 tile -> s, with the polynomial where the whole wave's tile allows it
-template <typename T, bool CAP>
-__device__ __forceinline__ void at_bend_tile(const AtArgs& a, at_f32x16& s) {
-  if constexpr (CAP && sizeof(T) == 2) {
-    float big = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(s[i]));
-    if (__any(big * a.sc.scale_cap > 1.f)) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = at_bent<T, true, false>(a.sc, s[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = at_bent<T, true, true>(a.sc, s[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = at_bent<T, CAP, false>(a.sc, s[i]);
-  }
-}
-
 // LDS of the 128-key workgroups: their V tile, two stages of (Q, dO) tiles of 32 queries of one head, two of the rows'
 // values (one DMA instruction each, whose upper 32 lanes bring zeros). K stays in registers as the score's operand; V does
 // not fit there beside the two accumulators (192 registers) and is read from LDS for each dP.
@@ -93,10 +75,13 @@ struct AtRowData {
 constexpr int AT_QT = 32;
 template <typename T, int DF> struct AtBwdLds {
   static constexpr int RB = AtPad<DF>::DP * AtT<T>::E;
-  static constexpr int KT = sizeof(T) == 4 ? 32 : 64;       // keys per tile of the 128-row workgroups
+  static constexpr int NG = sizeof(T) == 4 ? 1 : 2;         // groups of four waves
+  static constexpr int KT = sizeof(T) == 4 ? 32 : 64;       // keys per tile of the row workgroups
   static constexpr int QTILE = AT_QT * RB, VT = 128 * RB;
-  static constexpr int KEYS = VT + 4 * QTILE + 2 * (int)sizeof(AtRowData), ROWS = 4 * KT * RB;
-  static constexpr int BYTES = (KEYS > ROWS ? KEYS : ROWS) + 8 * (int)sizeof(int);
+  static constexpr int GROUP = 4 * QTILE + 2 * (int)sizeof(AtRowData);  // a group's stages
+  static constexpr int KEYS = VT + NG * GROUP, ROWS = 4 * KT * RB, ADD = NG > 1 ? 4 * 64 * DF / 2 * 4 : 0;
+  static constexpr int MOST = KEYS > ROWS ? KEYS : ROWS;
+  static constexpr int BYTES = (MOST > ADD ? MOST : ADD) + 16 * (int)sizeof(int);
 };
 
 // dk, dv of one key over the queries in [q0, q1] that see it: each lane holds dims lane and lane + 64
@@ -119,7 +104,7 @@ __device__ void at_key_alone(const AtArgs& a, int b, int kh, int j, int q0, int 
     const float g0 = on0 ? ld(g + lane) : 0.f, g1 = on1 ? ld(g + lane + 64) : 0.f;
     const float raw = wave_sum(fmaf(x0, k0, x1 * k1)), dp = wave_sum(fmaf(g0, v0, g1 * v1));
     float p, ds;
-    at_grad<T, CAP, SLOPE>(a, at_slope<T>(a, head), at_bent<T, CAP, false>(a.sc, raw), fabsf((float)(sp.at - j)),
+    at_grad<T, CAP, SLOPE>(a, at_slope<T>(a, head), at_bent<T, CAP, AT_ANY>(a.sc, raw), fabsf((float)(sp.at - j)),
                            a.lse[rb], dp, a.rowws[rb], p, ds);
     dk[0] = fmaf(ds, x0, dk[0]), dk[1] = fmaf(ds, x1, dk[1]);
     dv[0] = fmaf(p, g0, dv[0]), dv[1] = fmaf(p, g1, dv[1]);
@@ -146,7 +131,7 @@ __device__ void at_query_alone(const AtArgs& a, int b, int kh, int r, int lo, in
     const float v0 = on0 ? ld(vj + lane) : 0.f, v1 = on1 ? ld(vj + lane + 64) : 0.f;
     const float raw = wave_sum(fmaf(q0, k0, q1 * k1)), dp = wave_sum(fmaf(g0, v0, g1 * v1));
     float p, ds;
-    at_grad<T, CAP, SLOPE>(a, slope, at_bent<T, CAP, false>(a.sc, raw), fabsf((float)(at - j)), lse, dp, delta, p, ds);
+    at_grad<T, CAP, SLOPE>(a, slope, at_bent<T, CAP, AT_ANY>(a.sc, raw), fabsf((float)(at - j)), lse, dp, delta, p, ds);
     dq[0] = fmaf(ds, k0, dq[0]), dq[1] = fmaf(ds, k1, dq[1]);
   }
 }
@@ -171,8 +156,10 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
   typedef AtBwdLds<T, DF> L;
   constexpr int DP = AtPad<DF>::DP, KS = AtOffsets<T, DF>::KS, FD = DF / 32;
   constexpr int TILE = L::QTILE, STAGE = 2 * TILE;
-  int* range = (int*)(smem + L::BYTES) - 8;
-  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  constexpr int NG = L::NG;
+  int* range = (int*)(smem + L::BYTES) - 16;
+  const int lane = threadIdx.x & 63, w8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int wid = w8 & 3, grp = w8 >> 2;  // 32 keys; which of the query tiles
   const int b = bh / a.hk, kh = bh - b * a.hk;
   const int kb0 = ktile * 128, kw0 = kb0 + 32 * wid, key = kw0 + (lane & 31);
   const unsigned lds0 = (unsigned)(uintptr_t)((__attribute__((address_space(3))) char*)smem);
@@ -184,26 +171,26 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
   const int* w_lo = (const int*)a.rowws + nrows + (long long)b * a.lq;
   const int* w_hi = w_lo + nq;
   int q0 = 0x7fffffff, q1 = -1;
-  for (int i = threadIdx.x; i < a.lq; i += 1024) {
+  for (int i = threadIdx.x; i < a.lq; i += 1024 * NG) {
     int lo[4], hi[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int r = min(i + 256 * u, a.lq - 1);
+      const int r = min(i + 256 * NG * u, a.lq - 1);
       lo[u] = w_lo[r];
       hi[u] = w_hi[r];
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (i + 256 * u < a.lq && hi[u] > kb0 && lo[u] < kb0 + 128) {
-        q0 = min(q0, i + 256 * u);
-        q1 = max(q1, i + 256 * u);
+      if (i + 256 * NG * u < a.lq && hi[u] > kb0 && lo[u] < kb0 + 128) {
+        q0 = min(q0, i + 256 * NG * u);
+        q1 = max(q1, i + 256 * NG * u);
       }
   }
   q0 = at_wave_min(q0), q1 = at_wave_max(q1);
-  if (lane == 0) range[wid] = q0, range[4 + wid] = q1;
+  if (lane == 0) range[w8] = q0, range[8 + w8] = q1;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 4; ++w) q0 = min(q0, range[w]), q1 = max(q1, range[4 + w]);
+  for (int w = 0; w < 4 * NG; ++w) q0 = min(q0, range[w]), q1 = max(q1, range[8 + w]);
   q0 = __builtin_amdgcn_readfirstlane(q0);
   q1 = __builtin_amdgcn_readfirstlane(q1);
 
@@ -219,13 +206,13 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
   const long long rv0 = wid < 2 ? ((long long)b * a.hq + kh * a.group) * a.lq : 0, rvh = wid < 2 ? a.lq : 0;
   const unsigned rvo = lane < AT_QT ? (unsigned)lane * 4 : BUF_OOB;
   auto issue = [&](int stage, int g, int i0) {
-    const unsigned S = lds0 + L::VT + stage * STAGE;
+    const unsigned S = lds0 + L::VT + grp * L::GROUP + stage * STAGE;
     const int head = kh * a.group + g;
     ql.issue((const T*)a.q + b * a.q_sb + head * a.q_sh, i0, q1 + 1, S, wid);
     gl.issue((const T*)a.go + ((long long)b * a.lq * a.hq + head) * a.d, i0, q1 + 1, S + TILE, wid);
     // queries past the last arrive as zeros: an empty span
     at_dma4(buf_rsrc(rv + rv0 + g * rvh + i0, __builtin_amdgcn_readfirstlane(min(q1 + 1 - i0, AT_QT) * 4)), rvo,
-            lds0 + L::VT + 2 * STAGE + stage * (unsigned)sizeof(AtRowData) + wid * 256);
+            lds0 + L::VT + grp * L::GROUP + 2 * STAGE + stage * (unsigned)sizeof(AtRowData) + wid * 256);
   };
 
   at_f32x16 dk[FD], dv[FD];
@@ -234,24 +221,32 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
   const AtOffsets<T, DF> off(lane);
   const char* V = smem + wid * 32 * L::RB;
   const int n0 = (at_keys(a, b)) - a.lq;  // position of query 0
-  int g = 0, i0 = q0;                          // the tile in hand: head, first query
+  // tiles of 32 queries, head after head; the groups take them in turn
+  int g = 0, i0 = q0;  // the tile in hand: head (a.group or more: none), first query
+  auto advance = [&](int n, int& hd, int& i) {
+    for (; n > 0; --n) {
+      i += AT_QT;
+      if (i > q1) i = q0, ++hd;
+    }
+  };
+  const char* const base = smem + L::VT + grp * L::GROUP;
   auto step = [&](auto stage) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    int g1 = g, i1 = i0 + AT_QT;  // the next one
-    if (i1 > q1) i1 = q0, ++g1;
+    int g1 = g, i1 = i0;  // the next one
+    advance(NG, g1, i1);
     if (g1 < a.group) issue(1 - stage.value, g1, i1);
-    const char* Q = smem + L::VT + stage.value * STAGE;
+    const char* Q = base + stage.value * STAGE;
     const char* G = Q + TILE;
-    const AtRowData& x = *(const AtRowData*)(smem + L::VT + 2 * STAGE + stage.value * (int)sizeof(AtRowData));
+    const AtRowData& x = *(const AtRowData*)(base + 2 * STAGE + stage.value * (int)sizeof(AtRowData));
     const int f_lo = x.lo[lane & 31], f_hi = x.hi[lane & 31];
-    if (__any(f_hi > kw0 && f_lo < kw0 + 32)) {                     // some row sees some of this wave's keys
+    if (g < a.group && __any(f_hi > kw0 && f_lo < kw0 + 32)) {      // some row sees some of this wave's keys
       const bool full = __all(f_lo <= kw0 && f_hi >= kw0 + 32);     // every row sees all of them
       at_f32x16 s = at_zero(), dp = at_zero();
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) s = at_mfma<T>(at_row<T, DF>(Q, off, 0, ks), kf[ks], s);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) dp = at_mfma<T>(at_row<T, DF>(G, off, 0, ks), at_row<T, DF>(V, off, 0, ks), dp);
-      at_bend_tile<T, CAP>(a, s);
+      at_bend_tiles<T, CAP, 1>(a.sc, &s);
       const float slope = SLOPE ? at_slope<T>(a, kh * a.group + g) : 0.f;
       const float x0 = (float)(n0 + i0 + 4 * h - key);  // position of this lane's first row minus its key
       float p[16], ds[16];
@@ -285,15 +280,38 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
     g = g1, i0 = i1;
   };
   if (q1 >= 0) {
-    const AtLoad<T, DP, 128, 4> vl(a.v_sl, a.d, wid, lane);
-    vl.issue(vb, kb0, a.lk, lds0, wid);
-    issue(0, 0, q0);
-    while (true) {
+    const AtLoad<T, DP, 128, 4 * NG> vl(a.v_sl, a.d, w8, lane);
+    vl.issue(vb, kb0, a.lk, lds0, w8);
+    advance(grp, g, i0);
+    if (g < a.group) issue(0, g, i0);
+    // (uniform over the workgroup: the first group's count)
+    const int nt = (a.group * ((q1 - q0) / AT_QT + 1) + NG - 1) / NG;
+    for (int t = 0; t < nt; t += 2) {
       step(std::integral_constant<int, 0>{});
-      if (g >= a.group) break;
-      step(std::integral_constant<int, 1>{});
-      if (g >= a.group) break;
+      if (t + 1 < nt) step(std::integral_constant<int, 1>{});
     }
+  }
+  if constexpr (NG > 1) {  // the second group's sums through LDS, in two halves
+    float* sum = (float*)smem + wid * 64 * (DF / 2) + lane;
+    auto add = [&](at_f32x16* acc) {
+      __syncthreads();
+      if (grp == 1) {
+#pragma unroll
+        for (int f = 0; f < FD; ++f)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sum[(16 * f + i) * 64] = acc[f][i];
+      }
+      __syncthreads();
+      if (grp == 0) {
+#pragma unroll
+        for (int f = 0; f < FD; ++f)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[f][i] += sum[(16 * f + i) * 64];
+      }
+    };
+    add(dk);
+    add(dv);
+    if (grp == 1) return;
   }
   float bad = 0.f;
 #pragma unroll
@@ -325,10 +343,11 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
   typedef AtBwdLds<T, DF> L;
   constexpr int DP = AtPad<DF>::DP, KS = AtOffsets<T, DF>::KS, FD = DF / 32, KT = L::KT;
   constexpr int TILE = KT * L::RB, STAGE = 2 * TILE;
-  int* range = (int*)(smem + L::BYTES) - 8;
+  constexpr int NW = 4 * L::NG;
+  int* range = (int*)(smem + L::BYTES) - 16;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int b = bh / a.hk, kh = bh - b * a.hk, rows = a.lq * a.group;
-  const int row = tile * 128 + wid * 32 + (lane & 31);
+  const int row = tile * 32 * NW + wid * 32 + (lane & 31);
   const AtRow pr = at_packed(a, kh, row < rows ? row : 0);
   AtSpan sp = {0, 0, 0};
   float lse = INFINITY, delta = 0.f;
@@ -339,15 +358,20 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
     delta = a.rowws[r];
   }
   const bool live = sp.hi > sp.lo;
-  const int w_lo = at_wave_min(live ? sp.lo : 0x7fffffff), w_hi = at_wave_max(live ? sp.hi : 0);
-  const int i_lo = at_wave_max(live ? sp.lo : 0), i_hi = at_wave_min(live ? sp.hi : 0x7fffffff);
+  const AtBounds w = at_bounds(a, b, kh, tile * 32 * NW + wid * 32, rows, sp);
+  const int w_lo = w.lo, w_hi = w.hi, i_lo = w.i_lo, i_hi = w.i_hi;
   int k_lo = w_lo, k_hi = w_hi;
-  if (lane == 0) range[wid] = w_lo, range[4 + wid] = w_hi;
-  __syncthreads();
+  if (a.spans) {
+    if (lane == 0) range[wid] = w_lo, range[8 + wid] = w_hi;
+    __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 4; ++w) k_lo = min(k_lo, range[w]), k_hi = max(k_hi, range[4 + w]);
-  k_lo = __builtin_amdgcn_readfirstlane(k_lo);
-  k_hi = __builtin_amdgcn_readfirstlane(k_hi);
+    for (int i = 0; i < NW; ++i) k_lo = min(k_lo, range[i]), k_hi = max(k_hi, range[8 + i]);
+    k_lo = __builtin_amdgcn_readfirstlane(k_lo);
+    k_hi = __builtin_amdgcn_readfirstlane(k_hi);
+  } else {
+    k_lo = 0;
+    k_hi = __builtin_amdgcn_readfirstlane(max(at_span(a, b, at_packed(a, kh, min(tile * 32 * NW + 32 * NW, rows) - 1).qi).hi, 0));
+  }
   const unsigned lds0 = (unsigned)(uintptr_t)((__attribute__((address_space(3))) char*)smem);
   const T* kb = (const T*)a.k + b * a.k_sb + kh * a.k_sh;
   const T* vb = (const T*)a.v + b * a.v_sb + kh * a.v_sh;
@@ -361,7 +385,7 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
     qf[ks] = live && e < a.d ? *(const uint4*)(qp + e) : make_uint4(0, 0, 0, 0);
     gf[ks] = live && e < a.d ? *(const uint4*)(gp + e) : make_uint4(0, 0, 0, 0);
   }
-  const AtLoad<T, DP, KT, 4> kl(a.k_sl, a.d, wid, lane), vl(a.v_sl, a.d, wid, lane);
+  const AtLoad<T, DP, KT, NW> kl(a.k_sl, a.d, wid, lane), vl(a.v_sl, a.d, wid, lane);
   auto issue = [&](int stage, int k0) {
     kl.issue(kb, k0, k_hi, lds0 + stage * STAGE, wid);
     vl.issue(vb, k0, k_hi, lds0 + stage * STAGE + TILE, wid);
@@ -387,7 +411,7 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
       for (int ks = 0; ks < KS; ++ks) s = at_mfma<T>(at_row<T, DF>(K, off, 32 * f, ks), qf[ks], s);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) dp = at_mfma<T>(at_row<T, DF>(V, off, 32 * f, ks), gf[ks], dp);
-      at_bend_tile<T, CAP>(a, s);
+      at_bend_tiles<T, CAP, 1>(a.sc, &s);
       const float x0 = (float)(sp.at - k0 - 32 * f - 4 * h);
       float ds[16];
 #pragma unroll
@@ -436,25 +460,23 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
   }
 }
 
-// workgroups [0, nk): 128 keys each (the longer ones: they start first); [nk, ..): 128 packed rows each
+// blockIdx.y first counts the workgroups of 128 keys (the longer ones; the first keys are seen by most queries), then those
+// of 128 NG packed rows, the last rows first; heads vary fastest, as in the forward
 template <typename T, int DF, bool CAP, bool SLOPE>
-__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 1 : 2) k_mattn_bwd(AtArgs a) {
+__global__ void __launch_bounds__(256 * (sizeof(T) == 4 ? 1 : 2), sizeof(T) == 4 ? 1 : 2) k_mattn_bwd(AtArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int nbh = a.batch * a.hk;
-  const int ktiles = (a.lk + 127) / 128, rtiles = gridDim.x / nbh - ktiles;
-  const int bh = blockIdx.x % nbh, t = blockIdx.x / nbh;
+  const int ktiles = (a.lk + 127) / 128, t = blockIdx.y;
   if (t < ktiles)
-    at_bwd_keys<T, DF, CAP, SLOPE>(a, bh, t, smem);
+    at_bwd_keys<T, DF, CAP, SLOPE>(a, blockIdx.x, t, smem);
   else
-    at_bwd_rows<T, DF, CAP, SLOPE>(a, bh, rtiles - 1 - (t - ktiles), smem);
+    at_bwd_rows<T, DF, CAP, SLOPE>(a, blockIdx.x, gridDim.y - 1 - t, smem);
 }
 
 template <typename T, int DF, bool CAP, bool SLOPE>
 static int mattn_bwd_df(const AtArgs& a, hipStream_t stream) {
   constexpr size_t LDS = AtBwdLds<T, DF>::BYTES;
-  const long long nbh = (long long)a.batch * a.hk;
-  const long long blocks = nbh * (cdiv(a.lk, 128) + cdiv((long long)a.lq * a.group, 128));
-  hipLaunchKernelGGL((k_mattn_bwd<T, DF, CAP, SLOPE>), dim3((unsigned)blocks), dim3(256), LDS, stream, a);
+  const dim3 grid((unsigned)(a.batch * a.hk), (unsigned)(cdiv(a.lk, 128) + cdiv((long long)a.lq * a.group, 128 * AtBwdLds<T, DF>::NG)));
+  hipLaunchKernelGGL((k_mattn_bwd<T, DF, CAP, SLOPE>), grid, dim3(256 * AtBwdLds<T, DF>::NG), LDS, stream, a);
   DMF_LAUNCH_CHECK("dmf_mattn_bwd");
   return 0;
 }

@@ -17,7 +17,6 @@
 // costs nothing where the values are finite.
 #pragma once
 #include "masked_attn.h"
-#include <type_traits>
 
 namespace dmf {
 
@@ -64,26 +63,32 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) k_mattn_fwd(A
   __shared__ int range[2 * NW];
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int nbh = a.batch * a.hk, rows = a.lq * a.group;
-  // key heads vary fastest (their tiles of one row block go to different XCDs, each XCD keeps its heads' K / V in
-  // its L2); the last row blocks, the longest under a causal mask, start first
-  const int bh = blockIdx.x % nbh, tile = gridDim.x / nbh - 1 - blockIdx.x / nbh, split = blockIdx.y;
+  // Workgroups go to the eight XCDs in turn: splits, then heads vary fastest, so that an XCD gets a share of every batch
+  // row (ragged lengths) and row block, and the last row blocks, the longest under a causal mask, start first.
+  const int bh = a.splits > 1 ? blockIdx.x / a.splits : blockIdx.x, split = blockIdx.x - bh * a.splits;
+  const int tile = gridDim.y - 1 - blockIdx.y;
   const int b = bh / a.hk, kh = bh - b * a.hk;
   const int row = tile * 32 * NW + wid * 32 + (lane & 31);
   const AtRow pr = at_packed(a, kh, row < rows ? row : 0);
   const int qi = pr.qi, head = pr.head;
   AtSpan sp = row < rows ? at_span(a, b, qi) : AtSpan{0, 0, 0};
   const bool live = sp.hi > sp.lo;
-  // the wave's spans: union (w_lo, w_hi) and intersection (i_lo, i_hi) over the rows that see anything
-  const int w_lo = at_wave_min(live ? sp.lo : 0x7fffffff), w_hi = at_wave_max(live ? sp.hi : 0);
-  const int i_lo = at_wave_max(live ? sp.lo : 0), i_hi = at_wave_min(live ? sp.hi : 0x7fffffff);
+  const AtBounds w = at_bounds(a, b, kh, tile * 32 * NW + wid * 32, rows, sp);
+  const int w_lo = w.lo, w_hi = w.hi, i_lo = w.i_lo, i_hi = w.i_hi;
   int k_lo = w_lo, k_hi = w_hi;
   if constexpr (NW > 1) {
-    if (lane == 0) range[wid] = w_lo, range[NW + wid] = w_hi;
-    __syncthreads();
+    if (a.spans) {
+      if (lane == 0) range[wid] = w_lo, range[NW + wid] = w_hi;
+      __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; ++w) k_lo = min(k_lo, range[w]), k_hi = max(k_hi, range[NW + w]);
-    k_lo = __builtin_amdgcn_readfirstlane(k_lo);
-    k_hi = __builtin_amdgcn_readfirstlane(k_hi);
+      for (int i = 0; i < NW; ++i) k_lo = min(k_lo, range[i]), k_hi = max(k_hi, range[NW + i]);
+      k_lo = __builtin_amdgcn_readfirstlane(k_lo);
+      k_hi = __builtin_amdgcn_readfirstlane(k_hi);
+    } else {
+      k_lo = 0;
+      k_hi = __builtin_amdgcn_readfirstlane(
+          max(at_span(a, b, at_packed(a, kh, min(tile * 32 * NW + 32 * NW, rows) - 1).qi).hi, 0));
+    }
   }
   if (a.splits > 1) {
     k_lo = max(k_lo, split * a.chunk);
@@ -96,28 +101,31 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) k_mattn_fwd(A
   const float slope = SLOPE ? at_slope<T>(a, head) : 0.f;
   const unsigned lds0 = (unsigned)(uintptr_t)((__attribute__((address_space(3))) char*)smem);
 
+  const AtLoad<T, DP, KT, NW> kl(a.k_sl, a.d, wid, lane), vl(a.v_sl, a.d, wid, lane);
+  auto issue = [&](int stage, int k0) {
+    kl.issue(kb, k0, k_hi, lds0 + stage * STAGE, wid);
+    vl.issue(vb, k0, k_hi, lds0 + stage * STAGE + TILE, wid);
+  };
+  const int nt = k_hi > k_lo ? (k_hi - k_lo + KT - 1) / KT : 0;
+  if (nt > 0) issue(0, k_lo);  // (first: the rest of the set-up runs under its latency)
   uint4 qf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
     const int e = (2 * ks + h) * AtT<T>::CH;
     qf[ks] = live && e < a.d ? *(const uint4*)(qb + e) : make_uint4(0, 0, 0, 0);
   }
-  const AtLoad<T, DP, KT, NW> kl(a.k_sl, a.d, wid, lane), vl(a.v_sl, a.d, wid, lane);
-  auto issue = [&](int stage, int k0) {
-    kl.issue(kb, k0, k_hi, lds0 + stage * STAGE, wid);
-    vl.issue(vb, k0, k_hi, lds0 + stage * STAGE + TILE, wid);
-  };
-
   at_f32x16 acc[FD];
 #pragma unroll
   for (int f = 0; f < FD; ++f) acc[f] = at_zero();
   // ms: m, or 0 while there is none; l: the sum that o is divided by, of the probabilities as the products take them
   // (rounded: then the rounding of a dominant key cancels); lx: the unrounded sum, for lse
   float m = -INFINITY, ms = 0.f, l = 0.f, lx = 0.f;
-  const int nt = k_hi > k_lo ? (k_hi - k_lo + KT - 1) / KT : 0;
   const AtOffsets<T, DF> off(lane);
   // plain 16-bit scores stay raw and are scaled in the exponent's FMA (scale > 0); others become s in units U in place
   constexpr bool RAW = !(CAP || SLOPE || sizeof(T) == 4);
+  // capped 16-bit scores without a bias stay raw too: tanh does not change their order, so the maximum is taken of the raw
+  // products and bent alone
+  constexpr bool LATE = CAP && !SLOPE && sizeof(T) == 2;
   auto step = [&](auto stage, int t) {
     const int k0 = k_lo + t * KT;
     // this tile has landed (in every wave: the barrier); the other stage's last readers are past it too
@@ -133,29 +141,7 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) k_mattn_fwd(A
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) s[f] = at_mfma<T>(at_row<T, DF>(K, off, 32 * f, ks), qf[ks], s[f]);
     }
-    if constexpr (CAP && sizeof(T) == 2) {
-      float big = 0.f;
-#pragma unroll
-      for (int f = 0; f < KF; ++f)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(s[f][i]));
-      if (__any(big * a.sc.scale_cap > 1.f)) {
-#pragma unroll
-        for (int f = 0; f < KF; ++f)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[f][i] = at_bent<T, true, false>(a.sc, s[f][i]);
-      } else {
-#pragma unroll
-        for (int f = 0; f < KF; ++f)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[f][i] = at_bent<T, true, true>(a.sc, s[f][i]);
-      }
-    } else if constexpr (!RAW) {
-#pragma unroll
-      for (int f = 0; f < KF; ++f)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[f][i] = at_bent<T, CAP, false>(a.sc, s[f][i]);
-    }
+    if constexpr (SLOPE || (!RAW && !LATE)) at_bend_tiles<T, CAP, KF>(a.sc, s);
     if constexpr (SLOPE) {
       const float x0 = (float)(sp.at - k0 - 4 * h);  // position minus this lane's first key
 #pragma unroll
@@ -164,23 +150,34 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) k_mattn_fwd(A
         for (int i = 0; i < 16; ++i)
           s[f][i] = fmaf(-slope, fabsf(x0 - (float)(32 * f + 8 * (i >> 2) + (i & 3))), s[f][i]);
     }
-    if (k0 < i_lo || k0 + KT > i_hi) {  // (wave-uniform) some row does not see the whole tile
-      const int lo = sp.lo - k0 - 4 * h, hi = sp.hi - k0 - 4 * h;
+    const bool part = k0 < i_lo || k0 + KT > i_hi;  // (wave-uniform) some row does not see the whole tile
+    const int lo = sp.lo - k0 - 4 * h, hi = sp.hi - k0 - 4 * h;
+    float big = 0.f, mt = -INFINITY;
+    if constexpr (LATE) {
+#pragma unroll
+      for (int f = 0; f < KF; ++f)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(s[f][i]));
+    }
+    if (part) {
 #pragma unroll
       for (int f = 0; f < KF; ++f)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int j = 32 * f + 8 * (i >> 2) + (i & 3);
-          if (j < lo || j >= hi) s[f][i] = -INFINITY;
+          const float x = j < lo || j >= hi ? -INFINITY : s[f][i];
+          if constexpr (!LATE) s[f][i] = x;
+          mt = fmaxf(mt, x);
         }
+    } else {
+#pragma unroll
+      for (int f = 0; f < KF; ++f)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[f][i]);
     }
-    float mt = -INFINITY;
-#pragma unroll
-    for (int f = 0; f < KF; ++f)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[f][i]);
     mt = at_half_max(mt);
     if (RAW) mt *= a.sc.scale_u;
+    if (LATE) mt = mt == -INFINITY ? mt : at_bent<T, CAP, AT_ANY>(a.sc, mt);
     if (__any(mt > m + 8.f * AtUnit<T>::U / AT_LOG2E)) {
       const float mn = fmaxf(m, mt);
       ms = mn == -INFINITY ? 0.f : mn;
@@ -191,11 +188,38 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) k_mattn_fwd(A
 #pragma unroll
       for (int f = 0; f < FD; ++f) acc[f] *= alpha;
     }
+    if constexpr (LATE) {
+      at_by_form(big * a.sc.scale_cap, [&](auto form) {
+#pragma unroll
+        for (int f = 0; f < KF; ++f)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if constexpr (form.value == AT_ANY)
+              s[f][i] = at_exp<T>(at_bent<T, CAP, AT_ANY>(a.sc, s[f][i]) - ms);
+            else  // the polynomial's last product and the subtraction in one FMA
+              s[f][i] = at_exp<T>(fmaf(s[f][i], at_poly<form.value>(a.sc, s[f][i] * s[f][i]), -ms));
+          }
+      });
+      if (part) {
+        int lo2 = lo, hi2 = hi;  // (opaque: the comparisons above would be kept for here, two scalar registers each)
+        asm volatile("" : "+v"(lo2), "+v"(hi2));
+#pragma unroll
+        for (int f = 0; f < KF; ++f)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int j = 32 * f + 8 * (i >> 2) + (i & 3);
+            s[f][i] = j < lo2 || j >= hi2 ? 0.f : s[f][i];
+          }
+      }
+    } else {
+#pragma unroll
+      for (int f = 0; f < KF; ++f)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[f][i] = at_exp<T>(RAW ? fmaf(s[f][i], a.sc.scale_u, -ms) : s[f][i] - ms);
+    }
 #pragma unroll
     for (int f = 0; f < KF; ++f) {
-      float p[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) p[i] = at_exp<T>(RAW ? fmaf(s[f][i], a.sc.scale_u, -ms) : s[f][i] - ms);
+      const float* p = (const float*)&s[f];
       // p is rounded to the 16-bit operand type: half a step, random in sign over the keys
       const AtP<T> pk(p);
       if constexpr (sizeof(T) == 2) {
@@ -209,7 +233,6 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) k_mattn_fwd(A
       at_accumulate<T, DF>(V, off, 32 * f, pk, acc, lane);
     }
   };
-  if (nt > 0) issue(0, k_lo);
   for (int t = 0; t < nt; t += 2) {
     step(std::integral_constant<int, 0>{}, t);
     if (t + 1 < nt) step(std::integral_constant<int, 1>{}, t + 1);
@@ -358,9 +381,11 @@ template <typename T, int DF, bool CAP, bool SLOPE>
 static int mattn_fwd_df(const AtArgs& a, int nw, hipStream_t stream) {
   constexpr int RB = AtPad<DF>::DP * AtT<T>::E;
   const int rows = a.lq * a.group, nbh = a.batch * a.hk;
-  const dim3 grid((unsigned)((long long)cdiv(rows, 32 * nw) * nbh), (unsigned)a.splits);
-  if (nw == 4) {
-    constexpr int KT = sizeof(T) == 4 ? 32 : 64;  // f32 rows are twice as wide: the same LDS for half the keys
+  const dim3 grid((unsigned)(nbh * a.splits), (unsigned)cdiv(rows, 32 * nw));
+  constexpr int KT = sizeof(T) == 4 ? 32 : 64;  // f32 rows are twice as wide: the same LDS for half the keys
+  if (nw == 8) {
+    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, 8, KT>), grid, dim3(512), 4 * KT * RB, stream, a);
+  } else if (nw == 4) {
     hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, 4, KT>), grid, dim3(256), 4 * KT * RB, stream, a);
   } else {
     hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, 1, 32>), grid, dim3(64), 4 * 32 * RB, stream, a);
