@@ -55,6 +55,11 @@ struct AtArgs {
   void *dq, *dk, *dv;          // contiguous [batch][l][h][d]
 };
 
+// forward launch: row waves and key groups per workgroup, keys per split, splits
+struct AtPlan {
+  int nw, ng, chunk, splits;
+};
+
 constexpr float AT_LOG2E = 1.4426950408889634f;
 constexpr unsigned AT_RECORDS = 0x7ffffff0u;  // buffer range: offsets within a tile stay below, BUF_OOB is past it
 

@@ -4,9 +4,9 @@
 
 namespace dmf {
 
-int mattn_fwd_bf16(const AtArgs& a, int nw, hipStream_t stream);
-int mattn_fwd_f16(const AtArgs& a, int nw, hipStream_t stream);
-int mattn_fwd_f32(const AtArgs& a, int nw, hipStream_t stream);
+int mattn_fwd_bf16(const AtArgs& a, AtPlan p, hipStream_t stream);
+int mattn_fwd_f16(const AtArgs& a, AtPlan p, hipStream_t stream);
+int mattn_fwd_f32(const AtArgs& a, AtPlan p, hipStream_t stream);
 int mattn_bwd_bf16(const AtArgs& a, hipStream_t stream);
 int mattn_bwd_f16(const AtArgs& a, hipStream_t stream);
 int mattn_bwd_f32(const AtArgs& a, hipStream_t stream);
@@ -78,29 +78,57 @@ __global__ void __launch_bounds__(1024) k_mattn_spans(const int* __restrict__ do
   out[j - q0] = id[j] < 0 ? make_int2(0, 0) : make_int2(start, end);
 }
 
-struct AtPlan {
-  int nw, chunk, splits;
-};
-// Rows of 32 or fewer per key head take the one-wave workgroups; their keys are cut until about AT_FEW_BLOCKS workgroups
-// run. More rows take workgroups of 128 rows, cut only while they do not fill the card's 512 places (two per CU).
-constexpr long long AT_FEW_BLOCKS = 4096, AT_BLOCKS = 512;
-static AtPlan at_plan(int batch, int lq, int lk, int hk, int group) {
-  const long long rows = (long long)lq * group, nbh = (long long)batch * hk;
-  AtPlan p;
-#ifndef X_NW8
-#define X_NW8 1024
-#endif
-  p.nw = rows <= 32 ? 1 : (rows + 255) / 256 * nbh >= X_NW8 ? 8 : 4;
-  const long long blocks = ((rows + 32 * p.nw - 1) / (32 * p.nw)) * nbh;
-  const long long want = p.nw == 1 ? AT_FEW_BLOCKS : AT_BLOCKS, least = p.nw == 1 ? 64 : 256;
-  long long chunk = ((long long)lk * blocks + want - 1) / want;
-  chunk = (chunk + 63) / 64 * 64;
-  if (chunk < least) chunk = least;
-  if (chunk * 32768 < lk) chunk = ((long long)lk / 32768 + 64) / 64 * 64;
-  p.splits = (int)((lk + chunk - 1) / chunk);
-  if (nbh * p.splits >= (1LL << 31)) p.splits = 1;
-  if (p.splits < 1 || blocks * 2 > want) p.splits = 1;
-  p.chunk = p.splits > 1 ? (int)chunk : (lk > 0 ? lk : 1);
+// The forward's launch, from sizes alone.
+//
+// Up to 32 rows per key head (single tokens): one-wave workgroups, the keys cut until about AT_FEW_BLOCKS of them run (five
+// fit a CU; 8 x 32 query heads over 65536 keys: 279 us with 4096, 254 with 8192, 266 with 16384).
+//
+// More rows: 4 row waves (3, with 32-key tiles, where short rows would leave one of four without work and half a key tile
+// empty: 257 x 257 tokens, 12 heads of 64, batch 32: 32 -> 28 us). The keys are cut where that evens out the CUs: a CU's
+// n = ceil(workgroups / 256) run two at a time (an odd one out has the CU to itself, a third faster), each costs its key
+// tiles and about four tiles' time to start and end, and the cut costs the partials' traffic and a second launch (batch 2, 413
+// queries, 16 heads over 4, 32768 keys: 5 cuts 382 us, 7: 313, 9: 280, 12: 296). Ragged lengths leave whole cuts without
+// work, which two more even out (lengths 32768 and 8192: 9 cuts 280 us, 11: 242, 13: 239).
+// f32 tiles take about four times as long, and two key groups share a workgroup's rows while workgroups are scarce.
+constexpr long long AT_FEW_BLOCKS = 8192, AT_CUS = 256;
+static AtPlan at_plan(int dtype, int batch, int lq, int lk, int hk, int group, int d, bool ragged) {
+  const long long rows = (long long)lq * group, nbh = (long long)batch * hk, r32 = (rows + 31) / 32;
+  AtPlan p = {4, 1, lk > 0 ? lk : 1, 1};
+  long long chunk = 0;
+  if (rows <= 32) {
+    p.nw = 1;
+    if (nbh * 2 <= AT_FEW_BLOCKS) {
+      chunk = ((long long)lk * nbh + AT_FEW_BLOCKS - 1) / AT_FEW_BLOCKS;
+      chunk = chunk < 64 ? 64 : (chunk + 63) / 64 * 64;
+    }
+  } else {
+    const long long b4 = (r32 + 3) / 4 * nbh;
+    if ((r32 + 2) / 3 * 3 * nbh < b4 * 4 && lk <= 512 && (lk + 63) / 64 * 64 - lk >= 32) {
+      p.nw = 3;
+      return p;
+    }
+    const double fixed = dtype == DMF_F32 ? 1.0 : 4.0, tile_bytes = dtype == DMF_F32 ? 32e6 : 8e6;
+    double best = 0;
+    for (int s = 1; s <= 64 && (s == 1 || (long long)s * b4 <= 16 * AT_CUS); ++s) {
+      long long c = ((long long)lk + s - 1) / s;
+      c = (c + 63) / 64 * 64;
+      if (s > 1 && c < 128) break;
+      const long long n = c > 0 ? ((long long)lk + c - 1) / c : 1;
+      const long long turns = (b4 * n + AT_CUS - 1) / AT_CUS;
+      double cost = (turns + (turns % 2 ? 0.3 : 0.0)) * (c / 64.0 + fixed);
+      if (n > 1) cost += fixed + (double)n * rows * nbh * (d + 4) * 8 / tile_bytes;
+      if (s == 1 || cost < best) best = cost, chunk = n > 1 ? c : 0;
+    }
+    if (ragged && chunk > 0) {
+      const long long n = ((long long)lk + chunk - 1) / chunk + 2, c = ((long long)lk + n - 1) / n;
+      if (c >= 256) chunk = (c + 63) / 64 * 64;
+    }
+    if (dtype == DMF_F32 && lk > 64 && b4 * (chunk ? ((long long)lk + chunk - 1) / chunk : 1) <= AT_CUS) p.ng = 2;
+  }
+  if (chunk > 0 && lk > chunk && nbh * (((long long)lk + chunk - 1) / chunk) < (1LL << 31)) {
+    p.chunk = (int)chunk;
+    p.splits = (int)(((long long)lk + chunk - 1) / chunk);
+  }
   return p;
 }
 
@@ -146,9 +174,9 @@ extern "C" int dmf_mattn_spans(const int* documents, long long doc_sb, const int
   return 0;
 }
 
-extern "C" long long dmf_mattn_fwd_ws_floats(int batch, int lq, int lk, int hq, int hk, int d) {
+extern "C" long long dmf_mattn_fwd_ws_floats(int dtype, int batch, int lq, int lk, int hq, int hk, int d, int ragged) {
   if (batch <= 0 || lq <= 0 || lk <= 0 || hk <= 0 || hq < hk) return 0;
-  const AtPlan p = at_plan(batch, lq, lk, hk, hq / hk);
+  const AtPlan p = at_plan(dtype, batch, lq, lk, hk, hq / hk, d, ragged != 0);
   return p.splits > 1 ? (long long)p.splits * batch * lq * hq * (d + 4) : 0;
 }
 
@@ -171,7 +199,7 @@ extern "C" int dmf_mattn_fwd(int dtype, const void* q, long long q_sb, long long
   DMF_CHECK_ARG(q && o && (lk == 0 || (k && v)), "dmf_mattn_fwd: null operand");
   DMF_CHECK_ARG((uintptr_t)o % 16 == 0 && (uintptr_t)o_lo % 16 == 0 && (uintptr_t)spans % 8 == 0,
                 "dmf_mattn_fwd: outputs must be aligned to 16 bytes");
-  const AtPlan p = at_plan(batch, lq, lk, hk, a.group);
+  const AtPlan p = at_plan(dtype, batch, lq, lk, hk, a.group, d, kv_lens != nullptr);
   a.chunk = p.chunk, a.splits = p.splits;
   if (p.splits > 1) {
     DMF_CHECK_ARG(ws && (uintptr_t)ws % 16 == 0, "dmf_mattn_fwd: this size needs a workspace (dmf_mattn_fwd_ws_floats)");
@@ -179,8 +207,8 @@ extern "C" int dmf_mattn_fwd(int dtype, const void* q, long long q_sb, long long
     a.pml = ws + (long long)p.splits * batch * lq * hq * d;
   }
   hipStream_t s = (hipStream_t)stream;
-  return dtype == DMF_BF16 ? mattn_fwd_bf16(a, p.nw, s) : dtype == DMF_F16 ? mattn_fwd_f16(a, p.nw, s)
-                                                                          : mattn_fwd_f32(a, p.nw, s);
+  return dtype == DMF_BF16 ? mattn_fwd_bf16(a, p, s) : dtype == DMF_F16 ? mattn_fwd_f16(a, p, s)
+                                                                          : mattn_fwd_f32(a, p, s);
 }
 
 extern "C" int dmf_mattn_bwd(int dtype, const void* q, long long q_sb, long long q_sl, long long q_sh, const void* k,

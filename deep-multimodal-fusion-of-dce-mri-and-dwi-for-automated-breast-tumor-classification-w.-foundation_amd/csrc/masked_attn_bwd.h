@@ -6,8 +6,8 @@
 //   dv_j = sum_i p_ij do_i,  dk_j = scale sum_i ds_ij q_i,  dq_i = scale sum_j ds_ij k_j
 //
 // One launch holds two kinds of workgroups: those of 128 keys, which walk the queries that see them and keep dK and dV in
-// registers, and those of 128 (f32) or 256 packed rows, which walk their keys and keep dQ. The key workgroups' longest walk
-// (all queries of all heads of a group) decides how evenly a launch ends, so 16-bit types give each 128 keys two groups of
+// registers, and those of 256 (f32 over 64 dims: 128) packed rows, which walk their keys and keep dQ. The key workgroups' longest walk
+// (all queries of all heads of a group) decides how evenly a launch ends, so each 128 keys have, where LDS allows, two groups of
 // four waves that take the query tiles in turn and add up at the end. The scores are computed in
 // both (7 products for the 5 that one pass with dQ in atomics would take): no atomics, so the same bits every run, no
 // f32 dQ in HBM, and the sum over a group's query heads happens inside the dK / dV accumulators.
@@ -75,7 +75,7 @@ struct AtRowData {
 constexpr int AT_QT = 32;
 template <typename T, int DF> struct AtBwdLds {
   static constexpr int RB = AtPad<DF>::DP * AtT<T>::E;
-  static constexpr int NG = sizeof(T) == 4 ? 1 : 2;         // groups of four waves
+  static constexpr int NG = sizeof(T) == 4 && DF > 64 ? 1 : 2;  // groups of four waves (f32 at 128 dims: LDS for one)
   static constexpr int KT = sizeof(T) == 4 ? 32 : 64;       // keys per tile of the row workgroups
   static constexpr int QTILE = AT_QT * RB, VT = 128 * RB;
   static constexpr int GROUP = 4 * QTILE + 2 * (int)sizeof(AtRowData);  // a group's stages
@@ -463,7 +463,7 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
 // blockIdx.y first counts the workgroups of 128 keys (the longer ones; the first keys are seen by most queries), then those
 // of 128 NG packed rows, the last rows first; heads vary fastest, as in the forward
 template <typename T, int DF, bool CAP, bool SLOPE>
-__global__ void __launch_bounds__(256 * (sizeof(T) == 4 ? 1 : 2), sizeof(T) == 4 ? 1 : 2) k_mattn_bwd(AtArgs a) {
+__global__ void __launch_bounds__((256 * AtBwdLds<T, DF>::NG), (AtBwdLds<T, DF>::NG)) k_mattn_bwd(AtArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int ktiles = (a.lk + 127) / 128, t = blockIdx.y;
   if (t < ktiles)

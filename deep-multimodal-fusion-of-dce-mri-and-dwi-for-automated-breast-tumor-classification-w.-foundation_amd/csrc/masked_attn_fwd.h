@@ -55,13 +55,14 @@ __device__ __forceinline__ void at_store4(T* p, const float* v) {  // p aligned 
     *(uint2*)p = make_uint2(AtPair<T>::pack(v[0], v[1]), AtPair<T>::pack(v[2], v[3]));
 }
 
-template <typename T, int DF, bool CAP, bool SLOPE, int NW, int KT>
-__global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) k_mattn_fwd(AtArgs a) {
+template <typename T, int DF, bool CAP, bool SLOPE, int NW, int NG, int KT>
+__global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 && DF > 64 ? 1 : 2) k_mattn_fwd(AtArgs a) {
   constexpr int DP = AtPad<DF>::DP, KS = AtOffsets<T, DF>::KS, FD = DF / 32, KF = KT / 32;
   constexpr int TILE = KT * DP * AtT<T>::E, STAGE = 2 * TILE;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   __shared__ int range[2 * NW];
-  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
+  const int wid = NG > 1 ? wave % NW : wave, grp = NG > 1 ? wave / NW : 0;  // 32 rows; which of the key tiles
   const int nbh = a.batch * a.hk, rows = a.lq * a.group;
   // Workgroups go to the eight XCDs in turn: splits, then heads vary fastest, so that an XCD gets a share of every batch
   // row (ragged lengths) and row block, and the last row blocks, the longest under a causal mask, start first.
@@ -74,7 +75,8 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) k_mattn_fwd(A
   AtSpan sp = row < rows ? at_span(a, b, qi) : AtSpan{0, 0, 0};
   const bool live = sp.hi > sp.lo;
   const AtBounds w = at_bounds(a, b, kh, tile * 32 * NW + wid * 32, rows, sp);
-  const int w_lo = w.lo, w_hi = w.hi, i_lo = w.i_lo, i_hi = w.i_hi;
+  const int w_lo = w.lo, w_hi = w.hi, i_lo = w.i_lo;
+  int i_hi = w.i_hi;
   int k_lo = w_lo, k_hi = w_hi;
   if constexpr (NW > 1) {
     if (a.spans) {
@@ -94,20 +96,23 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) k_mattn_fwd(A
     k_lo = max(k_lo, split * a.chunk);
     k_hi = (int)min((long long)k_hi, (long long)(split + 1) * a.chunk);
     if (k_lo >= k_hi) return;
+    sp.hi = min(sp.hi, k_hi);  // (a tile that starts off the chunk's grid may reach past its end)
+    i_hi = min(i_hi, k_hi);
   }
   const T* kb = (const T*)a.k + b * a.k_sb + kh * a.k_sh;
   const T* vb = (const T*)a.v + b * a.v_sb + kh * a.v_sh;
   const T* qb = (const T*)a.q + b * a.q_sb + (long long)qi * a.q_sl + head * a.q_sh;
-  const float slope = SLOPE ? at_slope<T>(a, head) : 0.f;
+  const float slope = SLOPE ? at_slope<T>(a, head) / (!CAP && sizeof(T) == 2 ? a.sc.scale_u : 1.f) : 0.f;
   const unsigned lds0 = (unsigned)(uintptr_t)((__attribute__((address_space(3))) char*)smem);
 
   const AtLoad<T, DP, KT, NW> kl(a.k_sl, a.d, wid, lane), vl(a.v_sl, a.d, wid, lane);
   auto issue = [&](int stage, int k0) {
-    kl.issue(kb, k0, k_hi, lds0 + stage * STAGE, wid);
-    vl.issue(vb, k0, k_hi, lds0 + stage * STAGE + TILE, wid);
+    const unsigned S = lds0 + (grp * 2 + stage) * STAGE;
+    kl.issue(kb, k0, k_hi, S, wid);
+    vl.issue(vb, k0, k_hi, S + TILE, wid);
   };
   const int nt = k_hi > k_lo ? (k_hi - k_lo + KT - 1) / KT : 0;
-  if (nt > 0) issue(0, k_lo);  // (first: the rest of the set-up runs under its latency)
+  if (grp < nt) issue(0, k_lo + grp * KT);  // (first: the rest of the set-up runs under its latency)
   uint4 qf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
@@ -121,18 +126,20 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) k_mattn_fwd(A
   // (rounded: then the rounding of a dominant key cancels); lx: the unrounded sum, for lse
   float m = -INFINITY, ms = 0.f, l = 0.f, lx = 0.f;
   const AtOffsets<T, DF> off(lane);
-  // plain 16-bit scores stay raw and are scaled in the exponent's FMA (scale > 0); others become s in units U in place
-  constexpr bool RAW = !(CAP || SLOPE || sizeof(T) == 4);
+  // uncapped 16-bit scores stay raw, a bias divided by the scale, and are scaled in the exponent's FMA (scale > 0); others
+  // become s in units U in place
+  constexpr bool RAW = !CAP && sizeof(T) == 2;
   // capped 16-bit scores without a bias stay raw too: tanh does not change their order, so the maximum is taken of the raw
   // products and bent alone
   constexpr bool LATE = CAP && !SLOPE && sizeof(T) == 2;
-  auto step = [&](auto stage, int t) {
+  const char* const base = smem + grp * 2 * STAGE;
+  auto step = [&](auto stage, int t) {  // tile t of all, or none (t >= nt: a group that has run out keeps the barriers)
     const int k0 = k_lo + t * KT;
     // this tile has landed (in every wave: the barrier); the other stage's last readers are past it too
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (t + 1 < nt) issue(1 - stage.value, k0 + KT);
-    if (k0 >= w_hi || k0 + KT <= w_lo) return;  // (wave-uniform) nothing here for these rows
-    const char* K = smem + stage.value * STAGE;
+    if (t + NG < nt) issue(1 - stage.value, k0 + NG * KT);
+    if (t >= nt || k0 >= w_hi || k0 + KT <= w_lo) return;  // (wave-uniform) nothing here for these rows
+    const char* K = base + stage.value * STAGE;
     const char* V = K + TILE;
     at_f32x16 s[KF];
 #pragma unroll
@@ -141,7 +148,7 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) k_mattn_fwd(A
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) s[f] = at_mfma<T>(at_row<T, DF>(K, off, 32 * f, ks), qf[ks], s[f]);
     }
-    if constexpr (SLOPE || (!RAW && !LATE)) at_bend_tiles<T, CAP, KF>(a.sc, s);
+    if constexpr (!RAW && !LATE) at_bend_tiles<T, CAP, KF>(a.sc, s);
     if constexpr (SLOPE) {
       const float x0 = (float)(sp.at - k0 - 4 * h);  // position minus this lane's first key
 #pragma unroll
@@ -233,12 +240,35 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) k_mattn_fwd(A
       at_accumulate<T, DF>(V, off, 32 * f, pk, acc, lane);
     }
   };
-  for (int t = 0; t < nt; t += 2) {
-    step(std::integral_constant<int, 0>{}, t);
-    if (t + 1 < nt) step(std::integral_constant<int, 1>{}, t + 1);
+  for (int t = 0; t < nt; t += 2 * NG) {
+    step(std::integral_constant<int, 0>{}, t + grp);
+    if (t + NG < nt) step(std::integral_constant<int, 1>{}, t + NG + grp);
   }
   lx = at_half_sum(lx);
   l = sizeof(T) == 4 ? lx : at_half_sum(l);
+  if constexpr (NG > 1) {  // the second group's maxima, sums and accumulators through LDS
+    float* part = (float*)smem + wid * 64 * (DF / 2 + 3) + lane;
+    __syncthreads();
+    if (grp == 1) {
+      part[0] = m, part[64] = l, part[128] = lx;
+#pragma unroll
+      for (int f = 0; f < FD; ++f)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[(16 * f + i + 3) * 64] = acc[f][i];
+    }
+    __syncthreads();
+    if (grp == 1) return;
+    const float m1 = part[0], mn = fmaxf(m, m1);
+    ms = mn == -INFINITY ? 0.f : mn;
+    const float w0 = at_exp<T>(m - ms), w1 = at_exp<T>(m1 - ms);
+    m = mn;
+    l = l * w0 + part[64] * w1;
+    lx = lx * w0 + part[128] * w1;
+#pragma unroll
+    for (int f = 0; f < FD; ++f)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[f][i] = acc[f][i] * w0 + part[(16 * f + i + 3) * 64] * w1;
+  }
   float bad = l * 0.f;
 #pragma unroll
   for (int f = 0; f < FD; ++f)
@@ -316,57 +346,55 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 ? 1 : 2) k_mattn_fwd(A
 }
 
 // o of one packed row from its splits: sum exp(m_s - m) O_s / sum exp(m_s - m) l_s over the splits its span touches.
-// One workgroup per row: 8 groups of 32 lanes take every eighth split (four of its dims a lane), added up through LDS
-// in a fixed order.
-template <typename T>
+// G groups of 32 lanes (four dims a lane) per row take every G-th split and are added up through LDS in a fixed order:
+// 8 for few rows of many splits, 1 for many rows.
+template <typename T, int G>
 __global__ void __launch_bounds__(256) k_mattn_join(AtArgs a) {
   __shared__ float4 part[8][32];
-  __shared__ float sums[8][2], red[4];
+  __shared__ float sums[8][2];
   const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5, nbh = a.batch * a.hk, rows = a.lq * a.group;
-  const int bh = blockIdx.x % nbh, row = blockIdx.x / nbh;
+  const long long r0 = (long long)blockIdx.x * (8 / G) + grp / G, step = (long long)nbh * rows;  // r0 = bh * rows + row
+  const int g = grp % G;
+  const bool on = 4 * lane < a.d, in = r0 < step;
+  const int bh = in ? (int)(r0 / rows) : 0, row = in ? (int)(r0 - (long long)bh * rows) : 0;
   const int b = bh / a.hk, kh = bh - b * a.hk;
   const AtRow pr = at_packed(a, kh, row);
-  const int qi = pr.qi, head = pr.head;
-  const AtSpan sp = at_span(a, b, qi);
-  const bool live = sp.hi > sp.lo;
+  const AtSpan sp = at_span(a, b, pr.qi);
+  const bool live = in && sp.hi > sp.lo;
   const int s0 = sp.lo / a.chunk, s1 = live ? (sp.hi - 1) / a.chunk + 1 : s0;
-  const long long r0 = (long long)bh * rows + row, step = (long long)nbh * rows;
   float m = -INFINITY;
-  for (int s = s0 + threadIdx.x; s < s1; s += 256) m = fmaxf(m, a.pml[4 * (s * step + r0)]);
-  m = wave_max(m);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  for (int s = s0 + lane; s < s1; s += 32) m = fmaxf(m, a.pml[4 * (s * step + r0)]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
   const float ms = m == -INFINITY ? 0.f : m;
-  const bool on = 4 * lane < a.d;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f, lx = 0.f;
 #pragma unroll 4
-  for (int s = s0 + grp; s < s1; s += 8) {
-    const long long pr = s * step + r0;
-    const float4 ml = *(const float4*)(a.pml + 4 * pr);
-    const float4 x = on ? *(const float4*)(a.po + pr * a.d + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = s0 + g; s < s1; s += G) {
+    const long long at = s * step + r0;
+    const float4 ml = *(const float4*)(a.pml + 4 * at);
+    const float4 x = on ? *(const float4*)(a.po + at * a.d + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
     // (a split whose keys are all -inf for this row has w = 0 and finite sums)
     const float w = at_exp<T>(ml.x - ms);
     l = fmaf(w, ml.y, l);
     lx = fmaf(w, ml.z, lx);
     o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
   }
-  part[grp][lane] = o;
-  if (lane == 0) sums[grp][0] = l, sums[grp][1] = lx;
-  __syncthreads();
-  if (grp != 0) return;
-  l = lx = 0.f;
-  o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-  for (int g = 0; g < 8; ++g) {
-    const float4 x = part[g][lane];
-    o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
-    l += sums[g][0], lx += sums[g][1];
+  if constexpr (G > 1) {
+    part[grp][lane] = o;
+    if (lane == 0) sums[grp][0] = l, sums[grp][1] = lx;
+    __syncthreads();
+    if (g != 0) return;
+    for (int k = 1; k < G; ++k) {
+      const float4 x = part[grp + k][lane];
+      o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+      l += sums[grp + k][0], lx += sums[grp + k][1];
+    }
   }
-  if (a.lse && lane == 0) a.lse[((long long)b * a.hq + head) * a.lq + qi] = live ? ms + at_log<T>(lx) : INFINITY;
+  if (!in) return;
+  if (a.lse && lane == 0) a.lse[((long long)b * a.hq + pr.head) * a.lq + pr.qi] = live ? ms + at_log<T>(lx) : INFINITY;
   if (!on) return;
-  const long long orow = (((long long)b * a.lq + qi) * a.hq + head) * a.d + 4 * lane;
+  const long long orow = (((long long)b * a.lq + pr.qi) * a.hq + pr.head) * a.d + 4 * lane;
   const float inv = live ? 1.f / l : 0.f;
   float v[4] = {live ? o.x * inv : 0.f, live ? o.y * inv : 0.f, live ? o.z * inv : 0.f, live ? o.w * inv : 0.f};
   at_store4((T*)a.o + orow, v);
@@ -378,31 +406,33 @@ __global__ void __launch_bounds__(256) k_mattn_join(AtArgs a) {
 }
 
 template <typename T, int DF, bool CAP, bool SLOPE>
-static int mattn_fwd_df(const AtArgs& a, int nw, hipStream_t stream) {
+static int mattn_fwd_df(const AtArgs& a, AtPlan p, hipStream_t stream) {
   constexpr int RB = AtPad<DF>::DP * AtT<T>::E;
-  const int rows = a.lq * a.group, nbh = a.batch * a.hk;
-  const dim3 grid((unsigned)(nbh * a.splits), (unsigned)cdiv(rows, 32 * nw));
   constexpr int KT = sizeof(T) == 4 ? 32 : 64;  // f32 rows are twice as wide: the same LDS for half the keys
-  if (nw == 8) {
-    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, 8, KT>), grid, dim3(512), 4 * KT * RB, stream, a);
-  } else if (nw == 4) {
-    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, 4, KT>), grid, dim3(256), 4 * KT * RB, stream, a);
-  } else {
-    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, 1, 32>), grid, dim3(64), 4 * 32 * RB, stream, a);
-  }
+  constexpr size_t LDS = 4 * KT * RB;
+  const int rows = a.lq * a.group, nbh = a.batch * a.hk;
+  const dim3 grid((unsigned)(nbh * a.splits), (unsigned)cdiv(rows, 32 * p.nw));
+  if (p.nw == 1)
+    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, 1, 1, 32>), grid, dim3(64), 4 * 32 * RB, stream, a);
+  else if (p.nw == 3)
+    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, 3, 1, 32>), grid, dim3(192), 4 * 32 * RB, stream, a);
+  else if (p.ng == 1)
+    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, 4, 1, KT>), grid, dim3(256), LDS, stream, a);
+  else if constexpr (sizeof(T) == 4)  // (16-bit workgroups of 8 waves lose: two of 4 overlap better)
+    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, 4, 2, KT>), grid, dim3(512), 2 * LDS, stream, a);
   DMF_LAUNCH_CHECK("dmf_mattn_fwd");
   return 0;
 }
 
 template <typename T>
-static int mattn_fwd_t(AtArgs a, int nw, hipStream_t stream) {
+static int mattn_fwd_t(AtArgs a, AtPlan p, hipStream_t stream) {
   at_score_args<T>(a);
   int rc = 0;
 #define DMF_AT_MODE(DF)                                                                  \
-  rc = a.cap > 0.f ? (a.slopes ? mattn_fwd_df<T, DF, true, true>(a, nw, stream)          \
-                               : mattn_fwd_df<T, DF, true, false>(a, nw, stream))        \
-                   : (a.slopes ? mattn_fwd_df<T, DF, false, true>(a, nw, stream)         \
-                               : mattn_fwd_df<T, DF, false, false>(a, nw, stream))
+  rc = a.cap > 0.f ? (a.slopes ? mattn_fwd_df<T, DF, true, true>(a, p, stream)          \
+                               : mattn_fwd_df<T, DF, true, false>(a, p, stream))        \
+                   : (a.slopes ? mattn_fwd_df<T, DF, false, true>(a, p, stream)         \
+                               : mattn_fwd_df<T, DF, false, false>(a, p, stream))
   if (a.d <= 32) DMF_AT_MODE(32);
   else if (a.d <= 64) DMF_AT_MODE(64);
   else if (a.d <= 96) DMF_AT_MODE(96);
@@ -410,8 +440,11 @@ static int mattn_fwd_t(AtArgs a, int nw, hipStream_t stream) {
 #undef DMF_AT_MODE
   if (rc) return rc;
   if (a.splits > 1) {
-    hipLaunchKernelGGL((k_mattn_join<T>), dim3((unsigned)((long long)a.lq * a.group * a.batch * a.hk)), dim3(256), 0,
-                       stream, a);
+    const long long n = (long long)a.lq * a.group * a.batch * a.hk;
+    if (n >= 4096)
+      hipLaunchKernelGGL((k_mattn_join<T, 1>), dim3((unsigned)((n + 7) / 8)), dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((k_mattn_join<T, 8>), dim3((unsigned)n), dim3(256), 0, stream, a);
     DMF_LAUNCH_CHECK("dmf_mattn_fwd (join)");
   }
   return 0;

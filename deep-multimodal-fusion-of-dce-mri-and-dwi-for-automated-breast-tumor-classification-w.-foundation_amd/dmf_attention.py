@@ -225,7 +225,7 @@ def _attn_fwd(q, k, v, cfg, kv_lens, prefix, slopes, spans, train):
     o = torch.empty((b, lq, hq, d), dtype=q.dtype, device=q.device)
     o_lo = torch.empty_like(o) if train and q.dtype != torch.float32 else None
     lse = torch.empty(b * lq * hq, dtype=torch.float32, device=q.device) if train else None
-    n = N.load().dmf_mattn_fwd_ws_floats(b, lq, k.shape[1], hq, k.shape[2], d)
+    n = N.load().dmf_mattn_fwd_ws_floats(_DTYPES[q.dtype], b, lq, k.shape[1], hq, k.shape[2], d, int(kv_lens is not None))
     ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     with _on(q):
         N.call("dmf_mattn_fwd", *args, o.data_ptr(), _p(o_lo), _p(lse), _p(ws), N.stream_ptr(q.device))

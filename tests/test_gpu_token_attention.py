@@ -373,6 +373,10 @@ def test_attention_documents(causal, dt):
     docs[1] = _docs(1, 300, 3, 0, 2)[0]
     docs[2] = -1
     _attn_case(3, 300, 300, 4, 2, 64, dt, causal=causal, docs=docs, cap=30.0)
+    # the keys of one long row split over workgroups: documents across the cuts, tiles that start off their grid
+    assert N.load().dmf_mattn_fwd_ws_floats(N.dtype_code(dt), 1, 1100, 1100, 2, 1, 64, 0) > 0
+    _attn_case(1, 1100, 1100, 2, 1, 64, dt, causal=causal, docs=_docs(1, 1100, 90, 10, 4))
+    _attn_case(1, 1100, 1100, 2, 1, 64, dt, causal=causal, docs=_docs(1, 1100, 700, 10, 5))
 
 
 def test_attention_documents_with_prefix_cache_and_lengths():
@@ -392,7 +396,7 @@ def test_attention_single_query(hq, hk, lk, dt):
 @pytest.mark.parametrize("lq", [2, 9, 100])
 def test_attention_few_queries_split_over_keys(lq, dt):
     """Few rows against many keys: the keys are split over workgroups and joined, also for training."""
-    n = N.load().dmf_mattn_fwd_ws_floats(2, lq, 3000, 4, 2, 64)
+    n = N.load().dmf_mattn_fwd_ws_floats(N.dtype_code(dt), 2, lq, 3000, 4, 2, 64, 1)
     assert n > 0
     _attn_case(2, lq, 3000, 4, 2, 64, dt, causal=True, kv_lens=[3000, 700], slopes=True)
     _attn_case(1, lq, 3000, 4, 2, 64, dt, causal=True, prefix=[1500], cap=20.0, grad=False)
