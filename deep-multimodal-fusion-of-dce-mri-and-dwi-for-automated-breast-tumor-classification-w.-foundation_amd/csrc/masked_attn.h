@@ -216,6 +216,12 @@ template <typename T> struct AtP {
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = AtPair<T>::pack(p[2 * i], p[2 * i + 1]);
   }
+  // what rounding p to `r` left over, rounded in turn
+  __device__ __forceinline__ AtP(const float* p, const AtP& r) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      w[i] = AtPair<T>::pack(p[2 * i] - B16<T>::lo(r.w[i]), p[2 * i + 1] - B16<T>::hi(r.w[i]));
+  }
 };
 template <> struct AtP<float> {
   float w[16];
@@ -226,10 +232,10 @@ template <> struct AtP<float> {
 };
 
 // acc[fd] += X^T P for the 32 tile rows r0 .. r0 + 31: X's column block fd (32 dims) as the row operand, read transposed
-// from its tile
-template <typename T, int DF>
+// from its tile. TWO: P is p + rest.
+template <typename T, int DF, bool TWO = false>
 __device__ __forceinline__ void at_accumulate(const char* tile, const AtOffsets<T, DF>& o, int r0, const AtP<T>& p,
-                                              at_f32x16* acc, int lane) {
+                                              at_f32x16* acc, int lane, const AtP<T>* rest = nullptr) {
   constexpr int DP = AtPad<DF>::DP, RB = AtOffsets<T, DF>::RB;
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
@@ -242,6 +248,10 @@ __device__ __forceinline__ void at_accumulate(const char* tile, const AtOffsets<
         const uint2 g =
             __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_v4s*)(t + o.col[2 * fd + 1])));
         acc[fd] = at_mfma<T>(make_uint4(l.x, l.y, g.x, g.y), b, acc[fd]);
+        if constexpr (TWO)
+          acc[fd] = at_mfma<T>(make_uint4(l.x, l.y, g.x, g.y),
+                               make_uint4(rest->w[4 * c], rest->w[4 * c + 1], rest->w[4 * c + 2], rest->w[4 * c + 3]),
+                               acc[fd]);
       }
     }
   } else {

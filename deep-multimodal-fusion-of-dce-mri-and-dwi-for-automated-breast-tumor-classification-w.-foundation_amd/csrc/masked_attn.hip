@@ -197,6 +197,7 @@ extern "C" int dmf_mattn_fwd(int dtype, const void* q, long long q_sb, long long
   if (int rc = at_check("dmf_mattn_fwd", a, dtype)) return rc;
   if (batch == 0 || lq == 0) return 0;
   DMF_CHECK_ARG(q && o && (lk == 0 || (k && v)), "dmf_mattn_fwd: null operand");
+  DMF_CHECK_ARG(!lse || o_lo || dtype == DMF_F32, "dmf_mattn_fwd: lse of a 16-bit type goes with o_lo");
   DMF_CHECK_ARG((uintptr_t)o % 16 == 0 && (uintptr_t)o_lo % 16 == 0 && (uintptr_t)spans % 8 == 0,
                 "dmf_mattn_fwd: outputs must be aligned to 16 bytes");
   const AtPlan p = at_plan(dtype, batch, lq, lk, hk, a.group, d, kv_lens != nullptr);

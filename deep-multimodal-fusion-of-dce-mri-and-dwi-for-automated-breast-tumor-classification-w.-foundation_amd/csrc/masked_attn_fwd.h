@@ -55,7 +55,7 @@ __device__ __forceinline__ void at_store4(T* p, const float* v) {  // p aligned 
     *(uint2*)p = make_uint2(AtPair<T>::pack(v[0], v[1]), AtPair<T>::pack(v[2], v[3]));
 }
 
-template <typename T, int DF, bool CAP, bool SLOPE, int NW, int NG, int KT>
+template <typename T, int DF, bool CAP, bool SLOPE, bool TRAIN, int NW, int NG, int KT>
 __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 && DF > 64 ? 1 : 2) k_mattn_fwd(AtArgs a) {
   constexpr int DP = AtPad<DF>::DP, KS = AtOffsets<T, DF>::KS, FD = DF / 32, KF = KT / 32;
   constexpr int TILE = KT * DP * AtT<T>::E, STAGE = 2 * TILE;
@@ -122,8 +122,8 @@ __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 && DF > 64 ? 1 : 
   at_f32x16 acc[FD];
 #pragma unroll
   for (int f = 0; f < FD; ++f) acc[f] = at_zero();
-  // ms: m, or 0 while there is none; l: the sum that o is divided by, of the probabilities as the products take them
-  // (rounded: then the rounding of a dominant key cancels); lx: the unrounded sum, for lse
+  // ms: m, or 0 while there is none; the sum that o is divided by: l, of the probabilities as the products take them
+  // (rounded: then the rounding of a dominant key cancels), or lx, of the unrounded ones, where their rest is taken too
   float m = -INFINITY, ms = 0.f, l = 0.f, lx = 0.f;
   const AtOffsets<T, DF> off(lane);
   // uncapped 16-bit scores stay raw, a bias divided by the scale, and are scaled in the exponent's FMA (scale > 0); others
@@ -227,17 +227,26 @@ __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 && DF > 64 ? 1 : 
 #pragma unroll
     for (int f = 0; f < KF; ++f) {
       const float* p = (const float*)&s[f];
-      // p is rounded to the 16-bit operand type: half a step, random in sign over the keys
+      // p is rounded to the 16-bit operand type: half a step, random in sign over the keys. For a backward what that leaves
+      // is multiplied too: its delta = do.o stands for sum_j p dp, and an error of o would pass into dS through whole rows
+      // (dq's error against 64 bits 1.47 to 1.52 times a rounding's instead of 1.42).
       const AtP<T> pk(p);
       if constexpr (sizeof(T) == 2) {
+        if constexpr (TRAIN) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) l = AtPair<T>::add(pk.w[i], l);
-      }
-      if (sizeof(T) == 4 || a.lse) {
+          for (int i = 0; i < 16; ++i) lx += p[i];
+          const AtP<T> rest(p, pk);
+          at_accumulate<T, DF, true>(V, off, 32 * f, pk, acc, lane, &rest);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) l = AtPair<T>::add(pk.w[i], l);
+          at_accumulate<T, DF>(V, off, 32 * f, pk, acc, lane);
+        }
+      } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) lx += p[i];
+        at_accumulate<T, DF>(V, off, 32 * f, pk, acc, lane);
       }
-      at_accumulate<T, DF>(V, off, 32 * f, pk, acc, lane);
     }
   };
   for (int t = 0; t < nt; t += 2 * NG) {
@@ -245,7 +254,7 @@ __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 && DF > 64 ? 1 : 
     if (t + NG < nt) step(std::integral_constant<int, 1>{}, t + NG + grp);
   }
   lx = at_half_sum(lx);
-  l = sizeof(T) == 4 ? lx : at_half_sum(l);
+  l = sizeof(T) == 4 || TRAIN ? lx : at_half_sum(l);
   if constexpr (NG > 1) {  // the second group's maxima, sums and accumulators through LDS
     float* part = (float*)smem + wid * 64 * (DF / 2 + 3) + lane;
     __syncthreads();
@@ -279,7 +288,7 @@ __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 && DF > 64 ? 1 : 
 
   const long long prow = ((long long)split * nbh + bh) * rows + row;  // partials
   T* ob = (T*)a.o + (((long long)b * a.lq + qi) * a.hq + head) * a.d;
-  T* olo = a.o_lo ? (T*)a.o_lo + (((long long)b * a.lq + qi) * a.hq + head) * a.d : nullptr;
+  T* olo = TRAIN ? (T*)a.o_lo + (((long long)b * a.lq + qi) * a.hq + head) * a.d : nullptr;
   if (row < rows && !((alone >> (lane & 31)) & 1)) {
     if (a.splits > 1) {
       float* po = a.po + prow * a.d;
@@ -303,7 +312,7 @@ __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 && DF > 64 ? 1 : 
 #pragma unroll
           for (int r = 0; r < 4; ++r) v[r] = live ? acc[f][4 * g + r] * inv : 0.f;
           at_store4(ob + e, v);
-          if (olo) {
+          if (TRAIN) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) v[r] -= Cvt<T>::load(Cvt<T>::store(v[r]));
             at_store4(olo + e, v);
@@ -333,7 +342,7 @@ __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 && DF > 64 ? 1 : 
         a.po[pr * a.d + e] = o;
       } else {
         st((T*)a.o + orow + e, o);
-        if (a.o_lo) st((T*)a.o_lo + orow + e, o - Cvt<T>::load(Cvt<T>::store(o)));
+        if (TRAIN) st((T*)a.o_lo + orow + e, o - Cvt<T>::load(Cvt<T>::store(o)));
       }
     }
     if (lane == 0) {
@@ -405,7 +414,7 @@ __global__ void __launch_bounds__(256) k_mattn_join(AtArgs a) {
   }
 }
 
-template <typename T, int DF, bool CAP, bool SLOPE>
+template <typename T, int DF, bool CAP, bool SLOPE, bool TRAIN>
 static int mattn_fwd_df(const AtArgs& a, AtPlan p, hipStream_t stream) {
   constexpr int RB = AtPad<DF>::DP * AtT<T>::E;
   constexpr int KT = sizeof(T) == 4 ? 32 : 64;  // f32 rows are twice as wide: the same LDS for half the keys
@@ -413,15 +422,22 @@ static int mattn_fwd_df(const AtArgs& a, AtPlan p, hipStream_t stream) {
   const int rows = a.lq * a.group, nbh = a.batch * a.hk;
   const dim3 grid((unsigned)(nbh * a.splits), (unsigned)cdiv(rows, 32 * p.nw));
   if (p.nw == 1)
-    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, 1, 1, 32>), grid, dim3(64), 4 * 32 * RB, stream, a);
+    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, TRAIN, 1, 1, 32>), grid, dim3(64), 4 * 32 * RB, stream, a);
   else if (p.nw == 3)
-    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, 3, 1, 32>), grid, dim3(192), 4 * 32 * RB, stream, a);
+    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, TRAIN, 3, 1, 32>), grid, dim3(192), 4 * 32 * RB, stream, a);
   else if (p.ng == 1)
-    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, 4, 1, KT>), grid, dim3(256), LDS, stream, a);
+    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, TRAIN, 4, 1, KT>), grid, dim3(256), LDS, stream, a);
   else if constexpr (sizeof(T) == 4)  // (16-bit workgroups of 8 waves lose: two of 4 overlap better)
-    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, 4, 2, KT>), grid, dim3(512), 2 * LDS, stream, a);
+    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, TRAIN, 4, 2, KT>), grid, dim3(512), 2 * LDS, stream, a);
   DMF_LAUNCH_CHECK("dmf_mattn_fwd");
   return 0;
+}
+template <typename T, int DF, bool CAP, bool SLOPE>
+static int mattn_fwd_train(const AtArgs& a, AtPlan p, hipStream_t stream) {
+  // (f32 keeps no o_lo: one kernel for both)
+  if constexpr (sizeof(T) == 2)
+    if (a.o_lo) return mattn_fwd_df<T, DF, CAP, SLOPE, true>(a, p, stream);
+  return mattn_fwd_df<T, DF, CAP, SLOPE, false>(a, p, stream);
 }
 
 template <typename T>
@@ -429,10 +445,10 @@ static int mattn_fwd_t(AtArgs a, AtPlan p, hipStream_t stream) {
   at_score_args<T>(a);
   int rc = 0;
 #define DMF_AT_MODE(DF)                                                                  \
-  rc = a.cap > 0.f ? (a.slopes ? mattn_fwd_df<T, DF, true, true>(a, p, stream)          \
-                               : mattn_fwd_df<T, DF, true, false>(a, p, stream))        \
-                   : (a.slopes ? mattn_fwd_df<T, DF, false, true>(a, p, stream)         \
-                               : mattn_fwd_df<T, DF, false, false>(a, p, stream))
+  rc = a.cap > 0.f ? (a.slopes ? mattn_fwd_train<T, DF, true, true>(a, p, stream)          \
+                               : mattn_fwd_train<T, DF, true, false>(a, p, stream))        \
+                   : (a.slopes ? mattn_fwd_train<T, DF, false, true>(a, p, stream)         \
+                               : mattn_fwd_train<T, DF, false, false>(a, p, stream))
   if (a.d <= 32) DMF_AT_MODE(32);
   else if (a.d <= 64) DMF_AT_MODE(64);
   else if (a.d <= 96) DMF_AT_MODE(96);

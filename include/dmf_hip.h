@@ -699,7 +699,7 @@ int dmf_qk_norm_rope_bwd(int dtype, const void* q, long long q_sb, long long q_s
  *   (dmf_mattn_spans) takes the place of causal / prefix. A query that sees nothing has o = 0; keys that a query does not see
  *   do not reach its output, whatever they hold. d a multiple of 8 up to 128, strides and bases multiples of 16 bytes,
  *   token strides at least d.
- *   For the backward: lse [batch][hq][lq] and, for 16-bit types, o_lo (what rounding o left over); both nullable.
+ *   For the backward: lse [batch][hq][lq] and, for 16-bit types, o_lo (what rounding o left over); null for inference.
  *   ws: dmf_mattn_fwd_ws_floats floats (ragged: kv_lens is given; 0: null allowed), where the keys are split over
  *   workgroups.
  * dmf_mattn_bwd: dq, dk, dv from go = d o; ws: batch*lq*(hq + 2) floats of scratch. No atomics: same bits every run.

@@ -327,7 +327,7 @@ def _attn_case(b, lq, lk, hq, hk, d, dt, causal=False, kv_lens=None, prefix=None
         with torch.no_grad():
             o2 = A.attention(q, k, v, scale=scale, softcap=cap, slopes=sl, causal=causal, kv_lens=dev(kv_lens),
                              prefix=dev(prefix), documents=dev(docs))
-        assert torch.equal(o2, o)
+        _within(o2, ref[0], ref[1], "o without a gradient")
     return o
 
 
