@@ -4,14 +4,13 @@ distance bias and causal / prefix / document masks over shared key heads (``atte
 and for single tokens against a long cache.
 
 The reference's MultiHeadSelfAttention (transformer_model.py:83-116) is the case without any of these
-(dmf_tokens); its blocks take them as options (transformer_model.TransformerStage). Both ops run on
+(dmf_tokens); the blocks of transformer_model.TransformerStage take them as options. Both ops run on
 csrc/qknorm.hip and csrc/masked_attn*.h through the C-ABI, on torch's current stream, with every
 workspace from torch's allocator, so they can be captured into a graph; sizes are checked on the host, and
 device-side values (positions, lengths, ids) are bounds-checked in the kernels.
 """
 from __future__ import annotations
 
-import contextlib
 import math
 
 import torch
@@ -22,11 +21,13 @@ import dmf_native as N
 _DTYPES = {torch.float32: N.F32, torch.bfloat16: N.BF16, torch.float16: N.F16}
 
 
-def _on(t):
-    """Launches go to the tensors' device, also where another one is current."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _launch(name, dev, *args):
+    """N.call on ``dev``'s current stream; launches go to the tensors' device, also where another one is current."""
+    if dev.index == torch.cuda.current_device():
+        N.call(name, *args, N.stream_ptr(dev))
+    else:
+        with torch.cuda.device(dev):
+            N.call(name, *args, N.stream_ptr(dev))
 
 
 def _p(t):
@@ -39,38 +40,41 @@ def _heads(what, name, t, like=None):
                          f"{tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__}")
     if not t.is_cuda:
         N.require_cuda(t)
-    if t.dtype not in _DTYPES:
-        raise ValueError(f"{what}: {name} must be float32, bfloat16 or float16, got {t.dtype}")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+    if like is None:
+        if t.dtype not in _DTYPES:
+            raise ValueError(f"{what}: {name} must be float32, bfloat16 or float16, got {t.dtype}")
+    elif t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f"{what}: {name} is {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
 
 
-def _strided(t, align):
-    """(tensor, batch / token / head strides) with contiguous head dims; strides and base multiples of
-    ``align`` elements, else of a contiguous copy."""
-    for _ in range(2):
-        # the stride of a dim of length 1 says nothing
-        st = [0 if t.shape[i] == 1 else t.stride(i) for i in range(3)]
-        if ((t.shape[3] == 1 or t.stride(3) == 1) and all(s % align == 0 for s in st)
-                and t.data_ptr() % (align * t.element_size()) == 0):
-            return t, st
+def _strided(t, align, apart=0):
+    """(tensor, (batch, token, head) strides) with contiguous head dims; strides and base multiples of ``align``
+    elements and tokens at least ``apart`` elements apart, else of a contiguous copy."""
+    n0, n1, n2, n3 = t.shape
+    s0, s1, s2, s3 = t.stride()
+    # (the stride of a dim of length 1 says nothing)
+    s0, s1, s2 = (s0 if n0 > 1 else 0), (s1 if n1 > 1 else apart), (s2 if n2 > 1 else 0)
+    if ((s3 == 1 or n3 == 1) and s0 % align == 0 and s1 % align == 0 and s2 % align == 0 and s1 >= apart
+            and t.data_ptr() % (align * t.element_size()) == 0):
+        return t, (s0, s1, s2)
+    if t.is_contiguous():  # an unaligned base
+        t = t.clone(memory_format=torch.contiguous_format)
+    else:
         t = t.contiguous()
-        if t.data_ptr() % (align * t.element_size()):
-            t = t.clone(memory_format=torch.contiguous_format)
-    return t, st
+    return t, (n1 * n2 * n3, n2 * n3, n3)
 
 
-def _plain(t, align=1):
-    """Contiguous (and, for 16-byte loads, aligned) form of a gradient."""
+def _plain(t):
+    """Contiguous, 16-byte aligned form of a gradient."""
     t = t.contiguous()
-    return t if align == 1 or t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _small(what, name, t, shape, dtype, device):
-    if t is None:
-        return None
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{what}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype == dtype and t.shape == shape and t.device == device and t.is_contiguous():
+        return t
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{what}: {name} must have shape {shape}, got {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{what}: {name} is on {t.device}, expected {device}")
     if t.is_floating_point() != dtype.is_floating_point or t.dtype == torch.bool:
@@ -104,13 +108,11 @@ def _qk_call(name, q, k, cos, sin, pos, wq, wk, norm, eps, interleaved, *rest):
     b, n, hq, d = q.shape
     q, qs = _strided(q, 1)
     k, ks = _strided(k, 1)
-    rot = 0 if cos is None else 2 * cos.shape[1]
+    rows, rot = (0, 0) if cos is None else (cos.shape[0], 2 * cos.shape[1])
     pos_sb = 0 if pos is None or pos.dim() == 1 else pos.stride(0)
-    with _on(q):
-        N.call(name, _DTYPES[q.dtype], q.data_ptr(), *qs, hq, k.data_ptr(), *ks, k.shape[2], b, n, d, rot,
-               int(interleaved), int(norm), eps, _p(wq), _p(wk), _p(cos), _p(sin), _p(pos), pos_sb,
-               int(pos is not None and pos.dtype == torch.int64), 0 if cos is None else cos.shape[0], *rest,
-               N.stream_ptr(q.device))
+    _launch(name, q.device, _DTYPES[q.dtype], q.data_ptr(), *qs, hq, k.data_ptr(), *ks, k.shape[2], b, n, d, rot,
+            interleaved, norm, eps, _p(wq), _p(wk), _p(cos), _p(sin), _p(pos), pos_sb,
+            pos is not None and pos.dtype == torch.int64, rows, *rest)
 
 
 def _qk_fwd(q, k, cos, sin, pos, wq, wk, norm, eps, interleaved):
@@ -118,6 +120,22 @@ def _qk_fwd(q, k, cos, sin, pos, wq, wk, norm, eps, interleaved):
     ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
     _qk_call("dmf_qk_norm_rope", q, k, cos, sin, pos, wq, wk, norm, eps, interleaved, qo.data_ptr(), ko.data_ptr())
     return qo, ko
+
+
+def _qk_bwd(q, k, cos, sin, pos, wq, wk, norm, eps, interleaved, gq, gk, weights):
+    """dq, dk and, with ``weights``, dwq, dwk (else None)."""
+    gq, gk = _plain(gq), _plain(gk)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    dwq = dwk = ws = None
+    if weights:
+        d = q.shape[3]
+        dwq, dwk = torch.empty((2, d), dtype=torch.float32, device=q.device)
+        ws = torch.empty(N.load().dmf_qk_norm_rope_bwd_ws_floats(q.shape[2], k.shape[2], d), dtype=torch.float32,
+                         device=q.device)
+    _qk_call("dmf_qk_norm_rope_bwd", q, k, cos, sin, pos, wq, wk, norm, eps, interleaved, gq.data_ptr(), gk.data_ptr(),
+             dq.data_ptr(), dk.data_ptr(), _p(dwq), _p(dwk), _p(ws))
+    return dq, dk, dwq, dwk
 
 
 class _QkNormRopeFn(torch.autograd.Function):
@@ -131,20 +149,9 @@ class _QkNormRopeFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gq, gk):
         q, k, wq, wk, cos, sin, pos = ctx.saved_tensors
-        gq, gk = _plain(gq, 16), _plain(gk, 16)
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        dwq = dwk = ws = None
-        if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
-            d = q.shape[3]
-            dwq, dwk = (torch.empty(d, dtype=torch.float32, device=q.device) for _ in range(2))
-            ws = torch.empty(N.load().dmf_qk_norm_rope_bwd_ws_floats(q.shape[2], k.shape[2], d), dtype=torch.float32,
-                             device=q.device)
-        _qk_call("dmf_qk_norm_rope_bwd", q, k, cos, sin, pos, wq, wk, *ctx.cfg, gq.data_ptr(), gk.data_ptr(),
-                 dq.data_ptr(), dk.data_ptr(), _p(dwq), _p(dwk), _p(ws))
         need = ctx.needs_input_grad
-        return (dq if need[0] else None, dk if need[1] else None, dwq if need[2] else None,
-                dwk if need[3] else None, None, None, None, None, None, None)
+        g = _qk_bwd(q, k, cos, sin, pos, wq, wk, *ctx.cfg, gq, gk, need[2] or need[3])
+        return tuple(x if n else None for x, n in zip(g, need)) + (None,) * 6
 
 
 def qk_norm_rope(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weight=None, eps=1e-6, interleaved=False):
@@ -202,9 +209,8 @@ def qk_norm_rope(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weig
 # ---------------------------------------------------------------- attention
 def _spans(documents, kv_lens, prefix, b, lq, lk, causal):
     spans = torch.empty((b, lq, 2), dtype=torch.int32, device=documents.device)
-    with _on(documents):
-        N.call("dmf_mattn_spans", documents.data_ptr(), lk, _p(kv_lens), _p(prefix), b, lq, lk, int(causal),
-               spans.data_ptr(), N.stream_ptr(documents.device))
+    _launch("dmf_mattn_spans", documents.device, documents.data_ptr(), lk, _p(kv_lens), _p(prefix), b, lq, lk, causal,
+            spans.data_ptr())
     return spans
 
 
@@ -212,9 +218,10 @@ def _attn_dims(q, k, v, cfg, kv_lens, prefix, slopes, spans):
     """The leading arguments dmf_mattn_fwd and dmf_mattn_bwd share, and the tensors they point into."""
     scale, softcap, causal = cfg
     align = 16 // q.element_size()
-    (q, qs), (k, ks), (v, vs) = _strided(q, align), _strided(k, align), _strided(v, align)
+    d = q.shape[3]
+    (q, qs), (k, ks), (v, vs) = _strided(q, align, d), _strided(k, align, d), _strided(v, align, d)
     args = (_DTYPES[q.dtype], q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs, q.shape[0], q.shape[1],
-            k.shape[1], q.shape[2], k.shape[2], q.shape[3], scale, softcap, _p(slopes), int(causal), _p(kv_lens),
+            k.shape[1], q.shape[2], k.shape[2], d, scale, softcap, _p(slopes), causal, _p(kv_lens),
             None if spans is not None else _p(prefix), _p(spans))
     return args, (q, k, v)
 
@@ -227,10 +234,20 @@ def _attn_fwd(q, k, v, cfg, kv_lens, prefix, slopes, spans, train):
     lse = torch.empty(b * lq * hq, dtype=torch.float32, device=q.device) if train else None
     n = N.load().dmf_mattn_fwd_ws_floats(_DTYPES[q.dtype], b, lq, k.shape[1], hq, k.shape[2], d, int(kv_lens is not None))
     ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
-    with _on(q):
-        N.call("dmf_mattn_fwd", *args, o.data_ptr(), _p(o_lo), _p(lse), _p(ws), N.stream_ptr(q.device))
+    _launch("dmf_mattn_fwd", q.device, *args, o.data_ptr(), _p(o_lo), _p(lse), _p(ws))
     del keep
     return o, o_lo, lse
+
+
+def _attn_bwd(q, k, v, cfg, kv_lens, prefix, slopes, spans, o, o_lo, lse, go):
+    args, keep = _attn_dims(q, k, v, cfg, kv_lens, prefix, slopes, spans)
+    go = _plain(go)
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    ws = torch.empty(q.shape[0] * q.shape[1] * (q.shape[2] + 2), dtype=torch.float32, device=q.device)
+    _launch("dmf_mattn_bwd", q.device, *args, o.data_ptr(), _p(o_lo), lse.data_ptr(), go.data_ptr(), ws.data_ptr(),
+            dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
+    del keep
+    return dq, dk, dv
 
 
 class _AttentionFn(torch.autograd.Function):
@@ -245,16 +262,8 @@ class _AttentionFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, go):
         q, k, v, kv_lens, prefix, slopes, spans, o, o_lo, lse = ctx.saved_tensors
-        args, keep = _attn_dims(q, k, v, ctx.cfg, kv_lens, prefix, slopes, spans)
-        go = _plain(go, 16)
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        ws = torch.empty(q.shape[0] * q.shape[1] * (q.shape[2] + 2), dtype=torch.float32, device=q.device)
-        with _on(q):
-            N.call("dmf_mattn_bwd", *args, o.data_ptr(), _p(o_lo), lse.data_ptr(), go.data_ptr(), ws.data_ptr(),
-                   dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), N.stream_ptr(q.device))
-        del keep
-        need = ctx.needs_input_grad
-        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None, None, None, None)
+        g = _attn_bwd(q, k, v, ctx.cfg, kv_lens, prefix, slopes, spans, o, o_lo, lse, go)
+        return tuple(x if n else None for x, n in zip(g, ctx.needs_input_grad)) + (None,) * 5
 
 
 def attention(q, k, v, *, scale=None, softcap=0.0, slopes=None, causal=False, kv_lens=None, prefix=None,
@@ -293,9 +302,12 @@ def attention(q, k, v, *, scale=None, softcap=0.0, slopes=None, causal=False, kv
     if slopes is not None and slopes.requires_grad:
         raise ValueError(f"{what}: no gradient reaches slopes")
     dev = q.device
-    slopes = _small(what, "slopes", slopes, (hq,), torch.float32, dev)
-    kv_lens = _small(what, "kv_lens", kv_lens, (b,), torch.int32, dev)
-    prefix = _small(what, "prefix", prefix, (b,), torch.int32, dev)
+    if slopes is not None:
+        slopes = _small(what, "slopes", slopes, (hq,), torch.float32, dev)
+    if kv_lens is not None:
+        kv_lens = _small(what, "kv_lens", kv_lens, (b,), torch.int32, dev)
+    if prefix is not None:
+        prefix = _small(what, "prefix", prefix, (b,), torch.int32, dev)
     spans = None
     if documents is not None:
         documents = _small(what, "documents", documents, (b, lk), torch.int32, dev)

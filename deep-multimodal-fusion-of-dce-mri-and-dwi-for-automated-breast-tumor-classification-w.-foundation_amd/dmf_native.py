@@ -122,7 +122,7 @@ def load():
 
 def call(name, *args):
     """Invoke a C-ABI entry point; raise RuntimeError on a non-zero status."""
-    lib = load()
+    lib = _lib or load()
     rc = getattr(lib, name)(*args)
     if rc != 0:
         msg = lib.dmf_last_error().decode(errors="replace")
@@ -142,8 +142,14 @@ class BnDesc(ctypes.Structure):
 
 
 def stream_ptr(device=None):
-    """hipStream_t of torch's current stream (graph-capture aware)."""
-    return torch.cuda.current_stream(device).cuda_stream
+    """hipStream_t of torch's current stream (graph-capture aware); of ``device``, an index, a torch.device or None
+    for the current one."""
+    if isinstance(device, torch.device):
+        device = device.index
+    if device is None:
+        device = torch.cuda.current_device()
+    # (what torch.cuda.current_stream(device).cuda_stream is, without the Stream object: 0.1 instead of 2 us)
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def ptr(t):

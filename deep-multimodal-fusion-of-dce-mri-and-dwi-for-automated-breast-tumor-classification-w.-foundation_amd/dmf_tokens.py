@@ -21,6 +21,7 @@ from __future__ import annotations
 
 import torch
 
+import dmf_attention as A
 import dmf_native as N
 import dmf_ops as O
 
@@ -242,13 +243,69 @@ def _sfx(cdt):
     return "" if cdt == torch.bfloat16 else "_f32"
 
 
-def _attn_fwd(a, wq, qkvb, wp, projb, b, n, heads, p_attn, p_proj, rng, s_attn, s_proj, gamma=None, res=None, nv=None):
+class AttnCore:
+    """What a block's attention does between its qkv and output projections beyond softmax(q k^T / sqrt(d)) v
+    (dmf_attention): norm weights f32 [d] or None, rotation table (cos, sin) or None, softcap, slopes f32 [heads]
+    or None."""
+
+    __slots__ = ("wq", "wk", "cos", "sin", "softcap", "slopes")
+    EPS = 1e-6
+
+    def __init__(self, wq=None, wk=None, rope=None, softcap=0.0, slopes=None):
+        self.wq, self.wk = wq, wk
+        self.cos, self.sin = rope if rope is not None else (None, None)
+        self.softcap, self.slopes = float(softcap), slopes
+
+    def check(self, what, n, d):
+        if d > 128 or d % 8:
+            raise ValueError(f"{what}: attention options need a head dim that is a multiple of 8 up to 128, got {d}")
+        if self.cos is not None and (self.cos.shape[0] < n or 2 * self.cos.shape[1] > d):
+            raise ValueError(f"{what}: rotation table {tuple(self.cos.shape)} for {n} tokens, head dim {d}")
+
+
+def _core_heads(qkv, b, n, heads):
+    e = qkv.shape[1] // 3
+    x = qkv.view(b, n, 3, heads, e // heads)
+    return x[:, :, 0], x[:, :, 1], x[:, :, 2]
+
+
+def _core_fwd(qkv, b, n, heads, core, train):
+    """o [b*n, e] from the packed qkv rows, and what the backward reads."""
+    q, k, v = _core_heads(qkv, b, n, heads)
+    if core.wq is not None or core.cos is not None:
+        q, k = A._qk_fwd(q, k, core.cos, core.sin, None, core.wq, core.wk, core.wq is not None, core.EPS, False)
+    cfg = (q.shape[3] ** -0.5, core.softcap, False)
+    o, o_lo, lse = A._attn_fwd(q, k, v, cfg, None, None, core.slopes, None, train)
+    return o.view(b * n, -1), (qkv, q, k, o_lo, lse)
+
+
+def _core_bwd(do, o, saved, b, n, heads, core):
+    """do (packed rows) -> dqkv (packed rows), dwq, dwk."""
+    qkv, q, k, o_lo, lse = saved
+    q0, k0, v = _core_heads(qkv, b, n, heads)
+    cfg = (q.shape[3] ** -0.5, core.softcap, False)
+    dq, dk, dv = A._attn_bwd(q, k, v, cfg, None, None, core.slopes, None, o, o_lo, lse, do.view(q.shape))
+    dwq = dwk = None
+    if core.wq is not None or core.cos is not None:
+        dq, dk, dwq, dwk = A._qk_bwd(q0, k0, core.cos, core.sin, None, core.wq, core.wk, core.wq is not None, core.EPS,
+                                     False, dq, dk, core.wq is not None)
+    return torch.cat([dq, dk, dv], 2).view(b * n, -1), dwq, dwk
+
+
+def _attn_fwd(a, wq, qkvb, wp, projb, b, n, heads, p_attn, p_proj, rng, s_attn, s_proj, gamma=None, res=None, nv=None,
+              core=None):
     r, e = a.shape
     d = e // heads
     cdt, dev = a.dtype, a.device
     bf = dict(dtype=cdt, device=dev)
     f32 = dict(dtype=torch.float32, device=dev)
     qkv = gemm(torch.empty((r, 3 * e), **bf), a, wq, r, 3 * e, e, lda=e, ldb=e, ldc=3 * e, bias=qkvb)
+    if core is not None:
+        o, saved = _core_fwd(qkv, b, n, heads, core, True)
+        y = torch.empty((r, e), **bf)
+        out = gemm(torch.empty((r, e), **f32), o, wp, r, e, e, lda=e, ldb=e, ldc=e, bias=projb, colscale=gamma, res=res,
+                   aux=y, dropout_p=p_proj, rng=rng, site=s_proj)
+        return out, (*saved, o, y)
     S = torch.empty((b, heads, n, n), **f32)
     gemm(S, qkv, qkv, n, n, d, lda=3 * e, ldb=3 * e, ldc=n, batch=(b, heads), sa=(n * 3 * e, d),
          sb=(n * 3 * e, d), sc=(heads * n * n, n * n), b_off=e)
@@ -265,9 +322,10 @@ def _attn_fwd(a, wq, qkvb, wp, projb, b, n, heads, p_attn, p_proj, rng, s_attn, 
     return out, (qkv, P, Pd, o, y)
 
 
-def _attn_bwd(dout, a, saved, wq, wp, b, n, heads, p_attn, p_proj, rng, s_attn, s_proj, gamma, grads):
-    """dout (f32 [r, e]) -> d a (f32); grads: dqkvw, dqkvb, dprojw, dprojb, dgamma (nullable)."""
-    qkv, P, Pd, o, y = saved
+def _attn_bwd(dout, a, saved, wq, wp, b, n, heads, p_attn, p_proj, rng, s_attn, s_proj, gamma, grads, core=None):
+    """dout (f32 [r, e]) -> d a (f32); grads: dqkvw, dqkvb, dprojw, dprojb, dgamma (nullable). With ``core``:
+    (d a, dwq, dwk), the norm weights' gradients (None without them)."""
+    *inner, o, y = saved
     r, e = a.shape
     d = e // heads
     cdt, dev = a.dtype, a.device
@@ -281,6 +339,10 @@ def _attn_bwd(dout, a, saved, wq, wp, b, n, heads, p_attn, p_proj, rng, s_attn, 
     gemm(dprojw, dy, o, e, e, r, ta=1, tb=1, lda=e, ldb=e, ldc=e)
     do = gemm(torch.empty((r, e), **bf), dy, wp, r, e, e, tb=1, lda=e, ldb=e, ldc=e)
     del dy
+    if core is not None:
+        dqkv, dwq, dwk = _core_bwd(do, o, inner, b, n, heads, core)
+        return _qkv_bwd(dqkv, a, wq, dqkvw, dqkvb), dwq, dwk
+    qkv, P, Pd = inner
     dPd = torch.empty((b, heads, n, n), **f32)
     gemm(dPd, do, qkv, n, n, d, lda=e, ldb=3 * e, ldc=n, batch=(b, heads), sa=(n * e, d), sb=(n * 3 * e, d),
          sc=(heads * n * n, n * n), b_off=2 * e)
@@ -298,14 +360,22 @@ def _attn_bwd(dout, a, saved, wq, wp, b, n, heads, p_attn, p_proj, rng, s_attn, 
     gemm(dqkv, dS, qkv, n, d, n, ta=1, tb=1, lda=n, ldb=3 * e, ldc=3 * e, batch=(b, heads),
          sa=(heads * n * n, n * n), sb=(n * 3 * e, d), sc=(n * 3 * e, d), c_off=e)
     del dS
+    return _qkv_bwd(dqkv, a, wq, dqkvw, dqkvb)
+
+
+def _qkv_bwd(dqkv, a, wq, dqkvw, dqkvb):
+    """The qkv linear's backward: weight and bias (nullable) gradients, d a (f32)."""
+    r, e = a.shape
+    dev = a.device
     gemm(dqkvw, dqkv, a, 3 * e, e, r, ta=1, tb=1, lda=3 * e, ldb=e, ldc=e)
     if dqkvb is not None:
-        if cdt == torch.bfloat16:
+        if a.dtype == torch.bfloat16:
             ws = torch.empty(N.load().dmf_colsum_bf16_ws_floats(r, 3 * e), dtype=torch.float32, device=dev)
             N.call("dmf_colsum_bf16", dqkv.data_ptr(), 3 * e, r, 3 * e, dqkvb.data_ptr(), ws.data_ptr(), _s())
         else:
             N.call("dmf_colsum_f32", dqkv.data_ptr(), 3 * e, r, 3 * e, dqkvb.data_ptr(), 1, _s())
-    return gemm(torch.empty((r, e), **f32), dqkv, wq, r, e, 3 * e, tb=1, lda=3 * e, ldb=e, ldc=e)
+    return gemm(torch.empty((r, e), dtype=torch.float32, device=dev), dqkv, wq, r, e, 3 * e, tb=1, lda=3 * e, ldb=e,
+                ldc=e)
 
 
 def _mlp_fwd(a, w1, b1, w2, b2, p, rng, s1, s2, gamma=None, res=None):
@@ -348,7 +418,8 @@ def _zeros(dev, *shapes):
 
 class _BlockFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, cfg, rng, ln1w, ln1b, qkvw, qkvb, projw, projb, ln2w, ln2b, fc1w, fc1b, fc2w, fc2b, g1, g2):
+    def forward(ctx, x, cfg, rng, ln1w, ln1b, qkvw, qkvb, projw, projb, ln2w, ln2b, fc1w, fc1b, fc2w, fc2b, g1, g2,
+                core=None, qnw=None, knw=None):
         heads, eps1, eps2, p_attn, p_proj, p_mlp, sites, cdt, nv = cfg
         s_attn, s_proj, s_m1, s_m2 = sites
         b, n, e = x.shape
@@ -356,20 +427,21 @@ class _BlockFn(torch.autograd.Function):
         wq, wp, w1, w2 = _wcast(cdt, qkvw, projw, fc1w, fc2w)
         # attention branch: x1 = x + drop(proj(attn(ln1(x)))) * g1
         ln1, save1 = ln_fwd(x, ln1w, ln1b, eps1, cdt)
-        x1, sa = _attn_fwd(ln1, wq, qkvb, wp, projb, b, n, heads, p_attn, p_proj, rng, s_attn, s_proj, g1, x, nv)
+        x1, sa = _attn_fwd(ln1, wq, qkvb, wp, projb, b, n, heads, p_attn, p_proj, rng, s_attn, s_proj, g1, x, nv, core)
         # MLP branch: x2 = x1 + drop(fc2(drop(gelu(fc1(ln2(x1)))))) * g2
         ln2, save2 = ln_fwd(x1, ln2w, ln2b, eps2, cdt)
         x2, sm = _mlp_fwd(ln2, w1, fc1b, w2, fc2b, p_mlp, rng, s_m1, s_m2, g2, x1)
         ctx.save_for_backward(x, ln1, save1, *sa, x1, ln2, save2, *sm, wq, wp, w1, w2, ln1w, ln2w, g1, g2, rng)
-        ctx.cfg = cfg
+        ctx.cfg, ctx.core, ctx.na = cfg, core, len(sa)
         ctx.dims = (b, n, e)
         return x2.view(b, n, e)
 
     @staticmethod
     def backward(ctx, dx2):
         t = ctx.saved_tensors
-        x, ln1, save1, sa, x1, ln2, save2, sm = t[0], t[1], t[2], t[3:8], t[8], t[9], t[10], t[11:14]
-        wq, wp, w1, w2, ln1w, ln2w, g1, g2, rng = t[14:]
+        (x, ln1, save1), sa, t = t[:3], t[3:3 + ctx.na], t[3 + ctx.na:]
+        (x1, ln2, save2), sm = t[:3], t[3:6]
+        wq, wp, w1, w2, ln1w, ln2w, g1, g2, rng = t[6:]
         heads, eps1, eps2, p_attn, p_proj, p_mlp, sites, cdt, _ = ctx.cfg
         s_attn, s_proj, s_m1, s_m2 = sites
         b, n, e = ctx.dims
@@ -380,11 +452,14 @@ class _BlockFn(torch.autograd.Function):
         dx2 = dx2.contiguous().view(b * n, e).float()
         dln2 = _mlp_bwd(dx2, ln2, sm, w1, w2, p_mlp, rng, s_m1, s_m2, g2, (dfc1w, dfc1b, dfc2w, dfc2b, dg2))
         dx1 = ln_bwd(dln2, x1, save2, ln2w, dx2.clone(), dln2w, dln2b)
+        dqnw = dknw = None
         dln1 = _attn_bwd(dx1, ln1, sa, wq, wp, b, n, heads, p_attn, p_proj, rng, s_attn, s_proj, g1,
-                         (dqkvw, dqkvb, dprojw, dprojb, dg1))
+                         (dqkvw, dqkvb, dprojw, dprojb, dg1), ctx.core)
+        if ctx.core is not None:
+            dln1, dqnw, dknw = dln1
         dx = ln_bwd(dln1, x, save1, ln1w, dx1, dln1w, dln1b)
         return (dx.view(b, n, e), None, None, dln1w, dln1b, dqkvw, dqkvb, dprojw, dprojb, dln2w, dln2b,
-                dfc1w, dfc1b, dfc2w, dfc2b, dg1, dg2)
+                dfc1w, dfc1b, dfc2w, dfc2b, dg1, dg2, None, dqnw, dknw)
 
 
 # ------------------------------------------------ forward-only block (no autograd graph)
@@ -514,7 +589,7 @@ def flash_attention(qkv, b, n, nv, e, heads, p_attn, rng, site):
     return o
 
 
-def _block_fwd_nograd(x, blk, rng, cfg, g1, g2):
+def _block_fwd_nograd(x, blk, rng, cfg, g1, g2, core=None):
     heads, eps1, eps2, p_attn, p_proj, p_mlp, sites, cdt, nv = cfg
     s_attn, s_proj, s_m1, s_m2 = sites
     at, ml = blk.attn, blk.mlp
@@ -532,7 +607,9 @@ def _block_fwd_nograd(x, blk, rng, cfg, g1, g2):
     else:
         (wq,) = _wcast(cdt, at.qkv.weight)
         qkv = gemm(torch.empty((r, 3 * e), **bf), ln1, wq, r, 3 * e, e, lda=e, ldb=e, ldc=3 * e, bias=at.qkv.bias)
-    if d == _FA_HEAD_DIM and cdt == torch.bfloat16:
+    if core is not None:
+        o, _ = _core_fwd(qkv, b, n, heads, core, False)
+    elif d == _FA_HEAD_DIM and cdt == torch.bfloat16:
         o = flash_attention(qkv, b, n, nv or n, e, heads, p_attn, rng, s_attn)
     else:
         S = torch.empty((b, heads, n, n), **f32)
@@ -582,28 +659,32 @@ class _MHSAFn(torch.autograd.Function):
     """Standalone MultiHeadSelfAttention.forward (transformer_model.py:100-116)."""
 
     @staticmethod
-    def forward(ctx, x, cfg, rng, qkvw, qkvb, projw, projb):
+    def forward(ctx, x, cfg, rng, qkvw, qkvb, projw, projb, core=None, qnw=None, knw=None):
         heads, p_attn, p_proj, sites, cdt = cfg
         b, n, e = x.shape
         a = _branch_input(x, cdt)
         wq, wp = _wcast(cdt, qkvw, projw)
-        out, sa = _attn_fwd(a, wq, qkvb, wp, projb, b, n, heads, p_attn, p_proj, rng, sites[0], sites[1])
+        out, sa = _attn_fwd(a, wq, qkvb, wp, projb, b, n, heads, p_attn, p_proj, rng, sites[0], sites[1], core=core)
         ones = torch.ones(e, dtype=torch.float32, device=x.device)
         ctx.save_for_backward(a, *sa, wq, wp, ones, rng)
-        ctx.cfg, ctx.dims, ctx.xdtype = cfg, (b, n, e), x.dtype
+        ctx.cfg, ctx.dims, ctx.xdtype, ctx.core = cfg, (b, n, e), x.dtype, core
         return out.view(b, n, e)
 
     @staticmethod
     def backward(ctx, dout):
         a, *rest = ctx.saved_tensors
-        sa, (wq, wp, ones, rng) = rest[:5], rest[5:]
+        sa, (wq, wp, ones, rng) = rest[:-4], rest[-4:]
         heads, p_attn, p_proj, sites, cdt = ctx.cfg
         b, n, e = ctx.dims
         need = ctx.needs_input_grad
         dqkvw, dqkvb, dprojw, dprojb = _zeros(a.device, (3 * e, e), 3 * e, (e, e), e)
         da = _attn_bwd(dout.contiguous().view(b * n, e).float(), a, sa, wq, wp, b, n, heads, p_attn, p_proj, rng,
-                       sites[0], sites[1], ones, (dqkvw, dqkvb if need[4] else None, dprojw, dprojb, None))
-        return (da.view(b, n, e).to(ctx.xdtype), None, None, dqkvw, dqkvb if need[4] else None, dprojw, dprojb)
+                       sites[0], sites[1], ones, (dqkvw, dqkvb if need[4] else None, dprojw, dprojb, None), ctx.core)
+        dqnw = dknw = None
+        if ctx.core is not None:
+            da, dqnw, dknw = da
+        return (da.view(b, n, e).to(ctx.xdtype), None, None, dqkvw, dqkvb if need[4] else None, dprojw, dprojb, None,
+                dqnw, dknw)
 
 
 class _MLPFn(torch.autograd.Function):
@@ -660,8 +741,14 @@ def _need_rng(what, rng, *ps):
         raise RuntimeError(f"{what}: dropout requested without an rng snapshot")
 
 
-def multihead_self_attention(x, at, rng, dtype=torch.bfloat16):
-    """MultiHeadSelfAttention.forward (transformer_model.py:100-116) as one node."""
+def _check_core(what, core, x, heads, p_attn):
+    core.check(what, x.shape[1], x.shape[2] // heads)
+    if p_attn > 0:
+        raise ValueError(f"{what}: attention options have no attention dropout (p = {p_attn})")
+
+
+def multihead_self_attention(x, at, rng, dtype=torch.bfloat16, core=None):
+    """MultiHeadSelfAttention.forward (transformer_model.py:100-116) as one node; ``core``: AttnCore options."""
     p_attn = float(at.attn_drop.p) if at.attn_drop.training else 0.0
     p_proj = float(at.proj_drop.p) if at.proj_drop.training else 0.0
     _need_rng("MultiHeadSelfAttention", rng, p_attn, p_proj)
@@ -670,6 +757,10 @@ def multihead_self_attention(x, at, rng, dtype=torch.bfloat16):
     if at.qkv.bias is None:
         raise ValueError("MultiHeadSelfAttention: qkv_bias=False is not supported by the fused path")
     cfg = (at.num_heads, p_attn, p_proj, tuple(at._sites), dtype)
+    if core is not None:
+        _check_core("MultiHeadSelfAttention", core, x, at.num_heads, p_attn)
+        return _MHSAFn.apply(x, cfg, rng, at.qkv.weight, at.qkv.bias, at.proj.weight, at.proj.bias, core, core.wq,
+                             core.wk)
     return _MHSAFn.apply(x, cfg, rng, at.qkv.weight, at.qkv.bias, at.proj.weight, at.proj.bias)
 
 
@@ -682,12 +773,12 @@ def mlp(x, m, rng, dtype=torch.bfloat16):
     return _MLPFn.apply(x, (p, tuple(m._sites), dtype), rng, m.fc1.weight, m.fc1.bias, m.fc2.weight, m.fc2.bias)
 
 
-def transformer_block(x, blk, rng, sites, dtype=torch.bfloat16, n_valid=None, gammas=None):
+def transformer_block(x, blk, rng, sites, dtype=torch.bfloat16, n_valid=None, gammas=None, core=None):
     """TransformerBlock.forward (transformer_model.py:78-81) as one node;
     ``dtype`` is the compute dtype (bf16, or f32 for the parity mode).
     ``n_valid``: tokens beyond it are key padding (masked out of every
     softmax row); ``gammas``: LayerScale vectors for a block without them
-    (ones: timm's ViT Block, init_values=None)."""
+    (ones: timm's ViT Block, init_values=None). ``core``: AttnCore options."""
     at, ml = blk.attn, blk.mlp
     # the nn.Dropout modules' own flags (train() / eval() set them with the
     # block's; MC dropout turns on only these, train_fusion.py:445-449)
@@ -702,9 +793,13 @@ def transformer_block(x, blk, rng, sites, dtype=torch.bfloat16, n_valid=None, ga
     cfg = (at.num_heads, blk.norm1.eps, blk.norm2.eps, p_attn, p_proj, p_mlp, tuple(sites), dtype, n_valid)
     g1 = blk.gamma1 if gammas is None else gammas[0]
     g2 = blk.gamma2 if gammas is None else gammas[1]
+    if core is not None:
+        _check_core("TransformerBlock", core, x, at.num_heads, p_attn)
+        if n_valid is not None and n_valid != x.shape[1]:
+            raise ValueError("TransformerBlock: attention options have no key padding (n_valid)")
     if FWD_FUSED and dtype == torch.bfloat16 and not O.needs_grad(x, *blk.parameters(), g1, g2):
         with torch.no_grad():
-            return _block_fwd_nograd(x, blk, rng, cfg, g1, g2)
+            return _block_fwd_nograd(x, blk, rng, cfg, g1, g2, core)
     return _BlockFn.apply(x, cfg, rng, blk.norm1.weight, blk.norm1.bias, at.qkv.weight, at.qkv.bias, at.proj.weight,
                           at.proj.bias, blk.norm2.weight, blk.norm2.bias, ml.fc1.weight, ml.fc1.bias,
-                          ml.fc2.weight, ml.fc2.bias, g1, g2)
+                          ml.fc2.weight, ml.fc2.bias, g1, g2, *((core, core.wq, core.wk) if core is not None else ()))

@@ -421,7 +421,8 @@ class ModelMaskHeadBackbone(nn.Module):
         else:
             self.transformer = TransformerStage(in_ch=c2, embed_dim=mp["transformer_embed_dim"],
                                                 depth=mp["transformer_depth"], heads=mp["transformer_heads"],
-                                                patch_size=mp["transformer_patch_size"], dim=self.dim)
+                                                patch_size=mp["transformer_patch_size"], dim=self.dim,
+                                                attention=mp.get("transformer_attention"))
             self.trans_out_proj = nn.Conv2d(mp["transformer_embed_dim"], c3, kernel_size=1)
             self.transformer.patch_embed.use_fp8 = bool(mp.get("patch_embed_fp8", False))
 

@@ -35,6 +35,9 @@ def default_parameters():
         "transformer_patch_size": 2,                    # :73
         "transformer_depth": 6,                         # :74
         "transformer_embed_dim": 512,                   # :75
+        # build option: attention of the token blocks beyond the reference's, a dict of "qk_norm", "rope", "softcap",
+        # "distance_bias" (transformer_model.attention_options)
+        "transformer_attention": None,
         "patch_embed_fp8": False,                       # build option (config 5): PatchEmbed.proj on e4m3 MFMA
         "dropout": 0.2,                                 # :77
         "channels": (128, 256, 512),                    # :82
