@@ -79,7 +79,7 @@ template <typename T, int DF> struct AtBwdLds {
   static constexpr int KT = sizeof(T) == 4 ? 32 : 64;       // keys per tile of the row workgroups
   static constexpr int QTILE = AT_QT * RB, VT = 128 * RB;
   static constexpr int GROUP = 4 * QTILE + 2 * (int)sizeof(AtRowData);  // a group's stages
-  static constexpr int KEYS = VT + NG * GROUP, ROWS = 4 * KT * RB, ADD = NG > 1 ? 4 * 64 * DF / 2 * 4 : 0;
+  static constexpr int KEYS = VT + NG * GROUP, ROWS = 4 * KT * RB, ADD = NG > 1 ? 2 * 4 * 64 * DF / 2 * 4 : 0;
   static constexpr int MOST = KEYS > ROWS ? KEYS : ROWS;
   static constexpr int BYTES = (MOST > ADD ? MOST : ADD) + 16 * (int)sizeof(int);
 };
@@ -136,21 +136,6 @@ __device__ void at_query_alone(const AtArgs& a, int b, int kh, int r, int lo, in
   }
 }
 
-// one lane's column of a transposed accumulator, times `scale`, to its row of the output
-template <typename T, int DF>
-__device__ __forceinline__ void at_store_row(T* out, const at_f32x16* acc, int d, int h, float scale) {
-#pragma unroll
-  for (int f = 0; f < DF / 32; ++f)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int e = 32 * f + 8 * g + 4 * h;
-      if (e >= d) continue;
-      const float v[4] = {acc[f][4 * g] * scale, acc[f][4 * g + 1] * scale, acc[f][4 * g + 2] * scale,
-                          acc[f][4 * g + 3] * scale};
-      at_store4(out + e, v);
-    }
-}
-
 template <typename T, int DF, bool CAP, bool SLOPE>
 __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, char* smem) {
   typedef AtBwdLds<T, DF> L;
@@ -171,35 +156,40 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
   const int* w_lo = (const int*)a.rowws + nrows + (long long)b * a.lq;
   const int* w_hi = w_lo + nq;
   int q0 = 0x7fffffff, q1 = -1;
-  for (int i = threadIdx.x; i < a.lq; i += 1024 * NG) {
-    int lo[4], hi[4];
+  if (a.spans) {
+    for (int i = threadIdx.x; i < a.lq; i += 1024 * NG) {
+      int lo[4], hi[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int r = min(i + 256 * NG * u, a.lq - 1);
-      lo[u] = w_lo[r];
-      hi[u] = w_hi[r];
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (i + 256 * NG * u < a.lq && hi[u] > kb0 && lo[u] < kb0 + 128) {
-        q0 = min(q0, i + 256 * NG * u);
-        q1 = max(q1, i + 256 * NG * u);
+      for (int u = 0; u < 4; ++u) {
+        const int r = min(i + 256 * NG * u, a.lq - 1);
+        lo[u] = w_lo[r];
+        hi[u] = w_hi[r];
       }
-  }
-  q0 = at_wave_min(q0), q1 = at_wave_max(q1);
-  if (lane == 0) range[w8] = q0, range[8 + w8] = q1;
-  __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 4 * NG; ++w) q0 = min(q0, range[w]), q1 = max(q1, range[8 + w]);
-  q0 = __builtin_amdgcn_readfirstlane(q0);
-  q1 = __builtin_amdgcn_readfirstlane(q1);
+      for (int u = 0; u < 4; ++u)
+        if (i + 256 * NG * u < a.lq && hi[u] > kb0 && lo[u] < kb0 + 128) {
+          q0 = min(q0, i + 256 * NG * u);
+          q1 = max(q1, i + 256 * NG * u);
+        }
+    }
+    q0 = at_wave_min(q0), q1 = at_wave_max(q1);
+    if (lane == 0) range[w8] = q0, range[8 + w8] = q1;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4 * NG; ++w) q0 = min(q0, range[w]), q1 = max(q1, range[8 + w]);
+    q0 = __builtin_amdgcn_readfirstlane(q0);
+    q1 = __builtin_amdgcn_readfirstlane(q1);
+  } else {  // spans by position start at 0 and only widen: the last query, and the first whose end is past the keys' start
+    const int n = at_keys(a, b);
+    if (a.lq > 0 && at_span(a, b, a.lq - 1).hi > kb0) {
+      q1 = a.lq - 1;
+      // hi(i) = min(n, max(n - lq + i + 1, prefix)) under causal: past kb0 for all queries, or from i = kb0 - (n - lq)
+      q0 = at_span(a, b, 0).hi > kb0 ? 0 : max(kb0 - (n - a.lq), 0);
+    }
+    q0 = __builtin_amdgcn_readfirstlane(q0);
+    q1 = __builtin_amdgcn_readfirstlane(q1);
+  }
 
-  uint4 kf[KS];
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) {
-    const int e = (2 * ks + h) * AtT<T>::CH;
-    kf[ks] = key < a.lk && e < a.d ? *(const uint4*)(kb + key * a.k_sl + e) : make_uint4(0, 0, 0, 0);
-  }
   const AtLoad<T, DP, AT_QT, 4> ql(a.q_sl, a.d, wid, lane), gl((long long)a.hq * a.d, a.d, wid, lane);
   // wave w brings the tile's lse / delta / lo / hi
   const float* rv = wid == 0 ? a.lse : wid == 1 ? a.rowws : (const float*)(wid == 2 ? w_lo : w_hi);
@@ -215,12 +205,6 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
             lds0 + L::VT + grp * L::GROUP + 2 * STAGE + stage * (unsigned)sizeof(AtRowData) + wid * 256);
   };
 
-  at_f32x16 dk[FD], dv[FD];
-#pragma unroll
-  for (int f = 0; f < FD; ++f) dk[f] = at_zero(), dv[f] = at_zero();
-  const AtOffsets<T, DF> off(lane);
-  const char* V = smem + wid * 32 * L::RB;
-  const int n0 = (at_keys(a, b)) - a.lq;  // position of query 0
   // tiles of 32 queries, head after head; the groups take them in turn
   int g = 0, i0 = q0;  // the tile in hand: head (a.group or more: none), first query
   auto advance = [&](int n, int& hd, int& i) {
@@ -229,6 +213,24 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
       if (i > q1) i = q0, ++hd;
     }
   };
+  if (q1 >= 0) {  // (first: the rest of the set-up runs under the loads' latency)
+    advance(grp, g, i0);
+    if (g < a.group) issue(0, g, i0);
+    const AtLoad<T, DP, 128, 4 * NG> vl(a.v_sl, a.d, w8, lane);
+    vl.issue(vb, kb0, a.lk, lds0, w8);
+  }
+  uint4 kf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    const int e = (2 * ks + h) * AtT<T>::CH;
+    kf[ks] = key < a.lk && e < a.d ? *(const uint4*)(kb + key * a.k_sl + e) : make_uint4(0, 0, 0, 0);
+  }
+  at_f32x16 dk[FD], dv[FD];
+#pragma unroll
+  for (int f = 0; f < FD; ++f) dk[f] = at_zero(), dv[f] = at_zero();
+  const AtOffsets<T, DF> off(lane);
+  const char* V = smem + wid * 32 * L::RB;
+  const int n0 = (at_keys(a, b)) - a.lq;  // position of query 0
   const char* const base = smem + L::VT + grp * L::GROUP;
   auto step = [&](auto stage) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -280,10 +282,6 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
     g = g1, i0 = i1;
   };
   if (q1 >= 0) {
-    const AtLoad<T, DP, 128, 4 * NG> vl(a.v_sl, a.d, w8, lane);
-    vl.issue(vb, kb0, a.lk, lds0, w8);
-    advance(grp, g, i0);
-    if (g < a.group) issue(0, g, i0);
     // (uniform over the workgroup: the first group's count)
     const int nt = (a.group * ((q1 - q0) / AT_QT + 1) + NG - 1) / NG;
     for (int t = 0; t < nt; t += 2) {
@@ -291,39 +289,45 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
       if (t + 1 < nt) step(std::integral_constant<int, 1>{});
     }
   }
-  if constexpr (NG > 1) {  // the second group's sums through LDS, in two halves
-    float* sum = (float*)smem + wid * 64 * (DF / 2) + lane;
-    auto add = [&](at_f32x16* acc) {
-      __syncthreads();
-      if (grp == 1) {
+  if constexpr (NG > 1) {  // the groups' sums through LDS: dK's to the first group, dV's to the second
+    float* sum = (float*)smem + (w8 & 3) * 64 * (DF / 2) + lane;
+    constexpr int HALF = 4 * 64 * (DF / 2);  // floats
+    __syncthreads();
 #pragma unroll
-        for (int f = 0; f < FD; ++f)
+    for (int f = 0; f < FD; ++f)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sum[(16 * f + i) * 64] = acc[f][i];
+      for (int i = 0; i < 16; ++i) {
+        if (grp == 0)
+          sum[HALF + (16 * f + i) * 64] = dv[f][i];
+        else
+          sum[(16 * f + i) * 64] = dk[f][i];
       }
-      __syncthreads();
-      if (grp == 0) {
+    __syncthreads();
 #pragma unroll
-        for (int f = 0; f < FD; ++f)
+    for (int f = 0; f < FD; ++f)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[f][i] += sum[(16 * f + i) * 64];
+      for (int i = 0; i < 16; ++i) {
+        if (grp == 0)
+          dk[f][i] += sum[(16 * f + i) * 64];
+        else
+          dk[f][i] = sum[HALF + (16 * f + i) * 64] + dv[f][i];
       }
-    };
-    add(dk);
-    add(dv);
-    if (grp == 1) return;
   }
+  // with two groups each stores one of the two (dv of the second group now in dk)
   float bad = 0.f;
 #pragma unroll
   for (int f = 0; f < FD; ++f)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) bad = fmaf(dk[f][i], 0.f, fmaf(dv[f][i], 0.f, bad));
+    for (int i = 0; i < 16; ++i) bad = NG > 1 ? fmaf(dk[f][i], 0.f, bad) : fmaf(dk[f][i], 0.f, fmaf(dv[f][i], 0.f, bad));
   const unsigned long long redo = __ballot(key < a.lk && bad != bad);
   const unsigned alone = (unsigned)redo | (unsigned)(redo >> 32);
   const long long ko = ((long long)b * a.lk * a.hk + kh) * a.d, ks = (long long)a.hk * a.d;
-  if (key < a.lk && !((alone >> (lane & 31)) & 1)) {
-    at_store_row<T, DF>((T*)a.dk + ko + key * ks, dk, a.d, h, a.scale);
-    at_store_row<T, DF>((T*)a.dv + ko + key * ks, dv, a.d, h, 1.f);
+  const bool mine = key < a.lk && !((alone >> (lane & 31)) & 1);
+  if constexpr (NG > 1) {
+    at_store_row<T, DF>((T*)(grp ? a.dv : a.dk) + ko + key * ks, dk, a.d, h, grp ? 1.f : a.scale, mine);
+  } else {
+    at_store_row<T, DF>((T*)a.dk + ko + key * ks, dk, a.d, h, a.scale, mine);
+    at_store_row<T, DF>((T*)a.dv + ko + key * ks, dv, a.d, h, 1.f, mine);
   }
   for (unsigned todo = alone; todo; todo &= todo - 1) {
     const int j = kw0 + __builtin_ctz(todo);
@@ -332,8 +336,8 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       if (lane + 64 * e < a.d) {
-        st((T*)a.dk + ko + j * ks + lane + 64 * e, gk[e] * a.scale);
-        st((T*)a.dv + ko + j * ks + lane + 64 * e, gv[e]);
+        if (NG == 1 || grp == 0) st((T*)a.dk + ko + j * ks + lane + 64 * e, gk[e] * a.scale);
+        if (NG == 1 || grp == 1) st((T*)a.dv + ko + j * ks + lane + 64 * e, gv[e]);
       }
   }
 }
@@ -378,6 +382,13 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
   const T* qp = (const T*)a.q + b * a.q_sb + (long long)pr.qi * a.q_sl + pr.head * a.q_sh;
   const long long orow = (((long long)b * a.lq + pr.qi) * a.hq + pr.head) * a.d;
   const T* gp = (const T*)a.go + orow;
+  const AtLoad<T, DP, KT, NW> kl(a.k_sl, a.d, wid, lane), vl(a.v_sl, a.d, wid, lane);
+  auto issue = [&](int stage, int k0) {
+    kl.issue(kb, k0, k_hi, lds0 + stage * STAGE, wid);
+    vl.issue(vb, k0, k_hi, lds0 + stage * STAGE + TILE, wid);
+  };
+  const int nt = k_hi > k_lo ? (k_hi - k_lo + KT - 1) / KT : 0;
+  if (nt > 0) issue(0, k_lo);
   uint4 qf[KS], gf[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
@@ -385,17 +396,11 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
     qf[ks] = live && e < a.d ? *(const uint4*)(qp + e) : make_uint4(0, 0, 0, 0);
     gf[ks] = live && e < a.d ? *(const uint4*)(gp + e) : make_uint4(0, 0, 0, 0);
   }
-  const AtLoad<T, DP, KT, NW> kl(a.k_sl, a.d, wid, lane), vl(a.v_sl, a.d, wid, lane);
-  auto issue = [&](int stage, int k0) {
-    kl.issue(kb, k0, k_hi, lds0 + stage * STAGE, wid);
-    vl.issue(vb, k0, k_hi, lds0 + stage * STAGE + TILE, wid);
-  };
   const float slope = SLOPE ? at_slope<T>(a, pr.head) : 0.f;
   const AtOffsets<T, DF> off(lane);
   at_f32x16 dq[FD];
 #pragma unroll
   for (int f = 0; f < FD; ++f) dq[f] = at_zero();
-  const int nt = k_hi > k_lo ? (k_hi - k_lo + KT - 1) / KT : 0;
   auto step = [&](auto stage, int t) {
     const int k0 = k_lo + t * KT;
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -428,7 +433,6 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
       at_accumulate<T, DF>(K, off, 32 * f, AtP<T>(ds), dq, lane);
     }
   };
-  if (nt > 0) issue(0, k_lo);
   for (int t = 0; t < nt; t += 2) {
     step(std::integral_constant<int, 0>{}, t);
     if (t + 1 < nt) step(std::integral_constant<int, 1>{}, t + 1);
@@ -440,13 +444,11 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
     for (int i = 0; i < 16; ++i) bad = fmaf(dq[f][i], 0.f, bad);
   const unsigned long long redo = __ballot(live && bad != bad);
   const unsigned alone = (unsigned)redo | (unsigned)(redo >> 32);
-  if (row < rows && !((alone >> (lane & 31)) & 1)) {
-    if (!live) {
+  if (!live) {
 #pragma unroll
-      for (int f = 0; f < FD; ++f) dq[f] = at_zero();
-    }
-    at_store_row<T, DF>((T*)a.dq + orow, dq, a.d, h, a.scale);
+    for (int f = 0; f < FD; ++f) dq[f] = at_zero();
   }
+  at_store_row<T, DF>((T*)a.dq + orow, dq, a.d, h, a.scale, row < rows && !((alone >> (lane & 31)) & 1));
   for (unsigned todo = alone; todo; todo &= todo - 1) {
     const int n = __builtin_ctz(todo);
     const int r = __shfl(row, n, 64);

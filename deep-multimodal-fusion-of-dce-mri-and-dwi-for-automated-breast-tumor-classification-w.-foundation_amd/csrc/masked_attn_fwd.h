@@ -54,6 +54,48 @@ __device__ __forceinline__ void at_store4(T* p, const float* v) {  // p aligned 
   else
     *(uint2*)p = make_uint2(AtPair<T>::pack(v[0], v[1]), AtPair<T>::pack(v[2], v[3]));
 }
+// One lane's column of transposed accumulators, times `scale`, to its row `out` of d elements (and what the rounding left
+// over to `rest`, if REST). The two half waves hold alternate fours of a row's dims; 16-bit types swap halves of pairs of
+// them, so that each lane stores 16 B. All 64 lanes call this; `on` says whether a lane's row is stored.
+template <typename T, int DF, bool REST = false>
+__device__ __forceinline__ void at_store_row(T* out, const at_f32x16* acc, int d, int h, float scale, bool on,
+                                             T* rest = nullptr) {
+#pragma unroll
+  for (int f = 0; f < DF / 32; ++f) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int e = 32 * f + 8 * g + 4 * h;
+        const float v[4] = {acc[f][4 * g] * scale, acc[f][4 * g + 1] * scale, acc[f][4 * g + 2] * scale,
+                            acc[f][4 * g + 3] * scale};
+        if (on && e < d) at_store4(out + e, v);
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < 4; g += 2) {
+        const int e = 32 * f + 8 * (g + h);
+        float v[8];
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = acc[f][4 * g + i] * scale;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = AtPair<T>::pack(v[2 * i], v[2 * i + 1]);
+        auto put = [&](T* p, const uint32_t* x) {
+          const auto a = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false);
+          const auto b = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+          if (on && e < d) *(uint4*)(p + e) = make_uint4(a[0], b[0], a[1], b[1]);
+        };
+        put(out, w);
+        if constexpr (REST) {
+          uint32_t r[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) r[i] = AtPair<T>::pack(v[2 * i] - B16<T>::lo(w[i]), v[2 * i + 1] - B16<T>::hi(w[i]));
+          put(rest, r);
+        }
+      }
+    }
+  }
+}
 
 template <typename T, int DF, bool CAP, bool SLOPE, bool TRAIN, int NW, int NG, int KT>
 __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 && DF > 64 ? 1 : 2) k_mattn_fwd(AtArgs a) {
@@ -289,8 +331,9 @@ __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 && DF > 64 ? 1 : 
   const long long prow = ((long long)split * nbh + bh) * rows + row;  // partials
   T* ob = (T*)a.o + (((long long)b * a.lq + qi) * a.hq + head) * a.d;
   T* olo = TRAIN ? (T*)a.o_lo + (((long long)b * a.lq + qi) * a.hq + head) * a.d : nullptr;
-  if (row < rows && !((alone >> (lane & 31)) & 1)) {
-    if (a.splits > 1) {
+  const bool mine = row < rows && !((alone >> (lane & 31)) & 1);
+  if (a.splits > 1) {
+    if (mine) {
       float* po = a.po + prow * a.d;
 #pragma unroll
       for (int f = 0; f < FD; ++f)
@@ -300,26 +343,14 @@ __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 && DF > 64 ? 1 : 
           if (e < a.d) *(float4*)(po + e) = make_float4(acc[f][4 * g], acc[f][4 * g + 1], acc[f][4 * g + 2], acc[f][4 * g + 3]);
         }
       if (h == 0) *(float4*)(a.pml + 4 * prow) = make_float4(m, l, lx, 0.f);
-    } else {
-      const float inv = live ? 1.f / l : 0.f;
-#pragma unroll
-      for (int f = 0; f < FD; ++f)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int e = 32 * f + 8 * g + 4 * h;
-          if (e >= a.d) continue;
-          float v[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = live ? acc[f][4 * g + r] * inv : 0.f;
-          at_store4(ob + e, v);
-          if (TRAIN) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] -= Cvt<T>::load(Cvt<T>::store(v[r]));
-            at_store4(olo + e, v);
-          }
-        }
-      if (a.lse && h == 0) a.lse[((long long)b * a.hq + head) * a.lq + qi] = live ? ms + at_log<T>(lx) : INFINITY;
     }
+  } else {
+    if (!live) {
+#pragma unroll
+      for (int f = 0; f < FD; ++f) acc[f] = at_zero();
+    }
+    at_store_row<T, DF, TRAIN>(ob, acc, a.d, h, live ? 1.f / l : 0.f, mine, olo);
+    if (a.lse && mine && h == 0) a.lse[((long long)b * a.hq + head) * a.lq + qi] = live ? ms + at_log<T>(lx) : INFINITY;
   }
   for (unsigned todo = alone; todo; todo &= todo - 1) {
     const int n = __builtin_ctz(todo);
