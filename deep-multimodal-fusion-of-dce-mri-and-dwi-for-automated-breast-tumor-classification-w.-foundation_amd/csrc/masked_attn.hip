@@ -15,7 +15,8 @@ int mattn_bwd_f32(const AtArgs& a, hipStream_t stream);
 // at position p = kv_len - lq + i and sees its document, under `causal` only up to itself or the document's first
 // `prefix` tokens. One workgroup per 1024 positions and batch row: the run starts among them are bit masks (one ballot a
 // wave), a run that enters from the left or leaves to the right is followed 1024 positions at a time.
-__global__ void __launch_bounds__(1024) k_mattn_spans(const int* __restrict__ docs, long long doc_sb,
+template <typename I>
+__global__ void __launch_bounds__(1024) k_mattn_spans(const I* __restrict__ docs, long long doc_sb,
                                                       const int* kv_lens, const int* prefix, int lq, int lk, int causal,
                                                       int2* __restrict__ spans) {
   __shared__ unsigned long long starts[16];
@@ -23,7 +24,7 @@ __global__ void __launch_bounds__(1024) k_mattn_spans(const int* __restrict__ do
   const int b = blockIdx.y, t = threadIdx.x, lane = t & 63, wv = t >> 6;
   const int n = kv_lens ? min(max(kv_lens[b], 0), lk) : lk;
   const int q0 = n - lq;  // position of query 0
-  const int* id = docs + b * doc_sb;
+  const I* id = docs + b * doc_sb;
   int2* out = spans + (long long)b * lq;
   if (blockIdx.x == 0)  // queries before the first position
     for (int i = t; i < min(lq, -q0); i += 1024) out[i] = make_int2(0, 0);
@@ -163,15 +164,24 @@ static int at_check(const char* who, AtArgs& a, int dtype) {
 
 using namespace dmf;
 
+template <typename I>
+static int mattn_spans(const char* who, const I* documents, long long doc_sb, const int* kv_lens, const int* prefix,
+                       int batch, int lq, int lk, int causal, int* spans, void* stream) {
+  DMF_CHECK_ARG(batch >= 0 && batch < 65536 && lq >= 0 && lk >= 0, "%s: batch %d, lengths %d / %d", who, batch, lq, lk);
+  if (batch == 0 || lq == 0) return 0;
+  DMF_CHECK_ARG((documents || lk == 0) && spans && (uintptr_t)spans % 8 == 0, "%s: null operand", who);
+  hipLaunchKernelGGL((k_mattn_spans<I>), dim3((unsigned)cdiv(lk > 0 ? lk : 1, 1024), (unsigned)batch), dim3(1024), 0,
+                     (hipStream_t)stream, documents, doc_sb, kv_lens, prefix, lq, lk, causal, (int2*)spans);
+  DMF_LAUNCH_CHECK(who);
+  return 0;
+}
 extern "C" int dmf_mattn_spans(const int* documents, long long doc_sb, const int* kv_lens, const int* prefix, int batch,
                                int lq, int lk, int causal, int* spans, void* stream) {
-  DMF_CHECK_ARG(batch >= 0 && batch < 65536 && lq >= 0 && lk >= 0, "dmf_mattn_spans: batch %d, lengths %d / %d", batch, lq, lk);
-  if (batch == 0 || lq == 0) return 0;
-  DMF_CHECK_ARG((documents || lk == 0) && spans && (uintptr_t)spans % 8 == 0, "dmf_mattn_spans: null operand");
-  hipLaunchKernelGGL(k_mattn_spans, dim3((unsigned)cdiv(lk > 0 ? lk : 1, 1024), (unsigned)batch), dim3(1024), 0, (hipStream_t)stream, documents, doc_sb,
-                     kv_lens, prefix, lq, lk, causal, (int2*)spans);
-  DMF_LAUNCH_CHECK("dmf_mattn_spans");
-  return 0;
+  return mattn_spans("dmf_mattn_spans", documents, doc_sb, kv_lens, prefix, batch, lq, lk, causal, spans, stream);
+}
+extern "C" int dmf_mattn_spans64(const long long* documents, long long doc_sb, const int* kv_lens, const int* prefix,
+                                 int batch, int lq, int lk, int causal, int* spans, void* stream) {
+  return mattn_spans("dmf_mattn_spans64", documents, doc_sb, kv_lens, prefix, batch, lq, lk, causal, spans, stream);
 }
 
 extern "C" long long dmf_mattn_fwd_ws_floats(int dtype, int batch, int lq, int lk, int hq, int hk, int d, int ragged) {
@@ -198,6 +208,7 @@ extern "C" int dmf_mattn_fwd(int dtype, const void* q, long long q_sb, long long
   if (batch == 0 || lq == 0) return 0;
   DMF_CHECK_ARG(q && o && (lk == 0 || (k && v)), "dmf_mattn_fwd: null operand");
   DMF_CHECK_ARG(!lse || o_lo || dtype == DMF_F32, "dmf_mattn_fwd: lse of a 16-bit type goes with o_lo");
+  DMF_CHECK_ARG(!o_lo || dtype != DMF_F32, "dmf_mattn_fwd: f32 has no o_lo");
   DMF_CHECK_ARG((uintptr_t)o % 16 == 0 && (uintptr_t)o_lo % 16 == 0 && (uintptr_t)spans % 8 == 0,
                 "dmf_mattn_fwd: outputs must be aligned to 16 bytes");
   const AtPlan p = at_plan(dtype, batch, lq, lk, hk, a.group, d, kv_lens != nullptr);
@@ -231,6 +242,7 @@ extern "C" int dmf_mattn_bwd(int dtype, const void* q, long long q_sb, long long
   if (batch == 0 || (lq == 0 && lk == 0)) return 0;
   DMF_CHECK_ARG((lq == 0 || (q && o && lse && go && ws && dq)) && (lk == 0 || (k && v && dk && dv)),
                 "dmf_mattn_bwd: null operand");
+  DMF_CHECK_ARG(!o_lo || dtype != DMF_F32, "dmf_mattn_bwd: f32 has no o_lo");
   const uintptr_t al = (uintptr_t)o | (uintptr_t)o_lo | (uintptr_t)go | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv;
   DMF_CHECK_ARG(al % 16 == 0 && (uintptr_t)spans % 8 == 0, "dmf_mattn_bwd: operands must be aligned to 16 bytes");
   hipStream_t s = (hipStream_t)stream;

@@ -79,6 +79,8 @@ def _small(what, name, t, shape, dtype, device):
         raise ValueError(f"{what}: {name} is on {t.device}, expected {device}")
     if t.is_floating_point() != dtype.is_floating_point or t.dtype == torch.bool:
         raise ValueError(f"{what}: {name} must be {dtype}, got {t.dtype}")
+    if dtype == torch.int32:  # (a wider integer past 32 bits keeps its meaning as a bound)
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1) if t.dtype == torch.int64 else t
     return t.to(dtype).contiguous()
 
 
@@ -209,8 +211,8 @@ def qk_norm_rope(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weig
 # ---------------------------------------------------------------- attention
 def _spans(documents, kv_lens, prefix, b, lq, lk, causal):
     spans = torch.empty((b, lq, 2), dtype=torch.int32, device=documents.device)
-    _launch("dmf_mattn_spans", documents.device, documents.data_ptr(), lk, _p(kv_lens), _p(prefix), b, lq, lk, causal,
-            spans.data_ptr())
+    name = "dmf_mattn_spans64" if documents.dtype == torch.int64 else "dmf_mattn_spans"
+    _launch(name, documents.device, documents.data_ptr(), lk, _p(kv_lens), _p(prefix), b, lq, lk, causal, spans.data_ptr())
     return spans
 
 
@@ -310,7 +312,8 @@ def attention(q, k, v, *, scale=None, softcap=0.0, slopes=None, causal=False, kv
         prefix = _small(what, "prefix", prefix, (b,), torch.int32, dev)
     spans = None
     if documents is not None:
-        documents = _small(what, "documents", documents, (b, lk), torch.int32, dev)
+        documents = _small(what, "documents", documents, (b, lk),
+                           torch.int64 if documents.dtype == torch.int64 else torch.int32, dev)
         spans = _spans(documents, kv_lens, prefix, b, lq, lk, causal)
     cfg = (scale, softcap, bool(causal))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):

@@ -699,14 +699,18 @@ int dmf_qk_norm_rope_bwd(int dtype, const void* q, long long q_sb, long long q_s
  *   (dmf_mattn_spans) takes the place of causal / prefix. A query that sees nothing has o = 0; keys that a query does not see
  *   do not reach its output, whatever they hold. d a multiple of 8 up to 128, strides and bases multiples of 16 bytes,
  *   token strides at least d.
- *   For the backward: lse [batch][hq][lq] and, for 16-bit types, o_lo (what rounding o left over); null for inference.
+ *   For the backward: lse [batch][hq][lq] and, for 16-bit types alone, o_lo (what rounding o left over); null for
+ *   inference.
  *   ws: dmf_mattn_fwd_ws_floats floats (ragged: kv_lens is given; 0: null allowed), where the keys are split over
  *   workgroups.
  * dmf_mattn_bwd: dq, dk, dv from go = d o; ws: batch*lq*(hq + 2) floats of scratch. No atomics: same bits every run.
  * dmf_mattn_spans: spans of documents [batch] rows of doc_sb, lk ids each: a document is a maximal run of equal ids >= 0
- *   within kv_len; a query sees its document, under causal up to itself or the document's first prefix[b] tokens. */
+ *   within kv_len; a query sees its document, under causal up to itself or the document's first prefix[b] tokens.
+ *   dmf_mattn_spans64: the same of 64-bit ids. */
 int dmf_mattn_spans(const int* documents, long long doc_sb, const int* kv_lens, const int* prefix, int batch, int lq,
                     int lk, int causal, int* spans, void* stream);
+int dmf_mattn_spans64(const long long* documents, long long doc_sb, const int* kv_lens, const int* prefix, int batch,
+                      int lq, int lk, int causal, int* spans, void* stream);
 long long dmf_mattn_fwd_ws_floats(int dtype, int batch, int lq, int lk, int hq, int hk, int d, int ragged);
 int dmf_mattn_fwd(int dtype, const void* q, long long q_sb, long long q_sl, long long q_sh, const void* k,
                   long long k_sb, long long k_sl, long long k_sh, const void* v, long long v_sb, long long v_sl,

@@ -548,3 +548,35 @@ def test_qk_norm_rope_refusals():
         A.qk_norm_rope(q, k[:, :4], c, s)
     with pytest.raises(ValueError, match="even"):
         A.qk_norm_rope(q[..., :63], k[..., :63], q_weight=w[:63], k_weight=w[:63])
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_backward_of_many_key_blocks(d, dt):
+    """More than one 128-key block for each CU (other tests have fewer, and blocks of 64 keys in 16-bit types)."""
+    _attn_case(9, 200, 200, 32, 16, d, dt, causal=True, kv_lens=[200, 1, 128, 129, 0, 150, 200, 77, 200])
+
+
+def test_attention_wide_integers():
+    """64-bit ids and lengths keep their meaning past 32 bits: ids that agree in their low halves differ, those past 2^31
+    are no padding, lengths and prefixes are clamped."""
+    b, n, h, d = 2, 150, 2, 64
+    low = _docs(b, n, 40, 20, 7)
+    low[1, 60:90] = low[1, 30]          # one run in the low halves, three in the ids
+    low[1, 30:60] = low[1, 30]
+    wide = low.long()
+    wide[1, 60:75] += 2 ** 32
+    wide[1, 75:90] += 2 ** 31
+    wide[0, :40] = torch.where(wide[0, :40] >= 0, wide[0, :40] + 2 ** 31 + 5, -2 ** 40)
+    names = {int(x): i for i, x in enumerate(sorted(set(wide[wide >= 0].tolist())))}
+    small = torch.tensor([[names[int(x)] if x >= 0 else -1 for x in r] for r in wide], dtype=torch.int32)
+    q, k, v = (_randn((b, n, h, d), torch.bfloat16, s) for s in (1, 2, 3))
+    for causal in (False, True):
+        got = A.attention(q, k, v, causal=causal, documents=wide.to(DEV))
+        assert torch.equal(got, A.attention(q, k, v, causal=causal, documents=small.to(DEV)))
+        see, at = _see(b, n, n, causal, None, None, small)
+        _within(got, *_attn_ref(q, k, v, see, at, d ** -0.5, 0.0, None, None), "o")
+    lens = torch.tensor([2 ** 32 + 3, -2 ** 32 + 9], device=DEV)
+    got = A.attention(q, k, v, causal=True, kv_lens=lens, prefix=lens)
+    want = A.attention(q, k, v, causal=True, kv_lens=torch.tensor([n, 0], device=DEV), prefix=torch.tensor([n, 0], device=DEV))
+    assert torch.equal(got, want) and not want[1].any()
