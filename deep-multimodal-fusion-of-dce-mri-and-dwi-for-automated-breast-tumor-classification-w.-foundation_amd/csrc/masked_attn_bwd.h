@@ -5,10 +5,10 @@
 //   p_ij = exp(s_ij - lse_i),  dp_ij = do_i . v_j,  ds_ij = p_ij (dp_ij - delta_i) (1 - tanh^2(z_ij / cap))
 //   dv_j = sum_i p_ij do_i,  dk_j = scale sum_i ds_ij q_i,  dq_i = scale sum_j ds_ij k_j
 //
-// One launch holds two kinds of workgroups: those of 128 keys, which walk the queries that see them and keep dK and dV in
-// registers, and those of 256 (f32 over 64 dims: 128) packed rows, which walk their keys and keep dQ. The key workgroups' longest walk
-// (all queries of all heads of a group) decides how evenly a launch ends, so each 128 keys have, where LDS allows, two groups of
-// four waves that take the query tiles in turn and add up at the end. The scores are computed in
+// One launch holds two kinds of workgroups: those of 128 (or 64) keys, which walk the queries that see them and keep dK and
+// dV in registers, and those of 256 (f32 over 64 dims: 128) packed rows, which walk their keys and keep dQ. The key
+// workgroups' longest walk (all queries of all heads of a group) decides how evenly a launch ends, so each has, where LDS
+// allows, groups of waves that take the query tiles in turn and add up at the end. The scores are computed in
 // both (7 products for the 5 that one pass with dQ in atomics would take): no atomics, so the same bits every run, no
 // f32 dQ in HBM, and the sum over a group's query heads happens inside the dK / dV accumulators.
 #pragma once
@@ -65,7 +65,7 @@ __device__ __forceinline__ void at_grad(const AtArgs& a, float slope_u, float s,
   ds = p * (dp - delta);
   if constexpr (CAP) ds *= fmaf(s * s, a.sc.bend, 1.f);  // 1 - tanh^2
 }
-// LDS of the 128-key workgroups: their V tile, two stages of (Q, dO) tiles of 32 queries of one head, two of the rows'
+// LDS of the key workgroups: their V tile, two stages of (Q, dO) tiles of 32 queries of one head, two of the rows'
 // values (one DMA instruction each, whose upper 32 lanes bring zeros). K stays in registers as the score's operand; V does
 // not fit there beside the two accumulators (192 registers) and is read from LDS for each dP.
 struct AtRowData {
@@ -73,13 +73,15 @@ struct AtRowData {
   int lo[64], hi[64];
 };
 constexpr int AT_QT = 32;
-template <typename T, int DF> struct AtBwdLds {
+// KW: waves along the keys, 32 each
+template <typename T, int DF, int KW> struct AtBwdLds {
   static constexpr int RB = AtPad<DF>::DP * AtT<T>::E;
-  static constexpr int NG = sizeof(T) == 4 && DF > 64 ? 1 : 2;  // groups of four waves (f32 at 128 dims: LDS for one)
+  static constexpr int NW = sizeof(T) == 4 && DF > 64 ? 4 : 8, NG = NW / KW;  // waves (f32 at 128 dims: LDS for 4), groups
   static constexpr int KT = sizeof(T) == 4 ? 32 : 64;       // keys per tile of the row workgroups
-  static constexpr int QTILE = AT_QT * RB, VT = 128 * RB;
+  static constexpr int QTILE = AT_QT * RB, VT = 32 * KW * RB;
   static constexpr int GROUP = 4 * QTILE + 2 * (int)sizeof(AtRowData);  // a group's stages
-  static constexpr int KEYS = VT + NG * GROUP, ROWS = 4 * KT * RB, ADD = NG > 1 ? 2 * 4 * 64 * DF / 2 * 4 : 0;
+  static constexpr int SUM = KW * 64 * DF / 2;                          // floats of a group's dK or dV
+  static constexpr int KEYS = VT + NG * GROUP, ROWS = 4 * KT * RB, ADD = NG > 1 ? (NG > 2 ? 4 : 2) * SUM * 4 : 0;
   static constexpr int MOST = KEYS > ROWS ? KEYS : ROWS;
   static constexpr int BYTES = (MOST > ADD ? MOST : ADD) + 16 * (int)sizeof(int);
 };
@@ -136,47 +138,47 @@ __device__ void at_query_alone(const AtArgs& a, int b, int kh, int r, int lo, in
   }
 }
 
-template <typename T, int DF, bool CAP, bool SLOPE>
+template <typename T, int DF, bool CAP, bool SLOPE, int KW>
 __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, char* smem) {
-  typedef AtBwdLds<T, DF> L;
+  typedef AtBwdLds<T, DF, KW> L;
   constexpr int DP = AtPad<DF>::DP, KS = AtOffsets<T, DF>::KS, FD = DF / 32;
   constexpr int TILE = L::QTILE, STAGE = 2 * TILE;
-  constexpr int NG = L::NG;
+  constexpr int NG = L::NG, NT = 64 * L::NW;
   int* range = (int*)(smem + L::BYTES) - 16;
   const int lane = threadIdx.x & 63, w8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
-  const int wid = w8 & 3, grp = w8 >> 2;  // 32 keys; which of the query tiles
+  const int wid = w8 % KW, grp = w8 / KW;  // 32 keys; which of the query tiles
   const int b = bh / a.hk, kh = bh - b * a.hk;
-  const int kb0 = ktile * 128, kw0 = kb0 + 32 * wid, key = kw0 + (lane & 31);
+  const int kb0 = ktile * 32 * KW, kw0 = kb0 + 32 * wid, key = kw0 + (lane & 31);
   const unsigned lds0 = (unsigned)(uintptr_t)((__attribute__((address_space(3))) char*)smem);
   const T* kb = (const T*)a.k + b * a.k_sb + kh * a.k_sh;
   const T* vb = (const T*)a.v + b * a.v_sb + kh * a.v_sh;
 
-  // the queries that see any of the 128 keys lie in [q0, q1]
+  // the queries that see any of the keys lie in [q0, q1]
   const long long nrows = (long long)a.batch * a.hq * a.lq, nq = (long long)a.batch * a.lq;
   const int* w_lo = (const int*)a.rowws + nrows + (long long)b * a.lq;
   const int* w_hi = w_lo + nq;
   int q0 = 0x7fffffff, q1 = -1;
   if (a.spans) {
-    for (int i = threadIdx.x; i < a.lq; i += 1024 * NG) {
+    for (int i = threadIdx.x; i < a.lq; i += 4 * NT) {
       int lo[4], hi[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const int r = min(i + 256 * NG * u, a.lq - 1);
+        const int r = min(i + NT * u, a.lq - 1);
         lo[u] = w_lo[r];
         hi[u] = w_hi[r];
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        if (i + 256 * NG * u < a.lq && hi[u] > kb0 && lo[u] < kb0 + 128) {
-          q0 = min(q0, i + 256 * NG * u);
-          q1 = max(q1, i + 256 * NG * u);
+        if (i + NT * u < a.lq && hi[u] > kb0 && lo[u] < kb0 + 32 * KW) {
+          q0 = min(q0, i + NT * u);
+          q1 = max(q1, i + NT * u);
         }
     }
     q0 = at_wave_min(q0), q1 = at_wave_max(q1);
     if (lane == 0) range[w8] = q0, range[8 + w8] = q1;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 4 * NG; ++w) q0 = min(q0, range[w]), q1 = max(q1, range[8 + w]);
+    for (int w = 0; w < L::NW; ++w) q0 = min(q0, range[w]), q1 = max(q1, range[8 + w]);
     q0 = __builtin_amdgcn_readfirstlane(q0);
     q1 = __builtin_amdgcn_readfirstlane(q1);
   } else {  // spans by position start at 0 and only widen: the last query, and the first whose end is past the keys' start
@@ -190,10 +192,9 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
     q1 = __builtin_amdgcn_readfirstlane(q1);
   }
 
-  const AtLoad<T, DP, AT_QT, 4> ql(a.q_sl, a.d, wid, lane), gl((long long)a.hq * a.d, a.d, wid, lane);
-  // wave w brings the tile's lse / delta / lo / hi
-  const float* rv = wid == 0 ? a.lse : wid == 1 ? a.rowws : (const float*)(wid == 2 ? w_lo : w_hi);
-  const long long rv0 = wid < 2 ? ((long long)b * a.hq + kh * a.group) * a.lq : 0, rvh = wid < 2 ? a.lq : 0;
+  const AtLoad<T, DP, AT_QT, KW> ql(a.q_sl, a.d, wid, lane), gl((long long)a.hq * a.d, a.d, wid, lane);
+  // the tile's lse / delta / lo / hi: one a wave, or one pair
+  const long long rv0 = ((long long)b * a.hq + kh * a.group) * a.lq;
   const unsigned rvo = lane < AT_QT ? (unsigned)lane * 4 : BUF_OOB;
   auto issue = [&](int stage, int g, int i0) {
     const unsigned S = lds0 + L::VT + grp * L::GROUP + stage * STAGE;
@@ -201,8 +202,13 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
     ql.issue((const T*)a.q + b * a.q_sb + head * a.q_sh, i0, q1 + 1, S, wid);
     gl.issue((const T*)a.go + ((long long)b * a.lq * a.hq + head) * a.d, i0, q1 + 1, S + TILE, wid);
     // queries past the last arrive as zeros: an empty span
-    at_dma4(buf_rsrc(rv + rv0 + g * rvh + i0, __builtin_amdgcn_readfirstlane(min(q1 + 1 - i0, AT_QT) * 4)), rvo,
-            lds0 + L::VT + grp * L::GROUP + 2 * STAGE + stage * (unsigned)sizeof(AtRowData) + wid * 256);
+#pragma unroll
+    for (int n = 0; n < 4; n += KW) {
+      const int x = n + wid;
+      const float* rv = x < 2 ? (x == 0 ? a.lse : a.rowws) + rv0 + (long long)g * a.lq : (const float*)(x == 2 ? w_lo : w_hi);
+      at_dma4(buf_rsrc(rv + i0, __builtin_amdgcn_readfirstlane(min(q1 + 1 - i0, AT_QT) * 4)), rvo,
+              lds0 + L::VT + grp * L::GROUP + 2 * STAGE + stage * (unsigned)sizeof(AtRowData) + x * 256);
+    }
   };
 
   // tiles of 32 queries, head after head; the groups take them in turn
@@ -216,7 +222,7 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
   if (q1 >= 0) {  // (first: the rest of the set-up runs under the loads' latency)
     advance(grp, g, i0);
     if (g < a.group) issue(0, g, i0);
-    const AtLoad<T, DP, 128, 4 * NG> vl(a.v_sl, a.d, w8, lane);
+    const AtLoad<T, DP, 32 * KW, L::NW> vl(a.v_sl, a.d, w8, lane);
     vl.issue(vb, kb0, a.lk, lds0, w8);
   }
   uint4 kf[KS];
@@ -290,8 +296,25 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
     }
   }
   if constexpr (NG > 1) {  // the groups' sums through LDS: dK's to the first group, dV's to the second
-    float* sum = (float*)smem + (w8 & 3) * 64 * (DF / 2) + lane;
-    constexpr int HALF = 4 * 64 * (DF / 2);  // floats
+    float* sum = (float*)smem + wid * 64 * (DF / 2) + lane;
+    constexpr int HALF = L::SUM;
+    if constexpr (NG > 2) {  // first the upper two groups' to the lower two
+      float* two = sum + (grp & 1) * 2 * HALF;
+      __syncthreads();
+      if (grp > 1) {
+#pragma unroll
+        for (int f = 0; f < FD; ++f)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) two[(16 * f + i) * 64] = dk[f][i], two[HALF + (16 * f + i) * 64] = dv[f][i];
+      }
+      __syncthreads();
+      if (grp < 2) {
+#pragma unroll
+        for (int f = 0; f < FD; ++f)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dk[f][i] += two[(16 * f + i) * 64], dv[f][i] += two[HALF + (16 * f + i) * 64];
+      }
+    }
     __syncthreads();
 #pragma unroll
     for (int f = 0; f < FD; ++f)
@@ -299,10 +322,11 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
       for (int i = 0; i < 16; ++i) {
         if (grp == 0)
           sum[HALF + (16 * f + i) * 64] = dv[f][i];
-        else
+        else if (grp == 1)
           sum[(16 * f + i) * 64] = dk[f][i];
       }
     __syncthreads();
+    if (grp > 1) return;
 #pragma unroll
     for (int f = 0; f < FD; ++f)
 #pragma unroll
@@ -342,12 +366,12 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
   }
 }
 
-template <typename T, int DF, bool CAP, bool SLOPE>
+template <typename T, int DF, bool CAP, bool SLOPE, int KW>
 __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, char* smem) {
-  typedef AtBwdLds<T, DF> L;
+  typedef AtBwdLds<T, DF, KW> L;
   constexpr int DP = AtPad<DF>::DP, KS = AtOffsets<T, DF>::KS, FD = DF / 32, KT = L::KT;
   constexpr int TILE = KT * L::RB, STAGE = 2 * TILE;
-  constexpr int NW = 4 * L::NG;
+  constexpr int NW = L::NW;
   int* range = (int*)(smem + L::BYTES) - 16;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int b = bh / a.hk, kh = bh - b * a.hk, rows = a.lq * a.group;
@@ -462,25 +486,36 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
   }
 }
 
-// blockIdx.y first counts the workgroups of 128 keys (the longer ones; the first keys are seen by most queries), then those
-// of 128 NG packed rows, the last rows first; heads vary fastest, as in the forward
-template <typename T, int DF, bool CAP, bool SLOPE>
-__global__ void __launch_bounds__((256 * AtBwdLds<T, DF>::NG), (AtBwdLds<T, DF>::NG)) k_mattn_bwd(AtArgs a) {
+// blockIdx.y first counts the workgroups of 32 KW keys (the longer ones; the first keys are seen by most queries), then those
+// of 32 NW packed rows, the last rows first; heads vary fastest, as in the forward
+template <typename T, int DF, bool CAP, bool SLOPE, int KW>
+__global__ void __launch_bounds__((64 * AtBwdLds<T, DF, KW>::NW), (AtBwdLds<T, DF, KW>::NW / 4)) k_mattn_bwd(AtArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int ktiles = (a.lk + 127) / 128, t = blockIdx.y;
+  const int ktiles = (a.lk + 32 * KW - 1) / (32 * KW), t = blockIdx.y;
   if (t < ktiles)
-    at_bwd_keys<T, DF, CAP, SLOPE>(a, blockIdx.x, t, smem);
+    at_bwd_keys<T, DF, CAP, SLOPE, KW>(a, blockIdx.x, t, smem);
   else
-    at_bwd_rows<T, DF, CAP, SLOPE>(a, blockIdx.x, gridDim.y - 1 - t, smem);
+    at_bwd_rows<T, DF, CAP, SLOPE, KW>(a, blockIdx.x, gridDim.y - 1 - t, smem);
 }
 
-template <typename T, int DF, bool CAP, bool SLOPE>
-static int mattn_bwd_df(const AtArgs& a, hipStream_t stream) {
-  constexpr size_t LDS = AtBwdLds<T, DF>::BYTES;
-  const dim3 grid((unsigned)(a.batch * a.hk), (unsigned)(cdiv(a.lk, 128) + cdiv((long long)a.lq * a.group, 128 * AtBwdLds<T, DF>::NG)));
-  hipLaunchKernelGGL((k_mattn_bwd<T, DF, CAP, SLOPE>), grid, dim3(256 * AtBwdLds<T, DF>::NG), LDS, stream, a);
+template <typename T, int DF, bool CAP, bool SLOPE, int KW>
+static int mattn_bwd_kw(const AtArgs& a, hipStream_t stream) {
+  typedef AtBwdLds<T, DF, KW> L;
+  const dim3 grid((unsigned)(a.batch * a.hk), (unsigned)(cdiv(a.lk, 32 * KW) + cdiv((long long)a.lq * a.group, 32 * L::NW)));
+  hipLaunchKernelGGL((k_mattn_bwd<T, DF, CAP, SLOPE, KW>), grid, dim3(64 * L::NW), L::BYTES, stream, a);
   DMF_LAUNCH_CHECK("dmf_mattn_bwd");
   return 0;
+}
+// Keys per key workgroup: 128 in two groups of four waves, or, while those would leave half of the 256 CUs without one, 64 in
+// four groups of two (16-bit types, whose LDS holds four groups' stages): twice the workgroups with half the walk, for twice the loads a
+// product. bf16, 128 dims, backward: 2048 causal tokens, 32 heads over 8 (128 workgroups of 128 keys): 237 -> 163 us; the
+// same at 4096 (256 workgroups): 527 -> 547 us; 16 x 576 tokens, 4 heads (320): 68 -> 76 us.
+constexpr int AT_FEW_KEY_BLOCKS = 128;
+template <typename T, int DF, bool CAP, bool SLOPE>
+static int mattn_bwd_df(const AtArgs& a, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2)
+    if ((long long)a.batch * a.hk * cdiv(a.lk, 128) <= AT_FEW_KEY_BLOCKS) return mattn_bwd_kw<T, DF, CAP, SLOPE, 2>(a, stream);
+  return mattn_bwd_kw<T, DF, CAP, SLOPE, 4>(a, stream);
 }
 
 template <typename T>
