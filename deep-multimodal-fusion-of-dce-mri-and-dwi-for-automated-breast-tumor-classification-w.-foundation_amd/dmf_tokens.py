@@ -256,7 +256,15 @@ class AttnCore:
         self.cos, self.sin = rope if rope is not None else (None, None)
         self.softcap, self.slopes = float(softcap), slopes
 
-    def check(self, what, n, d):
+    def check(self, what, n, d, heads, dev):
+        for name, t, shape in (("q_norm", self.wq, (d,)), ("k_norm", self.wk, (d,)), ("slopes", self.slopes, (heads,)),
+                               ("the table's cos", self.cos, None), ("the table's sin", self.sin, None)):
+            if t is not None and (t.dtype != torch.float32 or t.device != dev or not t.is_contiguous()
+                                  or (t.dim() != 2 if shape is None else tuple(t.shape) != shape)):
+                raise ValueError(f"{what}: {name} must be contiguous float32 {shape or '[tokens, pairs]'} on {dev}, got "
+                                 f"{t.dtype} {tuple(t.shape)} on {t.device}")
+        if (self.wq is None) != (self.wk is None) or (self.cos is not None and self.cos.shape != self.sin.shape):
+            raise ValueError(f"{what}: q_norm and k_norm, cos and sin belong together")
         if d > 128 or d % 8:
             raise ValueError(f"{what}: attention options need a head dim that is a multiple of 8 up to 128, got {d}")
         if self.cos is not None and (self.cos.shape[0] < n or 2 * self.cos.shape[1] > d):
@@ -431,7 +439,8 @@ class _BlockFn(torch.autograd.Function):
         # MLP branch: x2 = x1 + drop(fc2(drop(gelu(fc1(ln2(x1)))))) * g2
         ln2, save2 = ln_fwd(x1, ln2w, ln2b, eps2, cdt)
         x2, sm = _mlp_fwd(ln2, w1, fc1b, w2, fc2b, p_mlp, rng, s_m1, s_m2, g2, x1)
-        ctx.save_for_backward(x, ln1, save1, *sa, x1, ln2, save2, *sm, wq, wp, w1, w2, ln1w, ln2w, g1, g2, rng)
+        # (the norm weights too: the core reads them, saved they are checked for changes in place)
+        ctx.save_for_backward(x, ln1, save1, *sa, x1, ln2, save2, *sm, wq, wp, w1, w2, ln1w, ln2w, g1, g2, rng, qnw, knw)
         ctx.cfg, ctx.core, ctx.na = cfg, core, len(sa)
         ctx.dims = (b, n, e)
         return x2.view(b, n, e)
@@ -441,7 +450,7 @@ class _BlockFn(torch.autograd.Function):
         t = ctx.saved_tensors
         (x, ln1, save1), sa, t = t[:3], t[3:3 + ctx.na], t[3 + ctx.na:]
         (x1, ln2, save2), sm = t[:3], t[3:6]
-        wq, wp, w1, w2, ln1w, ln2w, g1, g2, rng = t[6:]
+        wq, wp, w1, w2, ln1w, ln2w, g1, g2, rng = t[6:-2]
         heads, eps1, eps2, p_attn, p_proj, p_mlp, sites, cdt, _ = ctx.cfg
         s_attn, s_proj, s_m1, s_m2 = sites
         b, n, e = ctx.dims
@@ -666,14 +675,14 @@ class _MHSAFn(torch.autograd.Function):
         wq, wp = _wcast(cdt, qkvw, projw)
         out, sa = _attn_fwd(a, wq, qkvb, wp, projb, b, n, heads, p_attn, p_proj, rng, sites[0], sites[1], core=core)
         ones = torch.ones(e, dtype=torch.float32, device=x.device)
-        ctx.save_for_backward(a, *sa, wq, wp, ones, rng)
+        ctx.save_for_backward(a, *sa, wq, wp, ones, rng, qnw, knw)
         ctx.cfg, ctx.dims, ctx.xdtype, ctx.core = cfg, (b, n, e), x.dtype, core
         return out.view(b, n, e)
 
     @staticmethod
     def backward(ctx, dout):
         a, *rest = ctx.saved_tensors
-        sa, (wq, wp, ones, rng) = rest[:-4], rest[-4:]
+        sa, (wq, wp, ones, rng) = rest[:-6], rest[-6:-2]
         heads, p_attn, p_proj, sites, cdt = ctx.cfg
         b, n, e = ctx.dims
         need = ctx.needs_input_grad
@@ -742,7 +751,7 @@ def _need_rng(what, rng, *ps):
 
 
 def _check_core(what, core, x, heads, p_attn):
-    core.check(what, x.shape[1], x.shape[2] // heads)
+    core.check(what, x.shape[1], x.shape[2] // heads, heads, x.device)
     if p_attn > 0:
         raise ValueError(f"{what}: attention options have no attention dropout (p = {p_attn})")
 

@@ -297,3 +297,29 @@ def test_int64_lengths_bool_refused_and_wide_types():
     assert torch.equal(o1, o2)
     with pytest.raises(ValueError, match="documents"):
         A.attention(q, k, v, documents=torch.ones(2, 200, dtype=torch.bool, device=DEV))
+
+
+def test_options_refuse_cast_weights_tables_and_changes_before_the_backward():
+    """What the kernels take as float32 arrays is refused in another type or shape; norm weights changed between the
+    forward and the backward raise, as torch's own ops do."""
+    rope = A.rope_table_2d(4, 4, 64, device=DEV)
+    x = torch.randn(1, 16, 256, device=DEV, requires_grad=True)
+    for change, match in ((lambda b: setattr(b.attn, "q_norm", torch.nn.Parameter(b.attn.q_norm.bfloat16())), "q_norm"),
+                          (lambda b: setattr(b.attn, "slopes", b.attn.slopes[:2].clone()), "slopes"),
+                          (lambda b: setattr(b.attn, "slopes", b.attn.slopes.double()), "slopes"),
+                          (lambda b: setattr(b.attn, "k_norm", torch.nn.Parameter(torch.ones(32, device=DEV))), "k_norm")):
+        blk = _block(ALL, 3)
+        change(blk)
+        with pytest.raises(ValueError, match=match):
+            blk(x, rope)
+    blk = _block(ALL, 3)
+    with pytest.raises(ValueError, match="table"):
+        blk(x, (rope[0].bfloat16(), rope[1].bfloat16()))
+    with pytest.raises(ValueError, match="belong together"):
+        blk(x, (rope[0], rope[1][:, :8].contiguous()))
+    for m in (blk, blk.attn):
+        y = m(x, rope)
+        with torch.no_grad():
+            blk.attn.q_norm.mul_(2.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            y.sum().backward()
