@@ -6,9 +6,9 @@
 //   dv_j = sum_i p_ij do_i,  dk_j = scale sum_i ds_ij q_i,  dq_i = scale sum_j ds_ij k_j
 //
 // One launch holds two kinds of workgroups: those of 128 (or 64) keys, which walk the queries that see them and keep dK and
-// dV in registers, and those of 256 (f32 over 64 dims: 128) packed rows, which walk their keys and keep dQ. The key
-// workgroups' longest walk (all queries of all heads of a group) decides how evenly a launch ends, so each has, where LDS
-// allows, groups of waves that take the query tiles in turn and add up at the end. The scores are computed in
+// dV in registers, and those of 256 (or 128) packed rows, which walk their keys and keep dQ. The key workgroups' longest
+// walk (all queries of all heads of a group) decides how evenly a launch ends: where that weighs, groups of waves take a
+// workgroup's query tiles in turn and add up at the end (mattn_bwd_df). The scores are computed in
 // both (7 products for the 5 that one pass with dQ in atomics would take): no atomics, so the same bits every run, no
 // f32 dQ in HBM, and the sum over a group's query heads happens inside the dK / dV accumulators.
 #pragma once
@@ -73,10 +73,10 @@ struct AtRowData {
   int lo[64], hi[64];
 };
 constexpr int AT_QT = 32;
-// KW: waves along the keys, 32 each
-template <typename T, int DF, int KW> struct AtBwdLds {
+// NW: waves of a workgroup; KW: those along the keys, 32 each
+template <typename T, int DF, int NW, int KW> struct AtBwdLds {
   static constexpr int RB = AtPad<DF>::DP * AtT<T>::E;
-  static constexpr int NW = sizeof(T) == 4 && DF > 64 ? 4 : 8, NG = NW / KW;  // waves (f32 at 128 dims: LDS for 4), groups
+  static constexpr int NG = NW / KW;                        // groups of waves that take the query tiles in turn
   static constexpr int KT = sizeof(T) == 4 ? 32 : 64;       // keys per tile of the row workgroups
   static constexpr int QTILE = AT_QT * RB, VT = 32 * KW * RB;
   static constexpr int GROUP = 4 * QTILE + 2 * (int)sizeof(AtRowData);  // a group's stages
@@ -138,12 +138,12 @@ __device__ void at_query_alone(const AtArgs& a, int b, int kh, int r, int lo, in
   }
 }
 
-template <typename T, int DF, bool CAP, bool SLOPE, int KW>
+template <typename T, int DF, bool CAP, bool SLOPE, int NW, int KW>
 __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, char* smem) {
-  typedef AtBwdLds<T, DF, KW> L;
+  typedef AtBwdLds<T, DF, NW, KW> L;
   constexpr int DP = AtPad<DF>::DP, KS = AtOffsets<T, DF>::KS, FD = DF / 32;
   constexpr int TILE = L::QTILE, STAGE = 2 * TILE;
-  constexpr int NG = L::NG, NT = 64 * L::NW;
+  constexpr int NG = L::NG, NT = 64 * NW;
   int* range = (int*)(smem + L::BYTES) - 16;
   const int lane = threadIdx.x & 63, w8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int wid = w8 % KW, grp = w8 / KW;  // 32 keys; which of the query tiles
@@ -178,7 +178,7 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
     if (lane == 0) range[w8] = q0, range[8 + w8] = q1;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < L::NW; ++w) q0 = min(q0, range[w]), q1 = max(q1, range[8 + w]);
+    for (int w = 0; w < NW; ++w) q0 = min(q0, range[w]), q1 = max(q1, range[8 + w]);
     q0 = __builtin_amdgcn_readfirstlane(q0);
     q1 = __builtin_amdgcn_readfirstlane(q1);
   } else {  // spans by position start at 0 and only widen: the last query, and the first whose end is past the keys' start
@@ -222,7 +222,7 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
   if (q1 >= 0) {  // (first: the rest of the set-up runs under the loads' latency)
     advance(grp, g, i0);
     if (g < a.group) issue(0, g, i0);
-    const AtLoad<T, DP, 32 * KW, L::NW> vl(a.v_sl, a.d, w8, lane);
+    const AtLoad<T, DP, 32 * KW, NW> vl(a.v_sl, a.d, w8, lane);
     vl.issue(vb, kb0, a.lk, lds0, w8);
   }
   uint4 kf[KS];
@@ -366,12 +366,11 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
   }
 }
 
-template <typename T, int DF, bool CAP, bool SLOPE, int KW>
+template <typename T, int DF, bool CAP, bool SLOPE, int NW, int KW>
 __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, char* smem) {
-  typedef AtBwdLds<T, DF, KW> L;
+  typedef AtBwdLds<T, DF, NW, KW> L;
   constexpr int DP = AtPad<DF>::DP, KS = AtOffsets<T, DF>::KS, FD = DF / 32, KT = L::KT;
   constexpr int TILE = KT * L::RB, STAGE = 2 * TILE;
-  constexpr int NW = L::NW;
   int* range = (int*)(smem + L::BYTES) - 16;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int b = bh / a.hk, kh = bh - b * a.hk, rows = a.lq * a.group;
@@ -488,34 +487,45 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
 
 // blockIdx.y first counts the workgroups of 32 KW keys (the longer ones; the first keys are seen by most queries), then those
 // of 32 NW packed rows, the last rows first; heads vary fastest, as in the forward
-template <typename T, int DF, bool CAP, bool SLOPE, int KW>
-__global__ void __launch_bounds__((64 * AtBwdLds<T, DF, KW>::NW), (AtBwdLds<T, DF, KW>::NW / 4)) k_mattn_bwd(AtArgs a) {
+template <typename T, int DF, bool CAP, bool SLOPE, int NW, int KW>
+__global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DF > 64 ? 1 : 2) k_mattn_bwd(AtArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int ktiles = (a.lk + 32 * KW - 1) / (32 * KW), t = blockIdx.y;
   if (t < ktiles)
-    at_bwd_keys<T, DF, CAP, SLOPE, KW>(a, blockIdx.x, t, smem);
+    at_bwd_keys<T, DF, CAP, SLOPE, NW, KW>(a, blockIdx.x, t, smem);
   else
-    at_bwd_rows<T, DF, CAP, SLOPE, KW>(a, blockIdx.x, gridDim.y - 1 - t, smem);
+    at_bwd_rows<T, DF, CAP, SLOPE, NW, KW>(a, blockIdx.x, gridDim.y - 1 - t, smem);
 }
 
-template <typename T, int DF, bool CAP, bool SLOPE, int KW>
+template <typename T, int DF, bool CAP, bool SLOPE, int NW, int KW>
 static int mattn_bwd_kw(const AtArgs& a, hipStream_t stream) {
-  typedef AtBwdLds<T, DF, KW> L;
-  const dim3 grid((unsigned)(a.batch * a.hk), (unsigned)(cdiv(a.lk, 32 * KW) + cdiv((long long)a.lq * a.group, 32 * L::NW)));
-  hipLaunchKernelGGL((k_mattn_bwd<T, DF, CAP, SLOPE, KW>), grid, dim3(64 * L::NW), L::BYTES, stream, a);
+  typedef AtBwdLds<T, DF, NW, KW> L;
+  const dim3 grid((unsigned)(a.batch * a.hk), (unsigned)(cdiv(a.lk, 32 * KW) + cdiv((long long)a.lq * a.group, 32 * NW)));
+  hipLaunchKernelGGL((k_mattn_bwd<T, DF, CAP, SLOPE, NW, KW>), grid, dim3(64 * NW), L::BYTES, stream, a);
   DMF_LAUNCH_CHECK("dmf_mattn_bwd");
   return 0;
 }
-// Keys per key workgroup: 128 in two groups of four waves, or, while those would leave half of the 256 CUs without one, 64 in
-// four groups of two (16-bit types, whose LDS holds four groups' stages): twice the workgroups with half the walk, for twice the loads a
-// product. bf16, 128 dims, backward: 2048 causal tokens, 32 heads over 8 (128 workgroups of 128 keys): 237 -> 163 us; the
-// same at 4096 (256 workgroups): 527 -> 547 us; 16 x 576 tokens, 4 heads (320): 68 -> 76 us.
-constexpr int AT_FEW_KEY_BLOCKS = 128;
+// The workgroups of a 16-bit type, from sizes and the kind of mask (bf16, 128 dims unless said, the whole backward):
+//   4 waves, two workgroups a CU: their loads, barriers and stores fall apart in time and overlap. 32 x 576 tokens, 4 heads:
+//     138 -> 126 us against the next form; 32 x 257, 12 heads of 64: 100 -> 68; 8192 tokens, 4 heads: 570 -> 444.
+//   8 waves, two groups that share a key block's walk, one workgroup a CU: where a mask makes walks unequal and the longest
+//     one, which grows with the heads of a group, would end long after the others. 4096 causal tokens, 32 heads over 8 (256 key
+//     blocks): 484 us against 766 with 4 waves, 6144 (384): 1031 against 1238; with 512 key blocks the two meet (8192:
+//     1784 against 1800; 2 x 4096: 945 against 956) and then turn (3 x 4096: 1427 against 1421), and one head a group gains
+//     from 4 waves or comes out even.
+//   8 waves over 64 keys, four groups: while 128-key blocks would leave half of the 256 CUs without one: twice the workgroups
+//     with half the walk, for twice the loads a product. 2048 causal tokens, 32 heads over 8 (128 key blocks): 237 -> 163 us
+//     against the second form; at 4096 (256) 527 -> 547.
+constexpr int AT_FEW_KEY_BLOCKS = 128, AT_EVEN_KEY_BLOCKS = 512;
 template <typename T, int DF, bool CAP, bool SLOPE>
 static int mattn_bwd_df(const AtArgs& a, hipStream_t stream) {
-  if constexpr (sizeof(T) == 2)
-    if ((long long)a.batch * a.hk * cdiv(a.lk, 128) <= AT_FEW_KEY_BLOCKS) return mattn_bwd_kw<T, DF, CAP, SLOPE, 2>(a, stream);
-  return mattn_bwd_kw<T, DF, CAP, SLOPE, 4>(a, stream);
+  const long long blocks = (long long)a.batch * a.hk * cdiv(a.lk, 128);
+  if constexpr (sizeof(T) == 2) {
+    if (blocks <= AT_FEW_KEY_BLOCKS) return mattn_bwd_kw<T, DF, CAP, SLOPE, 8, 2>(a, stream);
+    const bool uneven = a.group > 1 && (a.causal || a.spans || a.kv_lens);
+    if (!uneven || blocks >= AT_EVEN_KEY_BLOCKS) return mattn_bwd_kw<T, DF, CAP, SLOPE, 4, 4>(a, stream);
+  }
+  return mattn_bwd_kw<T, DF, CAP, SLOPE, (sizeof(T) == 4 && DF > 64 ? 4 : 8), 4>(a, stream);
 }
 
 template <typename T>

@@ -553,8 +553,31 @@ def test_qk_norm_rope_refusals():
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("d", [64, 128])
 def test_attention_backward_of_many_key_blocks(d, dt):
-    """More than one 128-key block for each CU (other tests have fewer, and blocks of 64 keys in 16-bit types)."""
-    _attn_case(9, 200, 200, 32, 16, d, dt, causal=True, kv_lens=[200, 1, 128, 129, 0, 150, 200, 77, 200])
+    """More than one 128-key block for each CU (other tests have fewer, and blocks of 64 keys in 16-bit types): walks that a
+    mask makes unequal, equal ones, and more blocks than two for each CU."""
+    lens = [200, 1, 128, 129, 0, 150, 200, 77, 200]
+    _attn_case(9, 200, 200, 32, 16, d, dt, causal=True, kv_lens=lens)
+    _attn_case(9, 200, 200, 32, 16, d, dt, cap=20.0)
+    _attn_case(9, 200, 200, 16, 16, d, dt, causal=True, docs=_docs(9, 200, 90, 20, 1))
+    _attn_case(18, 150, 130, 32, 16, d, dt, causal=True, kv_lens=lens * 2, slopes=True)
+
+
+def test_attention_backward_of_many_key_blocks_hides_garbage():
+    """What a key's value or a query's gradient holds stays with the pairs that see it, in the 4-wave form too."""
+    b, n, h, d = 9, 140, 16, 64
+    q, k, v, go = (_randn((b, n, h, d), torch.bfloat16, s) for s in (1, 2, 3, 4))
+    v[:, 139] = float("inf")       # seen by the last query alone
+    go[:, 0] = float("nan")        # sees the first key alone
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    o = A.attention(q, k, v, causal=True)
+    dq, dk, dv = torch.autograd.grad(o, (q, k, v), go)
+    see, at = _see(b, n, n, True, None, None, None)
+    fin = [torch.where(torch.isfinite(t.detach()), t.detach(), 0.0) for t in (q, k, v, go)]
+    ref = _attn_ref(*fin[:3], see, at, d ** -0.5, 0.0, None, fin[3])
+    _within(o.detach()[:, :139], ref[0][:, :139], ref[1][:, :139], "o")
+    _within(dq[:, 1:139], ref[2][:, 1:139], ref[3][:, 1:139], "dq")
+    assert torch.isnan(dk).any() and torch.isnan(dv[:, 0]).all()
+    _within(dv[:, 1:], ref[6][:, 1:], ref[7][:, 1:], "dv")
 
 
 def test_attention_wide_integers():
