@@ -505,7 +505,7 @@ static int mattn_bwd_kw(const AtArgs& a, hipStream_t stream) {
   DMF_LAUNCH_CHECK("dmf_mattn_bwd");
   return 0;
 }
-// The workgroups of a 16-bit type, from sizes and the kind of mask (bf16, 128 dims unless said, the whole backward):
+// The workgroups, from sizes and the kind of mask (bf16, 128 dims unless said, the whole backward):
 //   4 waves, two workgroups a CU: their loads, barriers and stores fall apart in time and overlap. 32 x 576 tokens, 4 heads:
 //     138 -> 126 us against the next form; 32 x 257, 12 heads of 64: 100 -> 68; 8192 tokens, 4 heads: 570 -> 444.
 //   8 waves, two groups that share a key block's walk, one workgroup a CU: where a mask makes walks unequal and the longest
@@ -515,17 +515,18 @@ static int mattn_bwd_kw(const AtArgs& a, hipStream_t stream) {
 //     from 4 waves or comes out even.
 //   8 waves over 64 keys, four groups: while 128-key blocks would leave half of the 256 CUs without one: twice the workgroups
 //     with half the walk, for twice the loads a product. 2048 causal tokens, 32 heads over 8 (128 key blocks): 237 -> 163 us
-//     against the second form; at 4096 (256) 527 -> 547.
+//     against the second form; at 4096 (256) 527 -> 547. f32, 64 dims: 2 x 1024 causal tokens, 16 heads over 4: 519 -> 276 us;
+//     4 x 329 tokens, 4 heads: 59.6 -> 54.8.
 constexpr int AT_FEW_KEY_BLOCKS = 128, AT_EVEN_KEY_BLOCKS = 512;
 template <typename T, int DF, bool CAP, bool SLOPE>
 static int mattn_bwd_df(const AtArgs& a, hipStream_t stream) {
   const long long blocks = (long long)a.batch * a.hk * cdiv(a.lk, 128);
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (sizeof(T) == 2 || DF <= 64) {  // (f32 of more dims: LDS for one group of 4 waves)
     if (blocks <= AT_FEW_KEY_BLOCKS) return mattn_bwd_kw<T, DF, CAP, SLOPE, 8, 2>(a, stream);
     const bool uneven = a.group > 1 && (a.causal || a.spans || a.kv_lens);
     if (!uneven || blocks >= AT_EVEN_KEY_BLOCKS) return mattn_bwd_kw<T, DF, CAP, SLOPE, 4, 4>(a, stream);
   }
-  return mattn_bwd_kw<T, DF, CAP, SLOPE, (sizeof(T) == 4 && DF > 64 ? 4 : 8), 4>(a, stream);
+  return mattn_bwd_kw<T, DF, CAP, SLOPE, sizeof(T) == 4 && DF > 64 ? 4 : 8, 4>(a, stream);
 }
 
 template <typename T>
