@@ -526,7 +526,7 @@ static int mattn_bwd_df(const AtArgs& a, hipStream_t stream) {
     const bool uneven = a.group > 1 && (a.causal || a.spans || a.kv_lens);
     if (!uneven || blocks >= AT_EVEN_KEY_BLOCKS) return mattn_bwd_kw<T, DF, CAP, SLOPE, 4, 4>(a, stream);
   }
-  return mattn_bwd_kw<T, DF, CAP, SLOPE, sizeof(T) == 4 && DF > 64 ? 4 : 8, 4>(a, stream);
+  return mattn_bwd_kw<T, DF, CAP, SLOPE, (sizeof(T) == 4 && DF > 64 ? 4 : 8), 4>(a, stream);
 }
 
 template <typename T>
