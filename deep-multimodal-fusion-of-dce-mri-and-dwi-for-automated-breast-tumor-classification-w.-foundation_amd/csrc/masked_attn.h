@@ -55,9 +55,10 @@ struct AtArgs {
   void *dq, *dk, *dv;          // contiguous [batch][l][h][d]
 };
 
-// forward launch: row waves and key groups per workgroup, keys per split, splits
+// forward launch: row waves and key groups per workgroup, keys per split, splits; 32-key tiles for three workgroups a CU
 struct AtPlan {
   int nw, ng, chunk, splits;
+  bool three;
 };
 
 constexpr float AT_LOG2E = 1.4426950408889634f;

@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(1024) k_mattn_spans(const I* __restrict__ docs
 constexpr long long AT_FEW_BLOCKS = 8192, AT_CUS = 256;
 static AtPlan at_plan(int dtype, int batch, int lq, int lk, int hk, int group, int d, bool ragged) {
   const long long rows = (long long)lq * group, nbh = (long long)batch * hk, r32 = (rows + 31) / 32;
-  AtPlan p = {4, 1, lk > 0 ? lk : 1, 1};
+  AtPlan p = {4, 1, lk > 0 ? lk : 1, 1, false};
   long long chunk = 0;
   if (rows <= 32) {
     p.nw = 1;
@@ -131,6 +131,15 @@ static AtPlan at_plan(int dtype, int batch, int lq, int lk, int hk, int group, i
     p.splits = (int)(((long long)lk + chunk - 1) / chunk);
   }
   return p;
+}
+
+// Workgroups of 4 waves with 64-key tiles run two on a CU, with 32-key tiles (half the LDS, at most 168 registers) three, at
+// 3 to 10 % more time for the same work. That pays where all are equally long (no mask) and three or five come to a CU, which
+// two at a time leave an odd one of: bf16, 128 dims, 576 tokens, 4 heads, batch 32 (640 workgroups): 43 -> 36 us; 64 (1280):
+// 74 -> 63; but 48 (960): 50 -> 57, 8 (160): 20 -> 22.
+static bool at_three(const AtArgs& a) {
+  const long long n = ((long long)a.batch * a.hk * (((long long)a.lq * a.group + 127) / 128) + AT_CUS - 1) / AT_CUS;
+  return n == 3 || n == 5;
 }
 
 static int at_check(const char* who, AtArgs& a, int dtype) {
@@ -211,8 +220,9 @@ extern "C" int dmf_mattn_fwd(int dtype, const void* q, long long q_sb, long long
   DMF_CHECK_ARG(!o_lo || dtype != DMF_F32, "dmf_mattn_fwd: f32 has no o_lo");
   DMF_CHECK_ARG((uintptr_t)o % 16 == 0 && (uintptr_t)o_lo % 16 == 0 && (uintptr_t)spans % 8 == 0,
                 "dmf_mattn_fwd: outputs must be aligned to 16 bytes");
-  const AtPlan p = at_plan(dtype, batch, lq, lk, hk, a.group, d, kv_lens != nullptr);
+  AtPlan p = at_plan(dtype, batch, lq, lk, hk, a.group, d, kv_lens != nullptr);
   a.chunk = p.chunk, a.splits = p.splits;
+  p.three = p.nw == 4 && p.splits == 1 && !causal && !kv_lens && !spans && at_three(a);
   if (p.splits > 1) {
     DMF_CHECK_ARG(ws && (uintptr_t)ws % 16 == 0, "dmf_mattn_fwd: this size needs a workspace (dmf_mattn_fwd_ws_floats)");
     a.po = ws;

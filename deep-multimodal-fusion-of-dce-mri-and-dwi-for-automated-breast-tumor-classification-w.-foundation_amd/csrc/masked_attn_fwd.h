@@ -4,7 +4,7 @@
 // stream through two LDS stages of KT keys (LDS-DMA, the next tile in flight under the current one's products). A wave
 // holds its 32 queries and their output accumulators in registers and keeps a running maximum and sum per row. The
 // maximum may lag by 2^8 before the accumulators are rescaled (p <= 256 is exact enough in f32 and in range in f16), which
-// takes the rescale out of almost every tile. NW = 4, KT = 64 for rows that fill it; NW = 1, KT = 32 for up to 32 rows
+// takes the rescale out of almost every tile. NW = 4, KT = 64 for rows that fill it (KT = 32 where three on a CU pay, at_three); NW = 1, KT = 32 for up to 32 rows
 // (single tokens: one wave per workgroup, five in a CU's LDS, so that enough loads are in flight to draw on HBM).
 //
 // Splits: with few workgroups along the rows the keys are cut into chunks of a.chunk, each workgroup writes its
@@ -98,7 +98,7 @@ __device__ __forceinline__ void at_store_row(T* out, const at_f32x16* acc, int d
 }
 
 template <typename T, int DF, bool CAP, bool SLOPE, bool TRAIN, int NW, int NG, int KT>
-__global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 && DF > 64 ? 1 : 2) k_mattn_fwd(AtArgs a) {
+__global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 ? (DF > 64 ? 1 : 2) : NW == 4 && KT == 32 ? 3 : 2) k_mattn_fwd(AtArgs a) {
   constexpr int DP = AtPad<DF>::DP, KS = AtOffsets<T, DF>::KS, FD = DF / 32, KF = KT / 32;
   constexpr int TILE = KT * DP * AtT<T>::E, STAGE = 2 * TILE;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -456,6 +456,8 @@ static int mattn_fwd_df(const AtArgs& a, AtPlan p, hipStream_t stream) {
     hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, TRAIN, 1, 1, 32>), grid, dim3(64), 4 * 32 * RB, stream, a);
   else if (p.nw == 3)
     hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, TRAIN, 3, 1, 32>), grid, dim3(192), 4 * 32 * RB, stream, a);
+  else if (sizeof(T) == 2 && p.three)
+    hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, TRAIN, 4, 1, 32>), grid, dim3(256), 4 * 32 * RB, stream, a);
   else if (p.ng == 1)
     hipLaunchKernelGGL((k_mattn_fwd<T, DF, CAP, SLOPE, TRAIN, 4, 1, KT>), grid, dim3(256), LDS, stream, a);
   else if constexpr (sizeof(T) == 4)  // (16-bit workgroups of 8 waves lose: two of 4 overlap better)

@@ -7,7 +7,9 @@ The reference's MultiHeadSelfAttention (transformer_model.py:83-116) is the case
 (dmf_tokens); the blocks of transformer_model.TransformerStage take them as options. Both ops run on
 csrc/qknorm.hip and csrc/masked_attn*.h through the C-ABI, on torch's current stream, with every
 workspace from torch's allocator, so they can be captured into a graph; sizes are checked on the host, and
-device-side values (positions, lengths, ids) are bounds-checked in the kernels.
+device-side values (positions, lengths, ids) are bounds-checked in the kernels. A backward is captured, as with
+torch's own ops, on leaves that no eager graph still holds: torch's gradient accumulation would wait for that graph's
+stream inside the capture.
 """
 from __future__ import annotations
 

@@ -603,3 +603,11 @@ def test_attention_wide_integers():
     got = A.attention(q, k, v, causal=True, kv_lens=lens, prefix=lens)
     want = A.attention(q, k, v, causal=True, kv_lens=torch.tensor([n, 0], device=DEV), prefix=torch.tensor([n, 0], device=DEV))
     assert torch.equal(got, want) and not want[1].any()
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("mode", [dict(), dict(cap=20.0), dict(slopes=True), dict(cap=5.0, slopes=True)], ids=lambda m: "-".join(m) or "plain")
+@pytest.mark.parametrize("shape", [(32, 130, 127, 16, 8, 128), (17, 129, 97, 20, 20, 64), (41, 257, 33, 10, 10, 32)])
+def test_attention_three_workgroups_a_cu(shape, mode, dt):
+    """Unmasked rows whose workgroups come to three or five a CU (32-key tiles): odd key counts, shared heads."""
+    _attn_case(*shape, dt, **mode)
