@@ -517,12 +517,15 @@ static int mattn_bwd_kw(const AtArgs& a, hipStream_t stream) {
 //     with half the walk, for twice the loads a product. 2048 causal tokens, 32 heads over 8 (128 key blocks): 237 -> 163 us
 //     against the second form; at 4096 (256) 527 -> 547. f32, 64 dims: 2 x 1024 causal tokens, 16 heads over 4: 519 -> 276 us;
 //     4 x 329 tokens, 4 heads: 59.6 -> 54.8.
+//     Up to one block a CU under a document mask, whose longest document is the longest walk (8192 tokens, 16 heads over 4,
+//     second form -> this: 3 documents 461 -> 443, 12: 377 -> 264, 64: 112 -> 116; one of 8192: 961 -> 985), not beyond
+//     (4 x 4096 tokens, 8 documents each, 512 blocks: 349 -> 384).
 constexpr int AT_FEW_KEY_BLOCKS = 128, AT_EVEN_KEY_BLOCKS = 512;
 template <typename T, int DF, bool CAP, bool SLOPE>
 static int mattn_bwd_df(const AtArgs& a, hipStream_t stream) {
   const long long blocks = (long long)a.batch * a.hk * cdiv(a.lk, 128);
   if constexpr (sizeof(T) == 2 || DF <= 64) {  // (f32 of more dims: LDS for one group of 4 waves)
-    if (blocks <= AT_FEW_KEY_BLOCKS) return mattn_bwd_kw<T, DF, CAP, SLOPE, 8, 2>(a, stream);
+    if (blocks <= (a.spans && a.group > 1 ? 2 : 1) * AT_FEW_KEY_BLOCKS) return mattn_bwd_kw<T, DF, CAP, SLOPE, 8, 2>(a, stream);
     const bool uneven = a.group > 1 && (a.causal || a.spans || a.kv_lens);
     if (!uneven || blocks >= AT_EVEN_KEY_BLOCKS) return mattn_bwd_kw<T, DF, CAP, SLOPE, 4, 4>(a, stream);
   }

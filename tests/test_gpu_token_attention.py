@@ -560,6 +560,7 @@ def test_attention_backward_of_many_key_blocks(d, dt):
     _attn_case(9, 200, 200, 32, 16, d, dt, cap=20.0)
     _attn_case(9, 200, 200, 16, 16, d, dt, causal=True, docs=_docs(9, 200, 90, 20, 1))
     _attn_case(18, 150, 130, 32, 16, d, dt, causal=True, kv_lens=lens * 2, slopes=True)
+    _attn_case(5, 200, 200, 32, 16, d, dt, docs=_docs(5, 200, 150, 20, 2))
 
 
 def test_attention_backward_of_many_key_blocks_hides_garbage():
