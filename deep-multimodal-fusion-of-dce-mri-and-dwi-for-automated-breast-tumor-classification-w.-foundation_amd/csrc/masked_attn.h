@@ -53,6 +53,7 @@ struct AtArgs {
   const void* go;              // [batch][lq][hq][d]
   float* rowws;                // backward scratch: delta [batch][hq][lq], span lo [batch][lq], hi [batch][lq]
   void *dq, *dk, *dv;          // contiguous [batch][l][h][d]
+  int rows_first;              // launch order: row workgroups before key workgroups
 };
 
 // forward launch: row waves and key groups per workgroup, keys per split, splits; 32-key tiles for three workgroups a CU

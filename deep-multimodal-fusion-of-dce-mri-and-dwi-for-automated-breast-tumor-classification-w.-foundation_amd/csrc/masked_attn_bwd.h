@@ -485,12 +485,13 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
   }
 }
 
-// blockIdx.y first counts the workgroups of 32 KW keys (the longer ones; the first keys are seen by most queries), then those
-// of 32 NW packed rows, the last rows first; heads vary fastest, as in the forward
+// blockIdx.y first counts the workgroups of 32 KW keys (the first keys are seen by most queries), then those of 32 NW packed
+// rows, the last rows first, or the other way round (rows_first); heads vary fastest, as in the forward
 template <typename T, int DF, bool CAP, bool SLOPE, int NW, int KW>
 __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DF > 64 ? 1 : 2) k_mattn_bwd(AtArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int ktiles = (a.lk + 32 * KW - 1) / (32 * KW), t = blockIdx.y;
+  const int ktiles = (a.lk + 32 * KW - 1) / (32 * KW), y = blockIdx.y;
+  const int t = !a.rows_first ? y : y + ktiles < (int)gridDim.y ? y + ktiles : y + ktiles - gridDim.y;
   if (t < ktiles)
     at_bwd_keys<T, DF, CAP, SLOPE, NW, KW>(a, blockIdx.x, t, smem);
   else
@@ -498,8 +499,12 @@ __global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DF > 64 ? 1 : 2) k_
 }
 
 template <typename T, int DF, bool CAP, bool SLOPE, int NW, int KW>
-static int mattn_bwd_kw(const AtArgs& a, hipStream_t stream) {
+static int mattn_bwd_kw(AtArgs a, hipStream_t stream) {
   typedef AtBwdLds<T, DF, NW, KW> L;
+  // Without a mask the kind with the longer walks starts first: 4 lq group / groups products of a tile for a key workgroup's
+  // waves against 3 lk for a row workgroup's (1187 tokens, 12 heads of 64: 54 -> 43 us). Under a mask the first keys do (an
+  // order by the longest walks left was measured: even for causal masks, 20 % slower for documents).
+  a.rows_first = !a.causal && !a.spans && 3LL * a.lk * L::NG > 4LL * a.lq * a.group;
   const dim3 grid((unsigned)(a.batch * a.hk), (unsigned)(cdiv(a.lk, 32 * KW) + cdiv((long long)a.lq * a.group, 32 * NW)));
   hipLaunchKernelGGL((k_mattn_bwd<T, DF, CAP, SLOPE, NW, KW>), grid, dim3(64 * NW), L::BYTES, stream, a);
   DMF_LAUNCH_CHECK("dmf_mattn_bwd");
@@ -512,7 +517,8 @@ static int mattn_bwd_kw(const AtArgs& a, hipStream_t stream) {
 //     one, which grows with the heads of a group, would end long after the others. 4096 causal tokens, 32 heads over 8 (256 key
 //     blocks): 484 us against 766 with 4 waves, 6144 (384): 1031 against 1238; with 512 key blocks the two meet (8192:
 //     1784 against 1800; 2 x 4096: 945 against 956) and then turn (3 x 4096: 1427 against 1421), and one head a group gains
-//     from 4 waves or comes out even.
+//     from 4 waves or comes out even. Documents turn later (16384 tokens in 12, 16 heads over 4, 512 blocks: 851 against 1236;
+//     32768 in 60, 1024 blocks: 795 against 707).
 //   8 waves over 64 keys, four groups: while 128-key blocks would leave half of the 256 CUs without one: twice the workgroups
 //     with half the walk, for twice the loads a product. 2048 causal tokens, 32 heads over 8 (128 key blocks): 237 -> 163 us
 //     against the second form; at 4096 (256) 527 -> 547. f32, 64 dims: 2 x 1024 causal tokens, 16 heads over 4: 519 -> 276 us;
@@ -527,7 +533,7 @@ static int mattn_bwd_df(const AtArgs& a, hipStream_t stream) {
   if constexpr (sizeof(T) == 2 || DF <= 64) {  // (f32 of more dims: LDS for one group of 4 waves)
     if (blocks <= (a.spans && a.group > 1 ? 2 : 1) * AT_FEW_KEY_BLOCKS) return mattn_bwd_kw<T, DF, CAP, SLOPE, 8, 2>(a, stream);
     const bool uneven = a.group > 1 && (a.causal || a.spans || a.kv_lens);
-    if (!uneven || blocks >= AT_EVEN_KEY_BLOCKS) return mattn_bwd_kw<T, DF, CAP, SLOPE, 4, 4>(a, stream);
+    if (!uneven || blocks >= (a.spans ? 2 : 1) * AT_EVEN_KEY_BLOCKS) return mattn_bwd_kw<T, DF, CAP, SLOPE, 4, 4>(a, stream);
   }
   return mattn_bwd_kw<T, DF, CAP, SLOPE, (sizeof(T) == 4 && DF > 64 ? 4 : 8), 4>(a, stream);
 }
