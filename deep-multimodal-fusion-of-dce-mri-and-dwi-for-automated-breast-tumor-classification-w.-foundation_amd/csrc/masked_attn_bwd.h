@@ -11,13 +11,18 @@
 // workgroup's query tiles in turn and add up at the end (mattn_bwd_df). The scores are computed in
 // both (7 products for the 5 that one pass with dQ in atomics would take): no atomics, so the same bits every run, no
 // f32 dQ in HBM, and the sum over a group's query heads happens inside the dK / dV accumulators.
+//
+// Bound: matrix pipe, vector ALU and LDS reads within a fifth of each other (32 matrix instructions, about 250 vector ones and
+// 24 + 32 LDS reads a step of 32 x 32). 2 x 8192 tokens, 32 heads over 8 of 128, bf16: 6.9 ms, 1.11 PFLOP/s of the 7 products;
+// 32 x 576, 4 heads, capped: 132 us (0.58), of which a third is the workgroups' start and end.
 #pragma once
 #include "masked_attn.h"
 #include "masked_attn_fwd.h"
 
 namespace dmf {
 
-// What the backward needs of each row beside lse (a.rowws): delta, and the query's span. One lane group of 16 per row.
+// What the backward needs of each row beside lse (a.rowws): delta, and the query's span. One lane group of 16 per row. HBM:
+// o, its rest and do are read once (32 x 576 tokens, 4 heads of 128: 12 us, 4.7 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) k_mattn_rows(AtArgs a) {
   const long long g = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4;  // (b, query, head)
