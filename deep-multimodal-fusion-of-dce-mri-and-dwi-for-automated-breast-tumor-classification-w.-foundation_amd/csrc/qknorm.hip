@@ -269,7 +269,9 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope_bwd(QkArgs a) {
           for (int n = 0; n < NU; ++n)
 #pragma unroll
             for (int i = 0; i < 2 * V; ++i) ss = fmaf(v[j][n][i], v[j][n][i], ss);
-          r = rsqrtf(qk_group_sum(ss, a.lg) / (float)a.d + a.eps);
+          // (rows that are not there are zeros: without an eps their r would be infinite, and 0 * r would enter dw)
+          ss = qk_group_sum(ss, a.lg) / (float)a.d + a.eps;
+          r = live && h + j < h1 ? rsqrtf(ss) : 0.f;
         }
 #pragma unroll
         for (int n = 0; n < NU; ++n) {

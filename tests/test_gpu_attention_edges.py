@@ -1,0 +1,29 @@
+"""GPU: calls of qk_norm_rope and attention (dmf_attention) at the edges of what they take, against the 64-bit
+references and elementwise bounds of tests/test_gpu_token_attention.py."""
+import pytest
+import torch
+
+import dmf_attention as A
+import test_gpu_token_attention as T
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TYPES = T.TYPES
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("b,n,hq,hk,d", [(1, 1, 1, 1, 64), (1, 5, 3, 1, 128), (2, 37, 5, 3, 72), (3, 1187, 12, 5, 80), (1, 3, 2, 1, 512)])
+def test_qk_norm_rope_without_an_eps(b, n, hq, hk, d, dt):
+    """eps 0 with heads and tokens that leave places of the launch empty: finite inputs give finite weight gradients."""
+    q, k = (T._randn((b, n, h, d), dt, s, 1.5).requires_grad_() for h, s in ((hq, 1), (hk, 2)))
+    wq, wk = [(1 + 0.2 * T._randn((d,), torch.float32, s)).requires_grad_() for s in (3, 4)]
+    cos, sin = A.rope_table(n, d // 4 * 2, device=DEV)
+    pos = torch.arange(n, device=DEV).expand(b, n)
+    gq, gk = T._randn(q.shape, dt, 5), T._randn(k.shape, dt, 6)
+    y = A.qk_norm_rope(q, k, cos, sin, None, wq, wk, eps=0.0)
+    grads = torch.autograd.grad(y, (q, k, wq, wk), (gq, gk))
+    for i, (x, w, g) in enumerate(((q, wq, gq), (k, wk, gk))):
+        y0, by, dx, bx, dw, bw = T._qk_ref(x.detach(), w.detach(), cos, sin, pos, 0.0, False, g, dt)
+        T._within(y[i].detach(), y0, by, f"y{i}")
+        T._within(grads[i], dx, bx, f"dx{i}")
+        T._within(grads[2 + i], dw, bw, f"dw{i}")
