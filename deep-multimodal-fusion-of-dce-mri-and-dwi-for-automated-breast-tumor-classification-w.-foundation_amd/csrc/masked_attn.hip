@@ -176,7 +176,9 @@ using namespace dmf;
 template <typename I>
 static int mattn_spans(const char* who, const I* documents, long long doc_sb, const int* kv_lens, const int* prefix,
                        int batch, int lq, int lk, int causal, int* spans, void* stream) {
-  DMF_CHECK_ARG(batch >= 0 && batch < 65536 && lq >= 0 && lk >= 0, "%s: batch %d, lengths %d / %d", who, batch, lq, lk);
+  // (the kernel steps over positions 1024 at a time, in ints)
+  DMF_CHECK_ARG(batch >= 0 && batch < 65536 && lq >= 0 && lk >= 0 && lq < (1LL << 31) - 1024 && lk < (1LL << 31) - 1024,
+                "%s: batch %d, lengths %d / %d", who, batch, lq, lk);
   if (batch == 0 || lq == 0) return 0;
   DMF_CHECK_ARG((documents || lk == 0) && spans && (uintptr_t)spans % 8 == 0, "%s: null operand", who);
   hipLaunchKernelGGL((k_mattn_spans<I>), dim3((unsigned)cdiv(lk > 0 ? lk : 1, 1024), (unsigned)batch), dim3(1024), 0,
