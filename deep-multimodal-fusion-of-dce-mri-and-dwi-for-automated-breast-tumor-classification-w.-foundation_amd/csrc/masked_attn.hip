@@ -160,8 +160,8 @@ static int at_check(const char* who, AtArgs& a, int dtype) {
   for (long long s : st) DMF_CHECK_ARG(s >= 0 && s * e % 16 == 0, "%s: stride %lld is not a multiple of 16 bytes", who, s);
   DMF_CHECK_ARG((uintptr_t)a.q % 16 == 0 && (uintptr_t)a.k % 16 == 0 && (uintptr_t)a.v % 16 == 0,
                 "%s: q, k and v must be aligned to 16 bytes", who);
-  DMF_CHECK_ARG(130 * a.k_sl * e < (1LL << 31) && 130 * a.v_sl * e < (1LL << 31) &&
-                    (130 * a.q_sl + a.group * a.q_sh) * e < (1LL << 31) &&
+  // (offsets within a tile of one head; heads, batch rows and tiles are added in 64 bits)
+  DMF_CHECK_ARG(130 * a.k_sl * e < (1LL << 31) && 130 * a.v_sl * e < (1LL << 31) && 130 * a.q_sl * e < (1LL << 31) &&
                     (130LL * a.hq * a.d + (long long)a.hq * a.d) * e < (1LL << 31),
                 "%s: a tile of rows spans more than 2 GiB", who);
   if (a.lq <= 1) a.q_sl = a.d;  // (a length of one: any stride says the same)

@@ -12,3 +12,17 @@ def test_spans_refuse_lengths_past_their_index(name, lq, lk):
     """Positions are stepped over 1024 at a time: the last step has to stay below 2^31."""
     with pytest.raises(RuntimeError, match="lengths"):
         N.call(name, PTR, lk, None, None, 1, lq, lk, 0, PTR, None)
+
+
+def test_queries_heads_may_lie_far_apart():
+    """A tile holds rows of one head, so the distance of a group's heads is no limit (the call gets as far as its missing
+    output); the distance of a tile's tokens is."""
+    from test_attention_host import _dims
+
+    far = dict(hq=8, hk=1, q_sh=1 << 28, q_sb=1 << 31)
+    with pytest.raises(RuntimeError, match="null"):
+        N.call("dmf_mattn_fwd", *_dims(**far), None, None, None, None, None)
+    with pytest.raises(RuntimeError, match="null"):
+        N.call("dmf_mattn_bwd", *_dims(**far), None, None, PTR, PTR, PTR, PTR, PTR, PTR, None)
+    with pytest.raises(RuntimeError, match="2 GiB"):
+        N.call("dmf_mattn_fwd", *_dims(q_sl=1 << 28), None, None, None, None, None)

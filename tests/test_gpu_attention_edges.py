@@ -27,3 +27,19 @@ def test_qk_norm_rope_without_an_eps(b, n, hq, hk, d, dt):
         T._within(y[i].detach(), y0, by, f"y{i}")
         T._within(grads[i], dx, bx, f"dx{i}")
         T._within(grads[2 + i], dw, bw, f"dw{i}")
+
+
+def test_query_heads_past_32_bits():
+    """Head-major queries whose heads lie 256 MiB apart (a group of them past 2^31 bytes), forward and backward."""
+    far = 2 ** 27 + 64
+    q = torch.as_strided(torch.empty(8 * far + 4096, dtype=torch.bfloat16, device=DEV), (1, 40, 8, 64), (0, 64, far, 1))
+    q.copy_(T._randn((1, 40, 8, 64), torch.bfloat16, 1))
+    k, v, go = (T._randn((1, 70, 1, 64), torch.bfloat16, 2), T._randn((1, 70, 1, 64), torch.bfloat16, 3),
+                T._randn((1, 40, 8, 64), torch.bfloat16, 4))
+    runs = []
+    for x in (q, q.contiguous()):
+        ins = [t.detach().requires_grad_() for t in (x, k, v)]
+        assert ins[0].stride(2) == x.stride(2)
+        o = A.attention(*ins, causal=True)
+        runs.append((o.detach(), *torch.autograd.grad(o, ins, go)))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
