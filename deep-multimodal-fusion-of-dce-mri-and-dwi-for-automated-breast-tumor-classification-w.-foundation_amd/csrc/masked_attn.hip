@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(1024) k_mattn_spans(const I* __restrict__ docs
 // fit a CU; 8 x 32 query heads over 65536 keys: 279 us with 4096, 254 with 8192, 266 with 16384).
 //
 // More rows: 4 row waves (3, with 32-key tiles, where short rows would leave one of four without work and half a key tile
-// empty: 257 x 257 tokens, 12 heads of 64, batch 32: 32 -> 28 us). The keys are cut where that evens out the CUs: a CU's
+// empty: 257 x 257 tokens, 12 heads of 64, batch 32: 32 -> 28 us; and the grid holds that many row blocks). The keys are cut where that evens out the CUs: a CU's
 // n = ceil(workgroups / 256) run two at a time (an odd one out has the CU to itself, a third faster), each costs its key
 // tiles and about four tiles' time to start and end, and the cut costs the partials' traffic and a second launch (batch 2, 413
 // queries, 16 heads over 4, 32768 keys: 5 cuts 382 us, 7: 313, 9: 280, 12: 296). Ragged lengths leave whole cuts without
@@ -104,7 +104,7 @@ static AtPlan at_plan(int dtype, int batch, int lq, int lk, int hk, int group, i
     }
   } else {
     const long long b4 = (r32 + 3) / 4 * nbh;
-    if ((r32 + 2) / 3 * 3 * nbh < b4 * 4 && lk <= 512 && (lk + 63) / 64 * 64 - lk >= 32) {
+    if ((r32 + 2) / 3 * 3 * nbh < b4 * 4 && lk <= 512 && (lk + 63) / 64 * 64 - lk >= 32 && (r32 + 2) / 3 < 65536) {
       p.nw = 3;
       return p;
     }

@@ -43,3 +43,15 @@ def test_query_heads_past_32_bits():
         o = A.attention(*ins, causal=True)
         runs.append((o.detach(), *torch.autograd.grad(o, ins, go)))
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_rows_up_to_the_grid():
+    """More rows than 65535 blocks of 96 and keys that three-wave workgroups would take (one and a half tiles of 64): rows
+    at both ends and across the blocks' edges."""
+    n, lk, d = 200001 * 32, 257, 8
+    q, k, v = (T._randn((1, m, 1, d), torch.bfloat16, s) for m, s in ((n, 1), (lk, 2), (lk, 3)))
+    o = A.attention(q, k, v)
+    for at in (0, 96 * 65535 - 500, n - 1000):
+        see = torch.ones(1, 1000, lk, dtype=torch.bool)
+        ref, bound = T._attn_ref(q[:, at:at + 1000], k, v, see, torch.zeros(1, 1000, dtype=torch.long), d ** -0.5, 0.0, None, None)
+        T._within(o[:, at:at + 1000], ref, bound, f"o from {at}")
