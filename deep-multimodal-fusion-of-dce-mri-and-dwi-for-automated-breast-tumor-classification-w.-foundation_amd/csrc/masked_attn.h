@@ -30,6 +30,7 @@ struct AtScore {
   float bend;       // -1 / cap_u^2
   float poly[6];    // cap * U * tanh(x) = raw * poly(raw^2) for |x| = |raw| scale / cap <= 1 (16-bit types)
   float half[4];    // the same for |x| <= 0.5
+  float one_to, half_to;  // where they hold: 1 and 0.5, or less where a coefficient leaves f32's range (at_score_args)
 };
 
 struct AtArgs {
@@ -364,6 +365,9 @@ __device__ __forceinline__ float at_log(float x) {
 // cap (|x| <= 0.5, where trained scores mostly are) degree 3 does, with 5.4e-07. Every form is off by less than
 // 10 * 2^-24 * cap, below the 16-bit rounding of the probabilities; f32 calls tanhf, since that would be several f32 units of
 // the exponent.
+// A coefficient of x^(2 i + 1) carries cap (scale / cap)^(2 i + 1): under a large cap the last ones fall below f32's normal
+// numbers (the eleventh power from cap = 250 at scale 0.088), under a tiny one they pass its largest. The degree-5 form is then
+// left out, and the degree-3 one taken up to the x at which the terms that are left out reach 2^-24 of the first.
 template <typename T>
 inline void at_score_args(AtArgs& a) {
   static const double C[6] = {0.9999994039535522,    -0.3332904279232025,  0.13281433284282684,
@@ -378,6 +382,18 @@ inline void at_score_args(AtArgs& a) {
     a.sc.poly[i] = (float)(C[i] * a.sc.cap_u * x);
     if (i < 4) a.sc.half[i] = (float)(H[i] * a.sc.cap_u * x);
     x *= (double)a.sc.scale_cap * a.sc.scale_cap;
+  }
+  auto normal = [](float c) { return fabsf(c) >= 1.17549435e-38f && fabsf(c) < INFINITY; };
+  a.sc.one_to = 1.f;
+  for (float c : a.sc.poly)
+    if (!normal(c)) a.sc.one_to = -1.f;
+  // |H[i]| x^(2 i) = 2^-24 for i = 1, 2, 3
+  static const float TO[4] = {-1.f, 4.2e-4f, 0.0259f, 0.105f};
+  a.sc.half_to = 0.5f;
+  for (int i = 3; i >= 0; --i) {
+    if (normal(a.sc.half[i])) continue;
+    a.sc.half_to = a.sc.scale_cap < 1.f ? TO[i] : -1.f;
+    for (int k = i; k < 4; ++k) a.sc.half[k] = 0.f;
   }
 }
 template <typename T>
@@ -410,10 +426,10 @@ __device__ __forceinline__ float at_bent(const AtScore& c, float raw) {
 }
 // calls f with the form that the wave's largest |x| allows (a NaN among them: it is NaN in every form)
 template <typename F>
-__device__ __forceinline__ void at_by_form(float x, F&& f) {
-  if (!__any(!(x <= 0.5f)))
+__device__ __forceinline__ void at_by_form(const AtScore& c, float x, F&& f) {
+  if (!__any(!(x <= c.half_to)))
     f(std::integral_constant<int, AT_HALF>{});
-  else if (!__any(!(x <= 1.f)))
+  else if (!__any(!(x <= c.one_to)))
     f(std::integral_constant<int, AT_ONE>{});
   else
     f(std::integral_constant<int, AT_ANY>{});
@@ -434,7 +450,7 @@ __device__ __forceinline__ void at_bend_tiles(const AtScore& c, at_f32x16* s) {
     for (int f = 0; f < N; ++f)
 #pragma unroll
       for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(s[f][i]));
-    at_by_form(big * c.scale_cap, all);
+    at_by_form(c, big * c.scale_cap, all);
   } else {
     all(std::integral_constant<int, AT_ANY>{});
   }

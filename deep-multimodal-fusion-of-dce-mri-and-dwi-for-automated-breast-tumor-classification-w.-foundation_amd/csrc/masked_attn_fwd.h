@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 ? (DF > 64 ? 1 : 
       for (int f = 0; f < FD; ++f) acc[f] *= alpha;
     }
     if constexpr (LATE) {
-      at_by_form(big * a.sc.scale_cap, [&](auto form) {
+      at_by_form(a.sc, big * a.sc.scale_cap, [&](auto form) {
 #pragma unroll
         for (int f = 0; f < KF; ++f)
 #pragma unroll

@@ -55,3 +55,43 @@ def test_rows_up_to_the_grid():
         see = torch.ones(1, 1000, lk, dtype=torch.bool)
         ref, bound = T._attn_ref(q[:, at:at + 1000], k, v, see, torch.zeros(1, 1000, dtype=torch.long), d ** -0.5, 0.0, None, None)
         T._within(o[:, at:at + 1000], ref, bound, f"o from {at}")
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("cap,at", [(300.0, 0.9), (1000.0, 0.9), (1000.0, 0.45), (1e4, 0.9), (1e4, 0.45), (2e5, 0.01), (1e9, 1e-6)])
+def test_attention_large_caps(cap, at, slopes, dt):
+    """Scores that are a large share of a large cap, a few units apart: the bend of the cap shows in the probabilities."""
+    n, d, scale = 48, 8, 0.01
+    two = 2.0 if dt == torch.float16 else 1.0       # (f16 keeps the keys below 65504)
+    far = torch.tensor(cap * at / scale / two).bfloat16().item()
+    if dt == torch.float16 and far > 6e4:
+        two, far = two * 256, far / 256
+    q, k = torch.zeros(1, n, 2, d), torch.zeros(1, n, 1, d)
+    q[..., 0], q[..., 1] = two, two * torch.linspace(0.5, 1.5, 2 * n).view(1, n, 2)
+    k[..., 0], k[0, :, 0, 1] = far, torch.arange(n) % 16 * 100.0 / two
+    q, k, v, go = q.to(DEV).to(dt), k.to(DEV).to(dt), T._randn((1, n, 1, d), dt, 3), T._randn((1, n, 2, d), dt, 4)
+    sl = torch.tensor([0.02, 0.01], device=DEV) if slopes else None
+    ins = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = A.attention(*ins, scale=scale, softcap=cap, slopes=sl)
+    see, pos = T._see(1, n, n, False, None, None, None)
+    ref = T._attn_ref(q, k, v, see, pos, scale, cap, sl, go)
+    T._within(o.detach(), ref[0], ref[1], "o")
+    for g, r, bound, what in zip(torch.autograd.grad(o, ins, go), ref[2::2], ref[3::2], ("dq", "dk", "dv")):
+        T._within(g, r, bound, what)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("cap", [1e-4, 1e-6, 1e-8])
+def test_attention_tiny_caps(cap, dt):
+    """Caps whose powers leave the range of f32, over scores from zero (a query of zeros) to far past the cap."""
+    b, n, h, d = 1, 70, 2, 32
+    q, k, v, go = (T._randn((b, n, h, d), dt, s) for s in (1, 2, 3, 4))
+    q[:, :40] = 0.0
+    ins = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = A.attention(*ins, softcap=cap, causal=True)
+    see, pos = T._see(b, n, n, True, None, None, None)
+    ref = T._attn_ref(q, k, v, see, pos, d ** -0.5, cap, None, go)
+    T._within(o.detach(), ref[0], ref[1], "o")
+    for g, r, bound, what in zip(torch.autograd.grad(o, ins, go), ref[2::2], ref[3::2], ("dq", "dk", "dv")):
+        T._within(g, r, bound, what)
