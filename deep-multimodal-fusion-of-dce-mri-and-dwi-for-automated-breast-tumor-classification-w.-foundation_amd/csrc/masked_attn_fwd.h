@@ -231,7 +231,8 @@ __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 ? (DF > 64 ? 1 : 
     }
     mt = at_half_max(mt);
     if (RAW) mt *= a.sc.scale_u;
-    if (LATE) mt = mt == -INFINITY ? mt : at_bent<T, CAP, AT_ANY>(a.sc, mt);
+    // (-inf may be a product too, whose score is -cap: only a row that sees none of the tile has no maximum)
+    if (LATE) mt = sp.hi <= k0 || sp.lo >= k0 + KT ? -INFINITY : at_bent<T, CAP, AT_ANY>(a.sc, mt);
     if (__any(mt > m + 8.f * AtUnit<T>::U / AT_LOG2E)) {
       const float mn = fmaxf(m, mt);
       ms = mn == -INFINITY ? 0.f : mn;

@@ -95,3 +95,30 @@ def test_attention_tiny_caps(cap, dt):
     T._within(o.detach(), ref[0], ref[1], "o")
     for g, r, bound, what in zip(torch.autograd.grad(o, ins, go), ref[2::2], ref[3::2], ("dq", "dk", "dv")):
         T._within(g, r, bound, what)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("lq", [1, 40, 700])
+def test_attention_infinite_products_under_a_cap(lq, dt):
+    """A product of -inf is a score of -cap: such keys keep their weight, alone in a tile or before finite ones."""
+    n, d, cap = 700, 64, 2.0
+    q, k, v = torch.zeros(1, lq, 2, d), torch.zeros(1, n, 1, d), torch.zeros(1, n, 1, d)
+    q[..., :2] = 1.0
+    k[0, :500, 0, 0], k[0, 500:, 0, 1] = -float("inf"), -2.0
+    k[0, 600:620, 0, 0] = float("inf")
+    v[0, :500], v[0, 620:] = 1.0, -0.5
+    q, k, v = (t.to(DEV).to(dt) for t in (q, k, v))
+    for m, causal in ((n, False), (400, False), (n, True)):
+        if causal and lq > m:
+            continue
+        o = A.attention(q, k[:, :m], v[:, :m], scale=1.0, softcap=cap, causal=causal)
+        see, pos = T._see(1, lq, m, causal, None, None, None)
+        big = torch.where(k.double().isinf(), k.double().sign() * 1e6, k.double())  # (far past the cap: the same scores)
+        # the products are exact, so a score errs by the cap's 10 e cap and the exponent's 8 e |s|
+        s = cap * torch.tanh(big[0, :m, 0, :2].sum(-1) / cap)
+        p = torch.softmax(s[None].expand(lq, m).masked_fill(~see[0].to(DEV), float("-inf")), -1)
+        want, mag = p @ v[0, :m, 0].double(), p @ v[0, :m, 0].double().abs()
+        u = T._u(dt)
+        bound = (2 * (10 * T.E * cap + 8 * T.E * cap) + u + (m + 8) * T.E) * mag + u * want.abs() + T._tiny(dt) * (m + 1)
+        for h in range(2):
+            T._within(o[0, :, h], want, bound, f"o of head {h}")
