@@ -424,15 +424,19 @@ __device__ __forceinline__ float at_bent(const AtScore& c, float raw) {
     return fmaf(-2.f * c.cap_u, __builtin_amdgcn_rcpf(e), c.cap_u);
   }
 }
-// calls f with the form that the wave's largest |x| allows (a NaN among them: it is NaN in every form)
+// calls f with a (wave-uniform) form as a constant; the form that the wave's largest |x| allows (a NaN among them: it is NaN in
+// every form)
 template <typename F>
-__device__ __forceinline__ void at_by_form(const AtScore& c, float x, F&& f) {
-  if (!__any(!(x <= c.half_to)))
+__device__ __forceinline__ void at_by_form(int form, F&& f) {
+  if (form == AT_HALF)
     f(std::integral_constant<int, AT_HALF>{});
-  else if (!__any(!(x <= c.one_to)))
+  else if (form == AT_ONE)
     f(std::integral_constant<int, AT_ONE>{});
   else
     f(std::integral_constant<int, AT_ANY>{});
+}
+__device__ __forceinline__ int at_form(const AtScore& c, float x) {
+  return !__any(!(x <= c.half_to)) ? AT_HALF : !__any(!(x <= c.one_to)) ? AT_ONE : AT_ANY;
 }
 // raw products of N result tiles -> cap tanh(z / cap) or z in units U, in place, by the form that the whole wave's tile
 // allows
@@ -450,7 +454,7 @@ __device__ __forceinline__ void at_bend_tiles(const AtScore& c, at_f32x16* s) {
     for (int f = 0; f < N; ++f)
 #pragma unroll
       for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(s[f][i]));
-    at_by_form(c, big * c.scale_cap, all);
+    at_by_form(at_form(c, big * c.scale_cap), all);
   } else {
     all(std::integral_constant<int, AT_ANY>{});
   }

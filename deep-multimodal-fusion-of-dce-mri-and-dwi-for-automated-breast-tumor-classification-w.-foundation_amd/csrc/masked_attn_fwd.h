@@ -232,7 +232,12 @@ __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 ? (DF > 64 ? 1 : 
     mt = at_half_max(mt);
     if (RAW) mt *= a.sc.scale_u;
     // (-inf may be a product too, whose score is -cap: only a row that sees none of the tile has no maximum)
-    if (LATE) mt = sp.hi <= k0 || sp.lo >= k0 + KT ? -INFINITY : at_bent<T, CAP, AT_ANY>(a.sc, mt);
+    // (and bent as the tile's scores will be: under a large cap the forms differ by more than the lag)
+    const int form = LATE ? at_form(a.sc, big * a.sc.scale_cap) : AT_ANY;
+    if constexpr (LATE) {
+      at_by_form(form, [&](auto of) { mt = at_bent<T, CAP, of.value>(a.sc, mt); });
+      if (sp.hi <= k0 || sp.lo >= k0 + KT) mt = -INFINITY;
+    }
     if (__any(mt > m + 8.f * AtUnit<T>::U / AT_LOG2E)) {
       const float mn = fmaxf(m, mt);
       ms = mn == -INFINITY ? 0.f : mn;
@@ -244,15 +249,15 @@ __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 ? (DF > 64 ? 1 : 
       for (int f = 0; f < FD; ++f) acc[f] *= alpha;
     }
     if constexpr (LATE) {
-      at_by_form(a.sc, big * a.sc.scale_cap, [&](auto form) {
+      at_by_form(form, [&](auto of) {
 #pragma unroll
         for (int f = 0; f < KF; ++f)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            if constexpr (form.value == AT_ANY)
+            if constexpr (of.value == AT_ANY)
               s[f][i] = at_exp<T>(at_bent<T, CAP, AT_ANY>(a.sc, s[f][i]) - ms);
             else  // the polynomial's last product and the subtraction in one FMA
-              s[f][i] = at_exp<T>(fmaf(s[f][i], at_poly<form.value>(a.sc, s[f][i] * s[f][i]), -ms));
+              s[f][i] = at_exp<T>(fmaf(s[f][i], at_poly<of.value>(a.sc, s[f][i] * s[f][i]), -ms));
           }
       });
       if (part) {

@@ -122,3 +122,24 @@ def test_attention_infinite_products_under_a_cap(lq, dt):
         bound = (2 * (10 * T.E * cap + 8 * T.E * cap) + u + (m + 8) * T.E) * mag + u * want.abs() + T._tiny(dt) * (m + 1)
         for h in range(2):
             T._within(o[0, :, h], want, bound, f"o of head {h}")
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("cap", [1e7, 1e9, 1e15])
+def test_attention_caps_that_bend_nothing(cap, slopes, dt):
+    """Scores of about 1000 under caps so far above that tanh is the identity to 1e-8: the bounds of no cap at all."""
+    n, d, scale = 150, 8, 0.01
+    q, k = torch.zeros(1, n, 2, d), torch.zeros(1, n, 1, d)
+    q[..., 0], q[..., 1] = 2.0, torch.linspace(1.0, 3.0, 2 * n).view(1, n, 2)
+    k[..., 0], k[0, :, 0, 1] = 49920.0, torch.arange(n) % 16 * 50.0
+    q, k, v = q.to(DEV).to(dt), k.to(DEV).to(dt), T._randn((1, n, 1, d), dt, 3)
+    go = T._randn((1, n, 2, d), dt, 4)
+    sl = torch.tensor([0.02, 0.01], device=DEV) if slopes else None
+    ins = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = A.attention(*ins, scale=scale, softcap=cap, slopes=sl, causal=True)
+    see, pos = T._see(1, n, n, True, None, None, None)
+    ref = T._attn_ref(q, k, v, see, pos, scale, 0.0, sl, go)
+    T._within(o.detach(), ref[0], ref[1], "o")
+    for g, r, bound, what in zip(torch.autograd.grad(o, ins, go), ref[2::2], ref[3::2], ("dq", "dk", "dv")):
+        T._within(g, r, bound, what)
