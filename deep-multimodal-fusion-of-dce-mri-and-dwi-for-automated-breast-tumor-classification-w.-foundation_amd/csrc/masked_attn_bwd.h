@@ -21,7 +21,7 @@
 
 namespace dmf {
 
-// What the backward needs of each row beside lse (a.rowws): delta, and the query's span. One lane group of 16 per row. HBM:
+// What the backward needs of each row beside lse (a.rowws): -delta, and the query's span. One lane group of 16 per row. HBM:
 // o, its rest and do are read once (32 x 576 tokens, 4 heads of 128: 12 us, 4.7 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) k_mattn_rows(AtArgs a) {
@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(256) k_mattn_rows(AtArgs a) {
     const int head = (int)(g % a.hq);
     const long long bq = g / a.hq;
     const int qi = (int)(bq % a.lq), b = (int)(bq / a.lq);
-    a.rowws[((long long)b * a.hq + head) * a.lq + qi] = t;
+    a.rowws[((long long)b * a.hq + head) * a.lq + qi] = -t;
     if (head == 0) {
       const AtSpan sp = at_span(a, b, qi);
       ((int*)a.rowws)[n + bq] = sp.lo;
@@ -60,21 +60,50 @@ __global__ void __launch_bounds__(256) k_mattn_rows(AtArgs a) {
   }
 }
 
-// p and ds of one score s = cap tanh(z / cap) (units U); dist = |a - j|
+// p and ds of one score s = cap tanh(z / cap) (units U); dist = |a - j|; dpd = dp - delta
 template <typename T, bool CAP, bool SLOPE>
-__device__ __forceinline__ void at_grad(const AtArgs& a, float slope_u, float s, float dist, float lse, float dp,
-                                        float delta, float& p, float& ds) {
+__device__ __forceinline__ void at_grad(const AtArgs& a, float slope_u, float s, float dist, float lse, float dpd,
+                                        float& p, float& ds) {
   float e = s - lse;
   if constexpr (SLOPE) e = fmaf(-slope_u, dist, s) - lse;
   p = at_exp<T>(e);
-  ds = p * (dp - delta);
+  ds = p * dpd;
   if constexpr (CAP) ds *= fmaf(s * s, a.sc.bend, 1.f);  // 1 - tanh^2
+}
+// f16 holds dS up to 65504, and an output gradient that carries a loss scale may pass that where dq, dk and dv do not. A
+// column (one key, or one packed row) whose accumulators end up non-finite is therefore walked once more with its dS times 2^-25:
+// |dS| <= 2 * 128 * 65504^2 < 2^41 then fits, and what falls below f16's normal numbers is off by 2^-25 * 2^25 = 1 at most, a
+// 2^-16th of the column's largest. The second walk is the whole workgroup's. bf16 has f32's exponents.
+template <typename T> constexpr bool AT_AGAIN = false;
+template <> inline constexpr bool AT_AGAIN<f16_t> = true;
+constexpr float AT_DOWN = 2.98023224e-8f;  // 2^-25
+// lanes (of 32 columns) whose accumulators are not finite
+template <int FD>
+__device__ __forceinline__ unsigned at_not_finite(const at_f32x16* acc) {
+  float bad = 0.f;
+#pragma unroll
+  for (int f = 0; f < FD; ++f)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) bad = fmaf(acc[f][i], 0.f, bad);
+  const unsigned long long m = __ballot(bad != bad);
+  return (unsigned)m | (unsigned)(m >> 32);
+}
+// does any wave of the workgroup say yes? (`votes`: an int a wave)
+template <int NW>
+__device__ __forceinline__ bool at_vote(bool yes, int* votes) {
+  __syncthreads();  // (also: every wave is done with its tiles)
+  if ((threadIdx.x & 63) == 0) votes[threadIdx.x >> 6] = yes;
+  __syncthreads();
+  int any = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) any |= votes[w];
+  return __builtin_amdgcn_readfirstlane(any);
 }
 // LDS of the key workgroups: their V tile, two stages of (Q, dO) tiles of 32 queries of one head, two of the rows'
 // values (one DMA instruction each, whose upper 32 lanes bring zeros). K stays in registers as the score's operand; V does
 // not fit there beside the two accumulators (192 registers) and is read from LDS for each dP.
 struct AtRowData {
-  float lse[64], delta[64];
+  float lse[64], nd[64];  // nd: -delta
   int lo[64], hi[64];
 };
 constexpr int AT_QT = 32;
@@ -112,7 +141,7 @@ __device__ void at_key_alone(const AtArgs& a, int b, int kh, int j, int q0, int 
     const float raw = wave_sum(fmaf(x0, k0, x1 * k1)), dp = wave_sum(fmaf(g0, v0, g1 * v1));
     float p, ds;
     at_grad<T, CAP, SLOPE>(a, at_slope<T>(a, head), at_bent<T, CAP, AT_ANY>(a.sc, raw), fabsf((float)(sp.at - j)),
-                           a.lse[rb], dp, a.rowws[rb], p, ds);
+                           a.lse[rb], dp + a.rowws[rb], p, ds);
     dk[0] = fmaf(ds, x0, dk[0]), dk[1] = fmaf(ds, x1, dk[1]);
     dv[0] = fmaf(p, g0, dv[0]), dv[1] = fmaf(p, g1, dv[1]);
   }
@@ -128,7 +157,7 @@ __device__ void at_query_alone(const AtArgs& a, int b, int kh, int r, int lo, in
   const float q0 = on0 ? ld(q + lane) : 0.f, q1 = on1 ? ld(q + lane + 64) : 0.f;
   const float g0 = on0 ? ld(g + lane) : 0.f, g1 = on1 ? ld(g + lane + 64) : 0.f;
   const long long rb = ((long long)b * a.hq + x.head) * a.lq + x.qi;
-  const float lse = a.lse[rb], delta = a.rowws[rb];
+  const float lse = a.lse[rb], nd = a.rowws[rb];
   const float slope = at_slope<T>(a, x.head);
   dq[0] = dq[1] = 0.f;
   for (int j = lo; j < hi; ++j) {
@@ -138,7 +167,7 @@ __device__ void at_query_alone(const AtArgs& a, int b, int kh, int r, int lo, in
     const float v0 = on0 ? ld(vj + lane) : 0.f, v1 = on1 ? ld(vj + lane + 64) : 0.f;
     const float raw = wave_sum(fmaf(q0, k0, q1 * k1)), dp = wave_sum(fmaf(g0, v0, g1 * v1));
     float p, ds;
-    at_grad<T, CAP, SLOPE>(a, slope, at_bent<T, CAP, AT_ANY>(a.sc, raw), fabsf((float)(at - j)), lse, dp, delta, p, ds);
+    at_grad<T, CAP, SLOPE>(a, slope, at_bent<T, CAP, AT_ANY>(a.sc, raw), fabsf((float)(at - j)), lse, dp + nd, p, ds);
     dq[0] = fmaf(ds, k0, dq[0]), dq[1] = fmaf(ds, k1, dq[1]);
   }
 }
@@ -241,6 +270,7 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
   for (int f = 0; f < FD; ++f) dk[f] = at_zero(), dv[f] = at_zero();
   const AtOffsets<T, DF> off(lane);
   const char* V = smem + wid * 32 * L::RB;
+  float unit = 1.f;  // dS and dk stand in
   const int n0 = (at_keys(a, b)) - a.lq;  // position of query 0
   const char* const base = smem + L::VT + grp * L::GROUP;
   auto step = [&](auto stage) {
@@ -265,12 +295,14 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
       float p[16], ds[16];
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
-        const float4 lse = *(const float4*)(x.lse + 8 * r4 + 4 * h), delta = *(const float4*)(x.delta + 8 * r4 + 4 * h);
-        const float lp[4] = {lse.x, lse.y, lse.z, lse.w}, dl[4] = {delta.x, delta.y, delta.z, delta.w};
+        const float4 lse = *(const float4*)(x.lse + 8 * r4 + 4 * h);
+        const float4 nd = *(const float4*)(x.nd + 8 * r4 + 4 * h);
+        const float lp[4] = {lse.x, lse.y, lse.z, lse.w}, dl[4] = {nd.x, nd.y, nd.z, nd.w};
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int i = 4 * r4 + r;
-          at_grad<T, CAP, SLOPE>(a, slope, s[i], fabsf(x0 + (float)(8 * r4 + r)), lp[r], dp[i], dl[r], p[i], ds[i]);
+          at_grad<T, CAP, SLOPE>(a, slope, s[i], fabsf(x0 + (float)(8 * r4 + r)), lp[r],
+                                 AT_AGAIN<T> ? (dp[i] + dl[r]) * unit : dp[i] + dl[r], p[i], ds[i]);
         }
       }
       if (!full) {
@@ -292,13 +324,30 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
     }
     g = g1, i0 = i1;
   };
-  if (q1 >= 0) {
-    // (uniform over the workgroup: the first group's count)
-    const int nt = (a.group * ((q1 - q0) / AT_QT + 1) + NG - 1) / NG;
-    for (int t = 0; t < nt; t += 2) {
-      step(std::integral_constant<int, 0>{});
-      if (t + 1 < nt) step(std::integral_constant<int, 1>{});
+#pragma unroll 1
+  for (int walk = 0;; ++walk) {
+    if (q1 >= 0) {
+      // (uniform over the workgroup: the first group's count)
+      const int nt = (a.group * ((q1 - q0) / AT_QT + 1) + NG - 1) / NG;
+      for (int t = 0; t < nt; t += 2) {
+        step(std::integral_constant<int, 0>{});
+        if (t + 1 < nt) step(std::integral_constant<int, 1>{});
+      }
     }
+    if (!AT_AGAIN<T> || walk == 1) break;
+    const unsigned over = at_not_finite<FD>(dk);
+    if (!at_vote<NW>(over != 0, range)) break;
+    unit = (over >> (lane & 31)) & 1 ? AT_DOWN : 1.f;
+#pragma unroll
+    for (int f = 0; f < FD; ++f) dk[f] = at_zero(), dv[f] = at_zero();
+    g = 0, i0 = q0;
+    advance(grp, g, i0);
+    if (q1 >= 0 && g < a.group) issue(0, g, i0);
+  }
+  if constexpr (AT_AGAIN<T>) {
+    unit = 1.f / unit;
+#pragma unroll
+    for (int f = 0; f < FD; ++f) dk[f] *= unit;
   }
   if constexpr (NG > 1) {  // the groups' sums through LDS: dK's to the first group, dV's to the second
     float* sum = (float*)smem + wid * 64 * (DF / 2) + lane;
@@ -382,12 +431,12 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
   const int row = tile * 32 * NW + wid * 32 + (lane & 31);
   const AtRow pr = at_packed(a, kh, row < rows ? row : 0);
   AtSpan sp = {0, 0, 0};
-  float lse = INFINITY, delta = 0.f;
+  float lse = INFINITY, nd = 0.f;
   if (row < rows) {
     sp = at_span(a, b, pr.qi);
     const long long r = ((long long)b * a.hq + pr.head) * a.lq + pr.qi;
     lse = a.lse[r];
-    delta = a.rowws[r];
+    nd = a.rowws[r];
   }
   const bool live = sp.hi > sp.lo;
   const AtBounds w = at_bounds(a, b, kh, tile * 32 * NW + wid * 32, rows, sp);
@@ -426,6 +475,7 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
   }
   const float slope = SLOPE ? at_slope<T>(a, pr.head) : 0.f;
   const AtOffsets<T, DF> off(lane);
+  float unit = 1.f;  // dS and dq stand in: in the exponent of p
   at_f32x16 dq[FD];
 #pragma unroll
   for (int f = 0; f < FD; ++f) dq[f] = at_zero();
@@ -450,7 +500,8 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float p;
-        at_grad<T, CAP, SLOPE>(a, slope, s[i], fabsf(x0 - (float)(8 * (i >> 2) + (i & 3))), lse, dp[i], delta, p, ds[i]);
+        at_grad<T, CAP, SLOPE>(a, slope, s[i], fabsf(x0 - (float)(8 * (i >> 2) + (i & 3))), lse,
+                               dp[i] + nd, p, ds[i]);
       }
       if (part) {
         const int lo = sp.lo - k0 - 32 * f - 4 * h, hi = sp.hi - k0 - 32 * f - 4 * h;
@@ -461,9 +512,19 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
       at_accumulate<T, DF>(K, off, 32 * f, AtP<T>(ds), dq, lane);
     }
   };
-  for (int t = 0; t < nt; t += 2) {
-    step(std::integral_constant<int, 0>{}, t);
-    if (t + 1 < nt) step(std::integral_constant<int, 1>{}, t + 1);
+#pragma unroll 1
+  for (int walk = 0;; ++walk) {
+    for (int t = 0; t < nt; t += 2) {
+      step(std::integral_constant<int, 0>{}, t);
+      if (t + 1 < nt) step(std::integral_constant<int, 1>{}, t + 1);
+    }
+    if (!AT_AGAIN<T> || walk == 1) break;
+    const unsigned over = at_not_finite<FD>(dq);
+    if (!at_vote<NW>(over != 0, range)) break;
+    if ((over >> (lane & 31)) & 1) unit = AT_DOWN, lse += 25.f;
+#pragma unroll
+    for (int f = 0; f < FD; ++f) dq[f] = at_zero();
+    if (nt > 0) issue(0, k_lo);
   }
   float bad = 0.f;
 #pragma unroll
@@ -476,7 +537,7 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
 #pragma unroll
     for (int f = 0; f < FD; ++f) dq[f] = at_zero();
   }
-  at_store_row<T, DF>((T*)a.dq + orow, dq, a.d, h, a.scale, row < rows && !((alone >> (lane & 31)) & 1));
+  at_store_row<T, DF>((T*)a.dq + orow, dq, a.d, h, a.scale / unit, row < rows && !((alone >> (lane & 31)) & 1));
   for (unsigned todo = alone; todo; todo &= todo - 1) {
     const int n = __builtin_ctz(todo);
     const int r = __shfl(row, n, 64);
@@ -492,8 +553,10 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
 
 // blockIdx.y first counts the workgroups of 32 KW keys (the first keys are seen by most queries), then those of 32 NW packed
 // rows, the last rows first, or the other way round (rows_first); heads vary fastest, as in the forward
+// (f16 of 64 dims needs just over the 168 registers that let three waves a SIMD run: 32 x 257 tokens, 12 heads, capped: 94 us
+// without the bound, 81 with it)
 template <typename T, int DF, bool CAP, bool SLOPE, int NW, int KW>
-__global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DF > 64 ? 1 : 2) k_mattn_bwd(AtArgs a) {
+__global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DF > 64 ? 1 : AT_AGAIN<T> && DF == 64 ? 3 : 2) k_mattn_bwd(AtArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int ktiles = (a.lk + 32 * KW - 1) / (32 * KW), y = blockIdx.y;
   const int t = !a.rows_first ? y : y + ktiles < (int)gridDim.y ? y + ktiles : y + ktiles - gridDim.y;

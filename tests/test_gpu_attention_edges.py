@@ -143,3 +143,31 @@ def test_attention_caps_that_bend_nothing(cap, slopes, dt):
     T._within(o.detach(), ref[0], ref[1], "o")
     for g, r, bound, what in zip(torch.autograd.grad(o, ins, go), ref[2::2], ref[3::2], ("dq", "dk", "dv")):
         T._within(g, r, bound, what)
+
+
+def _grads(q, k, v, go, **kw):
+    ins = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = A.attention(*ins, **kw)
+    return (o.detach(), *torch.autograd.grad(o, ins, go))
+
+
+@pytest.mark.parametrize("mode", [dict(), dict(causal=True), dict(cap=20.0), dict(slopes=True, causal=True)], ids=lambda m: "-".join(m) or "plain")
+@pytest.mark.parametrize("shape", [(1, 130, 130, 4, 2, 64), (1, 257, 257, 3, 1, 128), (9, 200, 200, 32, 16, 32)])
+def test_attention_f16_large_score_gradients(shape, mode):
+    """Output gradients whose dS pass 65504 while dq, dk and dv do not, beside rows with small ones."""
+    b, lq, lk, hq, hk, d = shape
+    dt, mode = torch.float16, dict(mode)
+    q, k, v = (T._randn((b, n, h, d), dt, s, 0.5) for n, h, s in ((lq, hq, 1), (lk, hk, 2), (lk, hk, 3)))
+    v *= 16
+    go = T._randn((b, lq, hq, d), dt, 4)
+    go[:, ::3] *= 3000
+    go[:, 1::3] *= 1e-3
+    cap, causal = mode.get("cap", 0.0), mode.get("causal", False)
+    sl = torch.tensor([2.0 ** (-4.0 * (h + 1) / hq) for h in range(hq)], device=DEV) if mode.get("slopes") else None
+    see, pos = T._see(b, lq, lk, causal, None, None, None)
+    scale = 1 / 64
+    got = _grads(q, k, v, go, softcap=cap, slopes=sl, causal=causal, scale=scale)
+    ref = T._attn_ref(q, k, v, see, pos, scale, cap, sl, go)
+    for i, name in enumerate(("o", "dq", "dk", "dv")):
+        assert ref[2 * i].abs().max() < 65504, name
+        T._within(got[i], ref[2 * i], ref[2 * i + 1], name)
