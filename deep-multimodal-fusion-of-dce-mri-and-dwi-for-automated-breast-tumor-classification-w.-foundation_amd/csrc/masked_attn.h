@@ -272,6 +272,56 @@ __device__ __forceinline__ void at_accumulate(const char* tile, const AtOffsets<
   }
 }
 
+// What a mask hides. A masked pair has weight 0 exactly, but 0 * NaN is NaN: in a tile that some row sees in part, an element
+// of X that is not finite reaches the columns that may not see its row. Where accumulators end up non-finite under a mask, a
+// workgroup therefore walks its tiles once more, and takes at_accumulate_seen in such tiles with such an element (at_has_nonfinite):
+// the same sum row by row on the vector ALU, over the pairs that sees(row) lets through, at some 20 times a tile's products. So a
+// NaN that all may see costs a second walk, and finite inputs cost nothing but the check at the end.
+template <typename T, int DF>
+__device__ __forceinline__ bool at_has_nonfinite(const char* tile, int r0, int lane) {
+  constexpr int RB = AtOffsets<T, DF>::RB;
+  const uint4* p = (const uint4*)(tile + r0 * RB) + lane;
+  uint32_t most = 0, most2 = 0;  // of the magnitudes' bits: those of infinities and NaN are the largest
+#pragma unroll
+  for (int i = 0; i < 32 * RB / 1024; ++i) {
+    const uint4 u = p[64 * i];
+    for (uint32_t w : {u.x, u.y, u.z, u.w}) {
+      if constexpr (sizeof(T) == 4) {
+        most = max(most, w & 0x7fffffffu);
+      } else {
+        most = max(most, w & 0x7fffffffu);
+        most2 = max(most2, (w & 0x7fffu) << 16);
+      }
+    }
+  }
+  constexpr uint32_t INF = sizeof(T) == 4 ? 0x7f800000u : __is_same(T, f16_t) ? 0x7c000000u : 0x7f800000u;
+  return __any(max(most, most2) >= INF);
+}
+template <typename T, int DF, typename F>
+__device__ __forceinline__ void at_accumulate_seen(const char* tile, int r0, const float* p, at_f32x16* acc, int lane,
+                                                   F&& sees) {
+  constexpr int DP = AtPad<DF>::DP, E = AtT<T>::E, CH = AtT<T>::CH;
+  const int h = lane >> 5;
+#pragma unroll 1
+  for (int r = 0; r < 32; ++r) {  // its weight is in register 4 (r >> 3) + (r & 3) of half (r >> 2) & 1
+    const int n = 4 * (r >> 3) + (r & 3);
+    float w = p[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) w = n == i ? p[i] : w;
+    w = __shfl(w, (lane & 31) + 32 * ((r >> 2) & 1), 64);
+    const bool on = sees(r);
+#pragma unroll
+    for (int f = 0; f < DF / 32; ++f)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int e = 32 * f + 8 * g + 4 * h;
+        const T* x = (const T*)(tile + at_off<T, DP>(r0 + r, e / CH) + e % CH * E);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[f][4 * g + i] = on ? fmaf(w, ld(x + i), acc[f][4 * g + i]) : acc[f][4 * g + i];
+      }
+  }
+}
+
 // ------------------------------------------------------------------- spans
 struct AtSpan {
   int lo, hi;  // hi <= lo: nothing
@@ -341,6 +391,24 @@ __device__ __forceinline__ int at_wave_min(int v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 __device__ __forceinline__ int at_wave_max(int v) { return -at_wave_min(-v); }
+
+// lanes (of 32 columns) with an accumulator that is not finite
+template <int FD>
+__device__ __forceinline__ unsigned at_bad_columns(const at_f32x16* acc, float bad = 0.f) {
+#pragma unroll
+  for (int f = 0; f < FD; ++f)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) bad = fmaf(acc[f][i], 0.f, bad);
+  const unsigned long long m = __ballot(bad != bad);
+  return (unsigned)m | (unsigned)(m >> 32);
+}
+// does any wave of the workgroup say yes? `flag` (LDS) is 0 from before the tiles' barriers on; every wave is done with its tiles
+// after this
+__device__ __forceinline__ bool at_vote(bool yes, int* flag) {
+  if (yes) *flag = 1;
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(*flag);
+}
 
 // ------------------------------------------------------------------ scores
 // The exponent's unit U is the log2 domain for 16-bit types (v_exp_f32 is 2^x: one multiply saved per score) and the
@@ -459,12 +527,4 @@ __device__ __forceinline__ void at_bend_tiles(const AtScore& c, at_f32x16* s) {
     all(std::integral_constant<int, AT_ANY>{});
   }
 }
-// s (in units U) of one raw product; dist = |a - j|
-template <typename T, bool CAP, bool SLOPE>
-__device__ __forceinline__ float at_score(const AtScore& c, float slope_u, float raw, float dist) {
-  float s = at_bent<T, CAP, AT_ANY>(c, raw);
-  if constexpr (SLOPE) s = fmaf(-slope_u, dist, s);
-  return s;
-}
-
 }  // namespace dmf

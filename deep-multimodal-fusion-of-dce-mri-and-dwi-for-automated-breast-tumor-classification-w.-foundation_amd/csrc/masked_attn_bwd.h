@@ -70,34 +70,29 @@ __device__ __forceinline__ void at_grad(const AtArgs& a, float slope_u, float s,
   ds = p * dpd;
   if constexpr (CAP) ds *= fmaf(s * s, a.sc.bend, 1.f);  // 1 - tanh^2
 }
-// f16 holds dS up to 65504, and an output gradient that carries a loss scale may pass that where dq, dk and dv do not. A
-// column (one key, or one packed row) whose accumulators end up non-finite is therefore walked once more with its dS times 2^-25:
-// |dS| <= 2 * 128 * 65504^2 < 2^41 then fits, and what falls below f16's normal numbers is off by 2^-25 * 2^25 = 1 at most, a
-// 2^-16th of the column's largest. The second walk is the whole workgroup's. bf16 has f32's exponents.
-template <typename T> constexpr bool AT_AGAIN = false;
-template <> inline constexpr bool AT_AGAIN<f16_t> = true;
-constexpr float AT_DOWN = 2.98023224e-8f;  // 2^-25
-// lanes (of 32 columns) whose accumulators are not finite
+// f16 holds dS up to 65504, and an output gradient that carries a loss scale may pass that where dq, dk and dv do not. Such
+// accumulators end up non-finite too, and the second walk (at_accumulate_seen) brings dS into range: each lane's column (one key, or
+// one packed row) has a power of two that its ds and accumulators are in, lowered whenever a tile's largest ds passes 2^15
+// in it. What falls below f16's normal numbers is then off by a 2^-39th of the column's largest. bf16 has f32's exponents.
+template <typename T> constexpr bool AT_FIT = false;
+template <> inline constexpr bool AT_FIT<f16_t> = true;
 template <int FD>
-__device__ __forceinline__ unsigned at_not_finite(const at_f32x16* acc) {
-  float bad = 0.f;
+__device__ __forceinline__ void at_fit(float* ds, at_f32x16* acc, float& unit) {
+  float most = 0.f;
 #pragma unroll
-  for (int f = 0; f < FD; ++f)
+  for (int i = 0; i < 16; ++i) {
+    ds[i] *= unit;
+    most = fmaxf(most, fabsf(ds[i]) < INFINITY ? fabsf(ds[i]) : 0.f);
+  }
+  most = at_half_max(most);
+  if (!__any(most > 32768.f)) return;
+  // 2^(14 + e) <= most < 2^(15 + e): times 2^-e
+  const float down = most > 32768.f ? __uint_as_float((unsigned)(2 * 127 + 14 - (int)(__float_as_uint(most) >> 23)) << 23) : 1.f;
+  unit *= down;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) bad = fmaf(acc[f][i], 0.f, bad);
-  const unsigned long long m = __ballot(bad != bad);
-  return (unsigned)m | (unsigned)(m >> 32);
-}
-// does any wave of the workgroup say yes? (`votes`: an int a wave)
-template <int NW>
-__device__ __forceinline__ bool at_vote(bool yes, int* votes) {
-  __syncthreads();  // (also: every wave is done with its tiles)
-  if ((threadIdx.x & 63) == 0) votes[threadIdx.x >> 6] = yes;
-  __syncthreads();
-  int any = 0;
+  for (int i = 0; i < 16; ++i) ds[i] *= down;
 #pragma unroll
-  for (int w = 0; w < NW; ++w) any |= votes[w];
-  return __builtin_amdgcn_readfirstlane(any);
+  for (int f = 0; f < FD; ++f) acc[f] *= down;
 }
 // LDS of the key workgroups: their V tile, two stages of (Q, dO) tiles of 32 queries of one head, two of the rows'
 // values (one DMA instruction each, whose upper 32 lanes bring zeros). K stays in registers as the score's operand; V does
@@ -117,60 +112,8 @@ template <typename T, int DF, int NW, int KW> struct AtBwdLds {
   static constexpr int SUM = KW * 64 * DF / 2;                          // floats of a group's dK or dV
   static constexpr int KEYS = VT + NG * GROUP, ROWS = 4 * KT * RB, ADD = NG > 1 ? (NG > 2 ? 4 : 2) * SUM * 4 : 0;
   static constexpr int MOST = KEYS > ROWS ? KEYS : ROWS;
-  static constexpr int BYTES = (MOST > ADD ? MOST : ADD) + 16 * (int)sizeof(int);
+  static constexpr int BYTES = (MOST > ADD ? MOST : ADD) + 32 * (int)sizeof(int);  // (and 32 ints: ranges, a vote)
 };
-
-// dk, dv of one key over the queries in [q0, q1] that see it: each lane holds dims lane and lane + 64
-template <typename T, bool CAP, bool SLOPE>
-__device__ void at_key_alone(const AtArgs& a, int b, int kh, int j, int q0, int q1, int lane, float dk[2], float dv[2]) {
-  const T* kj = (const T*)a.k + b * a.k_sb + kh * a.k_sh + j * a.k_sl;
-  const T* vj = (const T*)a.v + b * a.v_sb + kh * a.v_sh + j * a.v_sl;
-  const bool on0 = lane < a.d, on1 = lane + 64 < a.d;
-  const float k0 = on0 ? ld(kj + lane) : 0.f, k1 = on1 ? ld(kj + lane + 64) : 0.f;
-  const float v0 = on0 ? ld(vj + lane) : 0.f, v1 = on1 ? ld(vj + lane + 64) : 0.f;
-  dk[0] = dk[1] = dv[0] = dv[1] = 0.f;
-  for (int n = 0; n < (q1 - q0 + 1) * a.group; ++n) {
-    const int qi = q0 + n / a.group, head = kh * a.group + n % a.group;
-    const AtSpan sp = at_span(a, b, qi);
-    if (j < sp.lo || j >= sp.hi) continue;
-    const T* q = (const T*)a.q + b * a.q_sb + (long long)qi * a.q_sl + head * a.q_sh;
-    const T* g = (const T*)a.go + (((long long)b * a.lq + qi) * a.hq + head) * a.d;
-    const long long rb = ((long long)b * a.hq + head) * a.lq + qi;
-    const float x0 = on0 ? ld(q + lane) : 0.f, x1 = on1 ? ld(q + lane + 64) : 0.f;
-    const float g0 = on0 ? ld(g + lane) : 0.f, g1 = on1 ? ld(g + lane + 64) : 0.f;
-    const float raw = wave_sum(fmaf(x0, k0, x1 * k1)), dp = wave_sum(fmaf(g0, v0, g1 * v1));
-    float p, ds;
-    at_grad<T, CAP, SLOPE>(a, at_slope<T>(a, head), at_bent<T, CAP, AT_ANY>(a.sc, raw), fabsf((float)(sp.at - j)),
-                           a.lse[rb], dp + a.rowws[rb], p, ds);
-    dk[0] = fmaf(ds, x0, dk[0]), dk[1] = fmaf(ds, x1, dk[1]);
-    dv[0] = fmaf(p, g0, dv[0]), dv[1] = fmaf(p, g1, dv[1]);
-  }
-}
-
-// dq of one packed row over its own span
-template <typename T, bool CAP, bool SLOPE>
-__device__ void at_query_alone(const AtArgs& a, int b, int kh, int r, int lo, int hi, int at, int lane, float dq[2]) {
-  const AtRow x = at_packed(a, kh, r);
-  const T* q = (const T*)a.q + b * a.q_sb + (long long)x.qi * a.q_sl + x.head * a.q_sh;
-  const T* g = (const T*)a.go + (((long long)b * a.lq + x.qi) * a.hq + x.head) * a.d;
-  const bool on0 = lane < a.d, on1 = lane + 64 < a.d;
-  const float q0 = on0 ? ld(q + lane) : 0.f, q1 = on1 ? ld(q + lane + 64) : 0.f;
-  const float g0 = on0 ? ld(g + lane) : 0.f, g1 = on1 ? ld(g + lane + 64) : 0.f;
-  const long long rb = ((long long)b * a.hq + x.head) * a.lq + x.qi;
-  const float lse = a.lse[rb], nd = a.rowws[rb];
-  const float slope = at_slope<T>(a, x.head);
-  dq[0] = dq[1] = 0.f;
-  for (int j = lo; j < hi; ++j) {
-    const T* kj = (const T*)a.k + b * a.k_sb + kh * a.k_sh + j * a.k_sl;
-    const T* vj = (const T*)a.v + b * a.v_sb + kh * a.v_sh + j * a.v_sl;
-    const float k0 = on0 ? ld(kj + lane) : 0.f, k1 = on1 ? ld(kj + lane + 64) : 0.f;
-    const float v0 = on0 ? ld(vj + lane) : 0.f, v1 = on1 ? ld(vj + lane + 64) : 0.f;
-    const float raw = wave_sum(fmaf(q0, k0, q1 * k1)), dp = wave_sum(fmaf(g0, v0, g1 * v1));
-    float p, ds;
-    at_grad<T, CAP, SLOPE>(a, slope, at_bent<T, CAP, AT_ANY>(a.sc, raw), fabsf((float)(at - j)), lse, dp + nd, p, ds);
-    dq[0] = fmaf(ds, k0, dq[0]), dq[1] = fmaf(ds, k1, dq[1]);
-  }
-}
 
 template <typename T, int DF, bool CAP, bool SLOPE, int NW, int KW>
 __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, char* smem) {
@@ -178,7 +121,8 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
   constexpr int DP = AtPad<DF>::DP, KS = AtOffsets<T, DF>::KS, FD = DF / 32;
   constexpr int TILE = L::QTILE, STAGE = 2 * TILE;
   constexpr int NG = L::NG, NT = 64 * NW;
-  int* range = (int*)(smem + L::BYTES) - 16;
+  int* range = (int*)(smem + L::BYTES) - 32;
+  if (threadIdx.x == 0) range[16] = 0;
   const int lane = threadIdx.x & 63, w8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int wid = w8 % KW, grp = w8 / KW;  // 32 keys; which of the query tiles
   const int b = bh / a.hk, kh = bh - b * a.hk;
@@ -270,17 +214,17 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
   for (int f = 0; f < FD; ++f) dk[f] = at_zero(), dv[f] = at_zero();
   const AtOffsets<T, DF> off(lane);
   const char* V = smem + wid * 32 * L::RB;
-  float unit = 1.f;  // dS and dk stand in
+  float unit = 1.f;  // that ds and dk are in (at_fit)
   const int n0 = (at_keys(a, b)) - a.lq;  // position of query 0
   const char* const base = smem + L::VT + grp * L::GROUP;
-  auto step = [&](auto stage) {
+  auto step = [&](auto stage, auto again) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     int g1 = g, i1 = i0;  // the next one
     advance(NG, g1, i1);
-    if (g1 < a.group) issue(1 - stage.value, g1, i1);
-    const char* Q = base + stage.value * STAGE;
+    if (g1 < a.group) issue(1 - stage, g1, i1);
+    const char* Q = base + stage * STAGE;
     const char* G = Q + TILE;
-    const AtRowData& x = *(const AtRowData*)(base + 2 * STAGE + stage.value * (int)sizeof(AtRowData));
+    const AtRowData& x = *(const AtRowData*)(base + 2 * STAGE + stage * (int)sizeof(AtRowData));
     const int f_lo = x.lo[lane & 31], f_hi = x.hi[lane & 31];
     if (g < a.group && __any(f_hi > kw0 && f_lo < kw0 + 32)) {      // some row sees some of this wave's keys
       const bool full = __all(f_lo <= kw0 && f_hi >= kw0 + 32);     // every row sees all of them
@@ -302,7 +246,7 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
         for (int r = 0; r < 4; ++r) {
           const int i = 4 * r4 + r;
           at_grad<T, CAP, SLOPE>(a, slope, s[i], fabsf(x0 + (float)(8 * r4 + r)), lp[r],
-                                 AT_AGAIN<T> ? (dp[i] + dl[r]) * unit : dp[i] + dl[r], p[i], ds[i]);
+                                 dp[i] + dl[r], p[i], ds[i]);
         }
       }
       if (!full) {
@@ -319,35 +263,48 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
         }
       }
       // p and ds are rounded to the 16-bit operand type (half a step each)
-      at_accumulate<T, DF>(G, off, 0, AtP<T>(p), dv, lane);
-      at_accumulate<T, DF>(Q, off, 0, AtP<T>(ds), dk, lane);
+      const auto sees = [&](int r) { return key >= x.lo[r] && key < x.hi[r]; };
+      if (again.value && !full && at_has_nonfinite<T, DF>(G, 0, lane))
+        at_accumulate_seen<T, DF>(G, 0, p, dv, lane, sees);
+      else
+        at_accumulate<T, DF>(G, off, 0, AtP<T>(p), dv, lane);
+      if constexpr (again.value && AT_FIT<T>) at_fit<FD>(ds, dk, unit);
+      if (again.value && !full && at_has_nonfinite<T, DF>(Q, 0, lane))
+        at_accumulate_seen<T, DF>(Q, 0, ds, dk, lane, sees);
+      else
+        at_accumulate<T, DF>(Q, off, 0, AtP<T>(ds), dk, lane);
     }
     g = g1, i0 = i1;
   };
+  auto walk = [&](auto again) {
+    if (q1 < 0) return;
+    // (uniform over the workgroup: the first group's count)
+    const int nt = (a.group * ((q1 - q0) / AT_QT + 1) + NG - 1) / NG;
+    if constexpr (again.value) {  // (one copy of the code: its stages need not be constants)
 #pragma unroll 1
-  for (int walk = 0;; ++walk) {
-    if (q1 >= 0) {
-      // (uniform over the workgroup: the first group's count)
-      const int nt = (a.group * ((q1 - q0) / AT_QT + 1) + NG - 1) / NG;
+      for (int t = 0; t < nt; ++t) step(t & 1, again);
+    } else {
       for (int t = 0; t < nt; t += 2) {
-        step(std::integral_constant<int, 0>{});
-        if (t + 1 < nt) step(std::integral_constant<int, 1>{});
+        step(std::integral_constant<int, 0>{}, again);
+        if (t + 1 < nt) step(std::integral_constant<int, 1>{}, again);
       }
     }
-    if (!AT_AGAIN<T> || walk == 1) break;
-    const unsigned over = at_not_finite<FD>(dk);
-    if (!at_vote<NW>(over != 0, range)) break;
-    unit = (over >> (lane & 31)) & 1 ? AT_DOWN : 1.f;
+  };
+  walk(std::false_type{});
+  const bool masked = a.causal || a.spans || a.kv_lens;
+  if (masked || AT_FIT<T>) {
+    const bool bad = at_bad_columns<FD>(dk) != 0 || (masked && at_bad_columns<FD>(dv) != 0);
+    if (__builtin_expect(at_vote(bad, range + 16), 0)) {  // (unlikely: its spills stay out of the first walk)
 #pragma unroll
-    for (int f = 0; f < FD; ++f) dk[f] = at_zero(), dv[f] = at_zero();
-    g = 0, i0 = q0;
-    advance(grp, g, i0);
-    if (q1 >= 0 && g < a.group) issue(0, g, i0);
-  }
-  if constexpr (AT_AGAIN<T>) {
-    unit = 1.f / unit;
+      for (int f = 0; f < FD; ++f) dk[f] = at_zero(), dv[f] = at_zero();
+      g = 0, i0 = q0;
+      advance(grp, g, i0);
+      if (q1 >= 0 && g < a.group) issue(0, g, i0);
+      walk(std::true_type{});
+      unit = 1.f / unit;
 #pragma unroll
-    for (int f = 0; f < FD; ++f) dk[f] *= unit;
+      for (int f = 0; AT_FIT<T> && f < FD; ++f) dk[f] *= unit;
+    }
   }
   if constexpr (NG > 1) {  // the groups' sums through LDS: dK's to the first group, dV's to the second
     float* sum = (float*)smem + wid * 64 * (DF / 2) + lane;
@@ -392,31 +349,13 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
       }
   }
   // with two groups each stores one of the two (dv of the second group now in dk)
-  float bad = 0.f;
-#pragma unroll
-  for (int f = 0; f < FD; ++f)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) bad = NG > 1 ? fmaf(dk[f][i], 0.f, bad) : fmaf(dk[f][i], 0.f, fmaf(dv[f][i], 0.f, bad));
-  const unsigned long long redo = __ballot(key < a.lk && bad != bad);
-  const unsigned alone = (unsigned)redo | (unsigned)(redo >> 32);
   const long long ko = ((long long)b * a.lk * a.hk + kh) * a.d, ks = (long long)a.hk * a.d;
-  const bool mine = key < a.lk && !((alone >> (lane & 31)) & 1);
+  const bool mine = key < a.lk;
   if constexpr (NG > 1) {
     at_store_row<T, DF>((T*)(grp ? a.dv : a.dk) + ko + key * ks, dk, a.d, h, grp ? 1.f : a.scale, mine);
   } else {
     at_store_row<T, DF>((T*)a.dk + ko + key * ks, dk, a.d, h, a.scale, mine);
     at_store_row<T, DF>((T*)a.dv + ko + key * ks, dv, a.d, h, 1.f, mine);
-  }
-  for (unsigned todo = alone; todo; todo &= todo - 1) {
-    const int j = kw0 + __builtin_ctz(todo);
-    float gk[2], gv[2];
-    at_key_alone<T, CAP, SLOPE>(a, b, kh, j, q0, q1, lane, gk, gv);
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (lane + 64 * e < a.d) {
-        if (NG == 1 || grp == 0) st((T*)a.dk + ko + j * ks + lane + 64 * e, gk[e] * a.scale);
-        if (NG == 1 || grp == 1) st((T*)a.dv + ko + j * ks + lane + 64 * e, gv[e]);
-      }
   }
 }
 
@@ -425,7 +364,8 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
   typedef AtBwdLds<T, DF, NW, KW> L;
   constexpr int DP = AtPad<DF>::DP, KS = AtOffsets<T, DF>::KS, FD = DF / 32, KT = L::KT;
   constexpr int TILE = KT * L::RB, STAGE = 2 * TILE;
-  int* range = (int*)(smem + L::BYTES) - 16;
+  int* range = (int*)(smem + L::BYTES) - 32;
+  if (threadIdx.x == 0) range[16] = 0;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int b = bh / a.hk, kh = bh - b * a.hk, rows = a.lq * a.group;
   const int row = tile * 32 * NW + wid * 32 + (lane & 31);
@@ -475,16 +415,16 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
   }
   const float slope = SLOPE ? at_slope<T>(a, pr.head) : 0.f;
   const AtOffsets<T, DF> off(lane);
-  float unit = 1.f;  // dS and dq stand in: in the exponent of p
+  float unit = 1.f;  // that ds and dq are in (at_fit)
   at_f32x16 dq[FD];
 #pragma unroll
   for (int f = 0; f < FD; ++f) dq[f] = at_zero();
-  auto step = [&](auto stage, int t) {
+  auto step = [&](auto stage, auto again, int t) {
     const int k0 = k_lo + t * KT;
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (t + 1 < nt) issue(1 - stage.value, k0 + KT);
+    if (t + 1 < nt) issue(1 - stage, k0 + KT);
     if (k0 >= w_hi || k0 + KT <= w_lo) return;
-    const char* K = smem + stage.value * STAGE;
+    const char* K = smem + stage * STAGE;
     const char* V = K + TILE;
     const bool part = k0 < i_lo || k0 + KT > i_hi;
 #pragma unroll
@@ -509,54 +449,49 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
         for (int i = 0; i < 16; ++i)
           if (8 * (i >> 2) + (i & 3) < lo || 8 * (i >> 2) + (i & 3) >= hi) ds[i] = 0.f;
       }
-      at_accumulate<T, DF>(K, off, 32 * f, AtP<T>(ds), dq, lane);
+      if constexpr (again.value && AT_FIT<T>) at_fit<FD>(ds, dq, unit);
+      if (again.value && part && at_has_nonfinite<T, DF>(K, 32 * f, lane))
+        at_accumulate_seen<T, DF>(K, 32 * f, ds, dq, lane,
+                                  [&](int r) { return k0 + 32 * f + r >= sp.lo && k0 + 32 * f + r < sp.hi; });
+      else
+        at_accumulate<T, DF>(K, off, 32 * f, AtP<T>(ds), dq, lane);
     }
   };
+  auto walk = [&](auto again) {
+    if constexpr (again.value) {
 #pragma unroll 1
-  for (int walk = 0;; ++walk) {
-    for (int t = 0; t < nt; t += 2) {
-      step(std::integral_constant<int, 0>{}, t);
-      if (t + 1 < nt) step(std::integral_constant<int, 1>{}, t + 1);
+      for (int t = 0; t < nt; ++t) step(t & 1, again, t);
+    } else {
+      for (int t = 0; t < nt; t += 2) {
+        step(std::integral_constant<int, 0>{}, again, t);
+        if (t + 1 < nt) step(std::integral_constant<int, 1>{}, again, t + 1);
+      }
     }
-    if (!AT_AGAIN<T> || walk == 1) break;
-    const unsigned over = at_not_finite<FD>(dq);
-    if (!at_vote<NW>(over != 0, range)) break;
-    if ((over >> (lane & 31)) & 1) unit = AT_DOWN, lse += 25.f;
+  };
+  walk(std::false_type{});
+  if (a.causal || a.spans || AT_FIT<T>) {
+    if (__builtin_expect(at_vote(at_bad_columns<FD>(dq) != 0, range + 16), 0)) {
 #pragma unroll
-    for (int f = 0; f < FD; ++f) dq[f] = at_zero();
-    if (nt > 0) issue(0, k_lo);
+      for (int f = 0; f < FD; ++f) dq[f] = at_zero();
+      if (nt > 0) issue(0, k_lo);
+      walk(std::true_type{});
+      unit = 1.f / unit;
+#pragma unroll
+      for (int f = 0; AT_FIT<T> && f < FD; ++f) dq[f] *= unit;
+    }
   }
-  float bad = 0.f;
-#pragma unroll
-  for (int f = 0; f < FD; ++f)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) bad = fmaf(dq[f][i], 0.f, bad);
-  const unsigned long long redo = __ballot(live && bad != bad);
-  const unsigned alone = (unsigned)redo | (unsigned)(redo >> 32);
   if (!live) {
 #pragma unroll
     for (int f = 0; f < FD; ++f) dq[f] = at_zero();
   }
-  at_store_row<T, DF>((T*)a.dq + orow, dq, a.d, h, a.scale / unit, row < rows && !((alone >> (lane & 31)) & 1));
-  for (unsigned todo = alone; todo; todo &= todo - 1) {
-    const int n = __builtin_ctz(todo);
-    const int r = __shfl(row, n, 64);
-    const AtRow x = at_packed(a, kh, r);
-    float g[2];
-    at_query_alone<T, CAP, SLOPE>(a, b, kh, r, __shfl(sp.lo, n, 64), __shfl(sp.hi, n, 64), __shfl(sp.at, n, 64), lane, g);
-    T* out = (T*)a.dq + (((long long)b * a.lq + x.qi) * a.hq + x.head) * a.d;
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (lane + 64 * e < a.d) st(out + lane + 64 * e, g[e] * a.scale);
-  }
+  at_store_row<T, DF>((T*)a.dq + orow, dq, a.d, h, a.scale, row < rows);
 }
 
 // blockIdx.y first counts the workgroups of 32 KW keys (the first keys are seen by most queries), then those of 32 NW packed
 // rows, the last rows first, or the other way round (rows_first); heads vary fastest, as in the forward
-// (f16 of 64 dims needs just over the 168 registers that let three waves a SIMD run: 32 x 257 tokens, 12 heads, capped: 94 us
-// without the bound, 81 with it)
+// (waves a SIMD: what the first walk's registers allow; the second one's would allow fewer, and spills instead)
 template <typename T, int DF, bool CAP, bool SLOPE, int NW, int KW>
-__global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 && DF > 64 ? 1 : AT_AGAIN<T> && DF == 64 ? 3 : 2) k_mattn_bwd(AtArgs a) {
+__global__ void __launch_bounds__(64 * NW, sizeof(T) == 4 ? (DF > 64 ? 1 : 2) : DF == 32 ? 4 : DF == 64 ? 3 : 2) k_mattn_bwd(AtArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int ktiles = (a.lk + 32 * KW - 1) / (32 * KW), y = blockIdx.y;
   const int t = !a.rows_first ? y : y + ktiles < (int)gridDim.y ? y + ktiles : y + ktiles - gridDim.y;

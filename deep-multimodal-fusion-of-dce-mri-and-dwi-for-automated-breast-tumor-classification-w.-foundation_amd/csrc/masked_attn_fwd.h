@@ -11,10 +11,8 @@
 // unnormalised accumulators with (max, sum), and k_mattn_join adds them. Chunks are cut at absolute keys, so a short row of a
 // long cache leaves workgroups that exit at once instead of long ones that hold the others up.
 //
-// A masked key has p = 0 exactly, but 0 * NaN is NaN: a NaN or infinity in a value that some row of the tile may not see
-// would reach that row. Keys outside the union of the workgroup's spans are zero-filled on load; for the rest, a wave whose
-// accumulators end up non-finite recomputes the rows in question key by key over their own spans (at_row_alone), which
-// costs nothing where the values are finite.
+// Keys outside the union of the workgroup's spans are zero-filled on load; a value inside it that is not finite stays with the
+// rows that see it by a second walk (at_accumulate_seen).
 //
 // Bound: for many rows the vector ALU (exponential, maximum, cap) beside the matrix pipe, which both waves of a SIMD share:
 // 8192 x 8192 tokens, 32 heads over 8 of 128, bf16: 1.04 to 1.18 ms by the inputs' scale (0.93 to 1.06 PFLOP/s; a large matrix
@@ -24,33 +22,6 @@
 #include "masked_attn.h"
 
 namespace dmf {
-
-// one row over its own span only: each lane holds dims lane and lane + 64
-template <typename T, bool CAP, bool SLOPE>
-__device__ void at_row_alone(const AtArgs& a, const T* q, const T* k, const T* v, int lo, int hi, int at, int head,
-                             int lane, float& m, float& l, float& o0, float& o1) {
-  const float slope = at_slope<T>(a, head);
-  const float q0 = lane < a.d ? ld(q + lane) : 0.f, q1 = lane + 64 < a.d ? ld(q + lane + 64) : 0.f;
-  m = -INFINITY;
-  l = o0 = o1 = 0.f;
-  for (int j = lo; j < hi; ++j) {
-    const T* kj = k + j * a.k_sl;
-    const T* vj = v + j * a.v_sl;
-    float dot = 0.f;
-    if (lane < a.d) dot = q0 * ld(kj + lane);
-    if (lane + 64 < a.d) dot = fmaf(q1, ld(kj + lane + 64), dot);
-    dot = wave_sum(dot);
-    const float s = at_score<T, CAP, SLOPE>(a.sc, slope, dot, fabsf((float)(at - j)));
-    const float mn = fmaxf(m, s), ms = mn == -INFINITY ? 0.f : mn;
-    const float alpha = at_exp<T>(m - ms), p = at_exp<T>(s - ms);
-    m = mn;
-    l = fmaf(l, alpha, p);
-    o0 = o0 * alpha;
-    o1 = o1 * alpha;
-    if (lane < a.d) o0 = fmaf(p, ld(vj + lane), o0);
-    if (lane + 64 < a.d) o1 = fmaf(p, ld(vj + lane + 64), o1);
-  }
-}
 
 template <typename T>
 __device__ __forceinline__ void at_store4(T* p, const float* v) {  // p aligned to 4 elements
@@ -102,12 +73,19 @@ __device__ __forceinline__ void at_store_row(T* out, const at_f32x16* acc, int d
   }
 }
 
+// waves a SIMD: what the first walk's registers allow (the second one's would allow fewer, and spills instead)
+template <typename T> constexpr int at_fwd_waves(int df, bool cap, int nw, int kt) {
+  if (sizeof(T) == 4) return df == 32 ? 4 : df == 64 ? (nw == 1 ? 2 : 3) : df == 96 ? 2 : 1;
+  if (nw == 1) return df == 32 ? 5 : df == 64 ? 3 : 2;  // (LDS for no more)
+  return df == 32 ? 5 : df == 64 ? 4 : df == 96 ? 3 : kt == 32 && (nw == 4 || !cap) ? 3 : 2;
+}
 template <typename T, int DF, bool CAP, bool SLOPE, bool TRAIN, int NW, int NG, int KT>
-__global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 ? (DF > 64 ? 1 : 2) : NW == 4 && KT == 32 ? 3 : 2) k_mattn_fwd(AtArgs a) {
+__global__ void __launch_bounds__(64 * NW * NG, at_fwd_waves<T>(DF, CAP, NW, KT)) k_mattn_fwd(AtArgs a) {
   constexpr int DP = AtPad<DF>::DP, KS = AtOffsets<T, DF>::KS, FD = DF / 32, KF = KT / 32;
   constexpr int TILE = KT * DP * AtT<T>::E, STAGE = 2 * TILE;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ int range[2 * NW];
+  __shared__ int range[2 * NW], again_flag;
+  if (threadIdx.x == 0) again_flag = 0;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5;
   const int wid = NG > 1 ? wave % NW : wave, grp = NG > 1 ? wave / NW : 0;  // 32 rows; which of the key tiles
   const int nbh = a.batch * a.hk, rows = a.lq * a.group;
@@ -180,13 +158,13 @@ __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 ? (DF > 64 ? 1 : 
   // products and bent alone
   constexpr bool LATE = CAP && !SLOPE && sizeof(T) == 2;
   const char* const base = smem + grp * 2 * STAGE;
-  auto step = [&](auto stage, int t) {  // tile t of all, or none (t >= nt: a group that has run out keeps the barriers)
+  auto step = [&](auto stage, auto again, int t) {  // tile t of all, or none (t >= nt: a group that has run out keeps the barriers)
     const int k0 = k_lo + t * KT;
     // this tile has landed (in every wave: the barrier); the other stage's last readers are past it too
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (t + NG < nt) issue(1 - stage.value, k0 + NG * KT);
+    if (t + NG < nt) issue(1 - stage, k0 + NG * KT);
     if (t >= nt || k0 >= w_hi || k0 + KT <= w_lo) return;  // (wave-uniform) nothing here for these rows
-    const char* K = base + stage.value * STAGE;
+    const char* K = base + stage * STAGE;
     const char* V = K + TILE;
     at_f32x16 s[KF];
 #pragma unroll
@@ -284,6 +262,18 @@ __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 ? (DF > 64 ? 1 : 
       // is multiplied too: its delta = do.o stands for sum_j p dp, and an error of o would pass into dS through whole rows
       // (dq's error against 64 bits 1.47 to 1.52 times a rounding's instead of 1.42).
       const AtP<T> pk(p);
+      if constexpr (again.value)
+        if (part && at_has_nonfinite<T, DF>(V, 32 * f, lane)) {
+          float w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            w[i] = sizeof(T) == 4 || TRAIN ? p[i] : Cvt<T>::load(Cvt<T>::store(p[i]));
+            (sizeof(T) == 4 || TRAIN ? lx : l) += w[i];
+          }
+          at_accumulate_seen<T, DF>(V, 32 * f, w, acc, lane,
+                                    [&](int r) { return k0 + 32 * f + r >= sp.lo && k0 + 32 * f + r < sp.hi; });
+          continue;
+        }
       if constexpr (sizeof(T) == 2) {
         if constexpr (TRAIN) {
 #pragma unroll
@@ -302,9 +292,27 @@ __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 ? (DF > 64 ? 1 : 
       }
     }
   };
-  for (int t = 0; t < nt; t += 2 * NG) {
-    step(std::integral_constant<int, 0>{}, t + grp);
-    if (t + NG < nt) step(std::integral_constant<int, 1>{}, t + NG + grp);
+  auto walk = [&](auto again) {
+    if constexpr (again.value) {  // (one copy of the code: its stages need not be constants)
+#pragma unroll 1
+      for (int t = 0, s = 0; t < nt; t += NG, s ^= 1) step(s, again, t + grp);
+    } else {
+      for (int t = 0; t < nt; t += 2 * NG) {
+        step(std::integral_constant<int, 0>{}, again, t + grp);
+        if (t + NG < nt) step(std::integral_constant<int, 1>{}, again, t + NG + grp);
+      }
+    }
+  };
+  walk(std::false_type{});
+  if (a.causal || a.spans) {
+    const bool bad = at_bad_columns<FD>(acc, (l + lx) * 0.f) != 0;
+    if (at_vote(bad, &again_flag)) {
+      m = -INFINITY, ms = l = lx = 0.f;
+#pragma unroll
+      for (int f = 0; f < FD; ++f) acc[f] = at_zero();
+      if (grp < nt) issue(0, k_lo + grp * KT);
+      walk(std::true_type{});
+    }
   }
   lx = at_half_sum(lx);
   l = sizeof(T) == 4 || TRAIN ? lx : at_half_sum(l);
@@ -331,18 +339,10 @@ __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 ? (DF > 64 ? 1 : 
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[f][i] = acc[f][i] * w0 + part[(16 * f + i + 3) * 64] * w1;
   }
-  float bad = l * 0.f;
-#pragma unroll
-  for (int f = 0; f < FD; ++f)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) bad = fmaf(acc[f][i], 0.f, bad);
-  const unsigned long long redo = __ballot(live && bad != bad);
-  const unsigned alone = (unsigned)redo | (unsigned)(redo >> 32);
-
   const long long prow = ((long long)split * nbh + bh) * rows + row;  // partials
   T* ob = (T*)a.o + (((long long)b * a.lq + qi) * a.hq + head) * a.d;
   T* olo = TRAIN ? (T*)a.o_lo + (((long long)b * a.lq + qi) * a.hq + head) * a.d : nullptr;
-  const bool mine = row < rows && !((alone >> (lane & 31)) & 1);
+  const bool mine = row < rows;
   if (a.splits > 1) {
     if (mine) {
       float* po = a.po + prow * a.d;
@@ -362,37 +362,6 @@ __global__ void __launch_bounds__(64 * NW * NG, sizeof(T) == 4 ? (DF > 64 ? 1 : 
     }
     at_store_row<T, DF, TRAIN>(ob, acc, a.d, h, live ? 1.f / l : 0.f, mine, olo);
     if (a.lse && mine && h == 0) a.lse[((long long)b * a.hq + head) * a.lq + qi] = live ? ms + at_log<T>(lx) : INFINITY;
-  }
-  for (unsigned todo = alone; todo; todo &= todo - 1) {
-    const int n = __builtin_ctz(todo);
-    const int r_lo = max(__shfl(sp.lo, n, 64), k_lo), r_hi = min(__shfl(sp.hi, n, 64), k_hi);
-    const int r_at = __shfl(sp.at, n, 64), r_qi = __shfl(qi, n, 64), r_head = __shfl(head, n, 64);
-    float rm, rl, o0, o1;
-    at_row_alone<T, CAP, SLOPE>(a, (const T*)a.q + b * a.q_sb + (long long)r_qi * a.q_sl + r_head * a.q_sh, kb, vb, r_lo,
-                                r_hi, r_at, r_head, lane, rm, rl, o0, o1);
-    const long long pr = prow - row + __shfl(row, n, 64), orow = (((long long)b * a.lq + r_qi) * a.hq + r_head) * a.d;
-    if (a.splits == 1) {
-      o0 /= rl;
-      o1 /= rl;
-    }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int e = lane + 64 * k;
-      const float o = k ? o1 : o0;
-      if (e >= a.d) continue;
-      if (a.splits > 1) {
-        a.po[pr * a.d + e] = o;
-      } else {
-        st((T*)a.o + orow + e, o);
-        if (TRAIN) st((T*)a.o_lo + orow + e, o - Cvt<T>::load(Cvt<T>::store(o)));
-      }
-    }
-    if (lane == 0) {
-      if (a.splits > 1)
-        *(float4*)(a.pml + 4 * pr) = make_float4(rm, rl, rl, 0.f);
-      else if (a.lse)
-        a.lse[((long long)b * a.hq + r_head) * a.lq + r_qi] = (rm == -INFINITY ? 0.f : rm) + at_log<T>(rl);
-    }
   }
 }
 

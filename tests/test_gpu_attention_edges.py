@@ -171,3 +171,84 @@ def test_attention_f16_large_score_gradients(shape, mode):
     for i, name in enumerate(("o", "dq", "dk", "dv")):
         assert ref[2 * i].abs().max() < 65504, name
         T._within(got[i], ref[2 * i], ref[2 * i + 1], name)
+
+
+def _ms(f):
+    f()
+    times = []
+    for _ in range(4):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        f()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b))
+    return min(times)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("where", ["key 0", "gradient", "all"])
+def test_attention_non_finite_inputs_cost_a_second_walk(where, causal, dt):
+    """What is not finite and seen (a key that all see, an output gradient that overflowed, everything) makes a call at most
+    a few times as long: a second walk over the tiles, and the pairs of its masked tiles one by one."""
+    n, h, d = 2048, 8, 64
+    q, k, v, go = (T._randn((1, n, h, d), dt, s) for s in (1, 2, 3, 4))
+
+    def step():
+        return _grads(q, k, v, go, causal=causal)
+
+    clean = _ms(step)
+    if where == "key 0":
+        k[:, 0, :, 3], v[:, 0, :, 5] = float("nan"), float("inf")
+    elif where == "gradient":
+        go[:, n // 2, :, 7] = float("inf")
+    else:
+        for t in (q, k, v, go):
+            t.fill_(float("nan"))
+    bad = _ms(step)
+    o, dq, dk, dv = step()
+    if where == "gradient":
+        assert torch.isfinite(o).all() and torch.isnan(dq[:, n // 2]).all() and torch.isinf(dv[:, 0, :, 7]).all()
+        assert torch.isfinite(dq[:, n // 2 + 1:]).all() and torch.isfinite(dq[:, :n // 2]).all()
+        if causal:
+            assert torch.isfinite(dk[:, n // 2 + 1:]).all() and torch.isfinite(dv[:, n // 2 + 1:]).all()
+    else:
+        assert torch.isnan(o).all() and torch.isnan(dq).all()
+    assert bad < 8 * clean, (bad, clean)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("hq,hk,d,mode", [(4, 1, 128, dict(cap=20.0)), (2, 2, 64, dict(slopes=True)), (3, 1, 80, dict())])
+def test_attention_long_rows_hide_garbage(hq, hk, d, mode, causal, dt):
+    """Packed documents beside padding that holds infinities and NaN in every operand, and a document whose last key nobody but
+    its own query sees: tiles that rows see in part, rows split over workgroups."""
+    n = 1300
+    docs = torch.full((1, n), -1, dtype=torch.int32)
+    for i, (a, b) in enumerate(((0, 7), (30, 500), (511, 640), (641, 1200))):
+        docs[0, a:b] = i
+    q, k, v, go = (T._randn((1, n, h, d), dt, s) for h, s in ((hq, 1), (hk, 2), (hk, 3), (hq, 4)))
+    see, at = T._see(1, n, n, causal, None, None, docs)
+    sl = torch.tensor([2.0 ** (-4.0 * (h + 1) / hq) for h in range(hq)], device=DEV) if mode.get("slopes") else None
+    cap = mode.get("cap", 0.0)
+    ref = T._attn_ref(q, k, v, see, at, d ** -0.5, cap, sl, go)
+    pad = (docs[0] < 0).to(DEV)
+    for j, t in enumerate((q, k, v, go)):
+        t[:, pad] = float("nan") if j % 2 else float("inf")
+        t[:, pad, :, ::3] = -float("inf")
+    if causal:
+        v[0, 499, :, 1] = float("inf")      # the key of its document's last query
+    ins = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = A.attention(*ins, causal=causal, documents=docs.to(DEV), softcap=cap, slopes=sl)
+    grads = torch.autograd.grad(o, ins, go)
+    keep = torch.ones(n, dtype=torch.bool, device=DEV)
+    if causal:
+        keep[499] = False                   # its output is infinite, its gradients not a number
+        assert torch.isinf(o[0, 499, :, 1]).all()
+    T._within(o.detach()[:, keep], ref[0][:, keep], ref[1][:, keep], "o")
+    T._within(grads[0][:, keep], ref[2][:, keep], ref[3][:, keep], "dq")
+    keep[30:500] &= not causal              # (its gradients reach its document's keys)
+    T._within(grads[1][:, keep], ref[4][:, keep], ref[5][:, keep], "dk")
+    keep[30:499] = True
+    T._within(grads[2][:, keep], ref[6][:, keep], ref[7][:, keep], "dv")
