@@ -426,6 +426,11 @@ __device__ __forceinline__ float at_log(float x) {
     return __builtin_amdgcn_logf(x);  // log2
 }
 
+// f16 probabilities below 2^-14 would be subnormal as operands and those of a long flat tail beside one dominant key vanish, so
+// they are multiplied by 2^LIFT: in the forward p <= 2^8 (the maximum's lag) becomes at most 2^15, through the exponent; in the
+// backward p <= 1 does. What is left is 2^-32 (2^-40) a key. bf16 has f32's exponents.
+template <typename T> struct AtLift { static constexpr float FWD = __is_same(T, f16_t) ? 7.f : 0.f, BWD = __is_same(T, f16_t) ? 32768.f : 1.f; };
+
 // CAP. The scores are bound by the vector ALU, and there by v_exp / v_rcp (a quarter of the rate): tanh as
 // 1 - 2 / (exp(2 x) + 1) takes two of them and four more operations. While no score of a tile exceeds the cap
 // (|x| <= 1, checked per wave and tile with half an operation a score), tanh(x) / x is a polynomial of degree 5 in x^2

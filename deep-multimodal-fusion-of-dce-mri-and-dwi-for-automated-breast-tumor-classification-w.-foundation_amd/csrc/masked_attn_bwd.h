@@ -262,6 +262,8 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
           }
         }
       }
+#pragma unroll
+      for (int i = 0; AtLift<T>::BWD != 1.f && i < 16; ++i) p[i] *= AtLift<T>::BWD;
       // p and ds are rounded to the 16-bit operand type (half a step each)
       const auto sees = [&](int r) { return key >= x.lo[r] && key < x.hi[r]; };
       if (again.value && !full && at_has_nonfinite<T, DF>(G, 0, lane))
@@ -352,10 +354,10 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
   const long long ko = ((long long)b * a.lk * a.hk + kh) * a.d, ks = (long long)a.hk * a.d;
   const bool mine = key < a.lk;
   if constexpr (NG > 1) {
-    at_store_row<T, DF>((T*)(grp ? a.dv : a.dk) + ko + key * ks, dk, a.d, h, grp ? 1.f : a.scale, mine);
+    at_store_row<T, DF>((T*)(grp ? a.dv : a.dk) + ko + key * ks, dk, a.d, h, grp ? 1.f / AtLift<T>::BWD : a.scale, mine);
   } else {
     at_store_row<T, DF>((T*)a.dk + ko + key * ks, dk, a.d, h, a.scale, mine);
-    at_store_row<T, DF>((T*)a.dv + ko + key * ks, dv, a.d, h, 1.f, mine);
+    at_store_row<T, DF>((T*)a.dv + ko + key * ks, dv, a.d, h, 1.f / AtLift<T>::BWD, mine);
   }
 }
 

@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(64 * NW * NG, at_fwd_waves<T>(DF, CAP, NW, KT)
   at_f32x16 acc[FD];
 #pragma unroll
   for (int f = 0; f < FD; ++f) acc[f] = at_zero();
-  // ms: m, or 0 while there is none; the sum that o is divided by: l, of the probabilities as the products take them
+  // ms: m (0 while there is none) less the lift; the sum that o is divided by: l, of the probabilities as the products take them
   // (rounded: then the rounding of a dominant key cancels), or lx, of the unrounded ones, where their rest is taken too
   float m = -INFINITY, ms = 0.f, l = 0.f, lx = 0.f;
   const AtOffsets<T, DF> off(lane);
@@ -221,6 +221,7 @@ __global__ void __launch_bounds__(64 * NW * NG, at_fwd_waves<T>(DF, CAP, NW, KT)
       ms = mn == -INFINITY ? 0.f : mn;
       const float alpha = at_exp<T>(m - ms);
       m = mn;
+      ms -= AtLift<T>::FWD;
       l *= alpha;
       lx *= alpha;
 #pragma unroll
@@ -332,6 +333,7 @@ __global__ void __launch_bounds__(64 * NW * NG, at_fwd_waves<T>(DF, CAP, NW, KT)
     ms = mn == -INFINITY ? 0.f : mn;
     const float w0 = at_exp<T>(m - ms), w1 = at_exp<T>(m1 - ms);
     m = mn;
+    ms -= AtLift<T>::FWD;
     l = l * w0 + part[64] * w1;
     lx = lx * w0 + part[128] * w1;
 #pragma unroll
@@ -412,7 +414,7 @@ __global__ void __launch_bounds__(256) k_mattn_join(AtArgs a) {
     }
   }
   if (!in) return;
-  if (a.lse && lane == 0) a.lse[((long long)b * a.hq + pr.head) * a.lq + pr.qi] = live ? ms + at_log<T>(lx) : INFINITY;
+  if (a.lse && lane == 0) a.lse[((long long)b * a.hq + pr.head) * a.lq + pr.qi] = live ? ms - AtLift<T>::FWD + at_log<T>(lx) : INFINITY;
   if (!on) return;
   const long long orow = (((long long)b * a.lq + pr.qi) * a.hq + pr.head) * a.d + 4 * lane;
   const float inv = live ? 1.f / l : 0.f;

@@ -252,3 +252,38 @@ def test_attention_long_rows_hide_garbage(hq, hk, d, mode, causal, dt):
     T._within(grads[1][:, keep], ref[4][:, keep], ref[5][:, keep], "dk")
     keep[30:499] = True
     T._within(grads[2][:, keep], ref[6][:, keep], ref[7][:, keep], "dv")
+
+
+@pytest.mark.parametrize("tail", [-14.9, -16.2, -17.5])
+@pytest.mark.parametrize("mode", [dict(), dict(cap=1000.0), dict(slopes=True)], ids=lambda m: "-".join(m) or "plain")
+def test_attention_f16_dominant_key_over_a_flat_tail(mode, tail):
+    """One key far above thousands of equal ones, whose probabilities together are a thousandth: in f16 each of them errs by a
+    half step of its own value down to 2^-32 of the largest (2^-40 in dV), not by 2^-25 (T._tiny, set accordingly)."""
+    import dmf_native as N
+
+    b, n, h, d, dt = 8, 4096, 4, 64, torch.float16
+    assert N.load().dmf_mattn_fwd_ws_floats(N.dtype_code(dt), b, n, n, h, h, d, 0) == 0   # (no split of the keys)
+    q, k, v = torch.zeros(b, n, h, d), torch.zeros(b, n, h, d), torch.ones(b, n, h, d)
+    q[..., 0] = 1.0
+    k[:, 1:, :, 0] = tail
+    v[:, 0] = 0.0
+    q, k, v = (t.to(DEV).to(dt) for t in (q, k, v))
+    go = (1 + 0.5 * T._randn((b, n, h, d), torch.float32, 4)).mul(8).to(dt)
+    sl = torch.full((h,), 1e-9, device=DEV) if mode.get("slopes") else None
+    kw = dict(scale=1.0, softcap=mode.get("cap", 0.0), slopes=sl)
+    o, _, _, dv = _grads(q, k, v, go, **kw)
+    with torch.no_grad():
+        o2 = A.attention(q, k, v, **kw)
+    see, at = torch.ones(1, n, n, dtype=torch.bool), torch.arange(n)[None]
+    tiny = T._tiny
+    one = [t[:1, :, :1] for t in (q, k, v, go)]
+    try:
+        T._tiny = lambda dt: 2.0 ** -32
+        ref = T._attn_ref(*one[:3], see, at, 1.0, kw["softcap"], None if sl is None else sl[:1], one[3])
+        T._within(o[:1, :, :1], ref[0], ref[1] + 2.0 ** -25, "o")         # (2^-25: o's own rounding)
+        T._within(o2[:1, :, :1], ref[0], ref[1] + 2.0 ** -25, "o without a gradient")
+        T._tiny = lambda dt: 2.0 ** -40
+        ref = T._attn_ref(*one[:3], see, at, 1.0, kw["softcap"], None if sl is None else sl[:1], one[3])
+        T._within(dv[:1, :, :1], ref[6], ref[7] + 2.0 ** -25, "dv")
+    finally:
+        T._tiny = tiny
