@@ -16,6 +16,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 import dmf_native as N
@@ -47,6 +48,12 @@ def _heads(what, name, t, like=None):
             raise ValueError(f"{what}: {name} must be float32, bfloat16 or float16, got {t.dtype}")
     elif t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f"{what}: {name} is {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+
+
+def _no_tangents(what, *tensors):
+    """Forward-mode derivatives are refused: the kernels would drop the tangents."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: forward-mode derivatives are not supported")
 
 
 def _strided(t, align, apart=0):
@@ -202,6 +209,7 @@ def qk_norm_rope(q, k, cos=None, sin=None, positions=None, q_weight=None, k_weig
             positions = positions.contiguous()
     elif cos is not None and cos.shape[0] < n:
         raise ValueError(f"{what}: the table has {cos.shape[0]} rows for {n} tokens")
+    _no_tangents(what, q, k, q_weight, k_weight, cos, sin)
     if not (math.isfinite(eps) and eps >= 0):
         raise ValueError(f"{what}: eps {eps}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad
@@ -305,6 +313,7 @@ def attention(q, k, v, *, scale=None, softcap=0.0, slopes=None, causal=False, kv
         raise ValueError(f"{what}: a prefix needs causal=True")
     if slopes is not None and slopes.requires_grad:
         raise ValueError(f"{what}: no gradient reaches slopes")
+    _no_tangents(what, q, k, v, slopes)
     dev = q.device
     if slopes is not None:
         slopes = _small(what, "slopes", slopes, (hq,), torch.float32, dev)

@@ -287,3 +287,24 @@ def test_attention_f16_dominant_key_over_a_flat_tail(mode, tail):
         T._within(dv[:1, :, :1], ref[6], ref[7] + 2.0 ** -25, "dv")
     finally:
         T._tiny = tiny
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent would be dropped without a word: dual inputs raise, plain ones inside a dual level do not."""
+    from torch.autograd import forward_ad
+
+    q, k = (T._randn((1, 6, 2, 32), torch.float32, s) for s in (1, 2))
+    w = torch.ones(32, device=DEV)
+    cos, sin = A.rope_table(6, 32, device=DEV)
+    with forward_ad.dual_level():
+        want = A.attention(q, k, k), *A.qk_norm_rope(q, k, cos, sin, None, w, w)
+        dual = [forward_ad.make_dual(t, torch.ones_like(t)) for t in (q, w, cos)]
+        for args, kw in (((dual[0], k, k), {}), ((q, dual[0], k), {}), ((q, k, dual[0]), {}),
+                         ((q, k, k), dict(slopes=forward_ad.make_dual(w[:2].clone(), w[:2].clone())))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                A.attention(*args, **kw)
+        for args in ((dual[0], k, cos, sin, None, w, w), (q, dual[0], cos, sin, None, w, w), (q, k, cos, sin, None, dual[1], w),
+                     (q, k, cos, sin, None, w, dual[1]), (q, k, dual[2], sin, None, w, w)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                A.qk_norm_rope(*args)
+    assert torch.equal(want[0], A.attention(q, k, k))
