@@ -256,6 +256,10 @@ class AttnCore:
         self.cos, self.sin = rope if rope is not None else (None, None)
         self.softcap, self.slopes = float(softcap), slopes
 
+    def tensors(self):
+        """What the backward reads again: saved by the nodes, so that a change in place before it raises."""
+        return self.wq, self.wk, self.cos, self.sin, self.slopes
+
     def check(self, what, n, d, heads, dev):
         for name, t, shape in (("q_norm", self.wq, (d,)), ("k_norm", self.wk, (d,)), ("slopes", self.slopes, (heads,)),
                                ("the table's cos", self.cos, None), ("the table's sin", self.sin, None)):
@@ -439,8 +443,9 @@ class _BlockFn(torch.autograd.Function):
         # MLP branch: x2 = x1 + drop(fc2(drop(gelu(fc1(ln2(x1)))))) * g2
         ln2, save2 = ln_fwd(x1, ln2w, ln2b, eps2, cdt)
         x2, sm = _mlp_fwd(ln2, w1, fc1b, w2, fc2b, p_mlp, rng, s_m1, s_m2, g2, x1)
-        # (the norm weights too: the core reads them, saved they are checked for changes in place)
-        ctx.save_for_backward(x, ln1, save1, *sa, x1, ln2, save2, *sm, wq, wp, w1, w2, ln1w, ln2w, g1, g2, rng, qnw, knw)
+        # (and what the core reads again: saved, it is checked for changes in place)
+        ctx.save_for_backward(x, ln1, save1, *sa, x1, ln2, save2, *sm, wq, wp, w1, w2, ln1w, ln2w, g1, g2, rng,
+                              *(core.tensors() if core is not None else ()))
         ctx.cfg, ctx.core, ctx.na = cfg, core, len(sa)
         ctx.dims = (b, n, e)
         return x2.view(b, n, e)
@@ -450,7 +455,7 @@ class _BlockFn(torch.autograd.Function):
         t = ctx.saved_tensors
         (x, ln1, save1), sa, t = t[:3], t[3:3 + ctx.na], t[3 + ctx.na:]
         (x1, ln2, save2), sm = t[:3], t[3:6]
-        wq, wp, w1, w2, ln1w, ln2w, g1, g2, rng = t[6:-2]
+        wq, wp, w1, w2, ln1w, ln2w, g1, g2, rng = t[6:15]
         heads, eps1, eps2, p_attn, p_proj, p_mlp, sites, cdt, _ = ctx.cfg
         s_attn, s_proj, s_m1, s_m2 = sites
         b, n, e = ctx.dims
@@ -675,14 +680,14 @@ class _MHSAFn(torch.autograd.Function):
         wq, wp = _wcast(cdt, qkvw, projw)
         out, sa = _attn_fwd(a, wq, qkvb, wp, projb, b, n, heads, p_attn, p_proj, rng, sites[0], sites[1], core=core)
         ones = torch.ones(e, dtype=torch.float32, device=x.device)
-        ctx.save_for_backward(a, *sa, wq, wp, ones, rng, qnw, knw)
-        ctx.cfg, ctx.dims, ctx.xdtype, ctx.core = cfg, (b, n, e), x.dtype, core
+        ctx.save_for_backward(a, *sa, wq, wp, ones, rng, *(core.tensors() if core is not None else ()))
+        ctx.cfg, ctx.dims, ctx.xdtype, ctx.core, ctx.na = cfg, (b, n, e), x.dtype, core, len(sa)
         return out.view(b, n, e)
 
     @staticmethod
     def backward(ctx, dout):
         a, *rest = ctx.saved_tensors
-        sa, (wq, wp, ones, rng) = rest[:-6], rest[-6:-2]
+        sa, (wq, wp, ones, rng) = rest[:ctx.na], rest[ctx.na:ctx.na + 4]
         heads, p_attn, p_proj, sites, cdt = ctx.cfg
         b, n, e = ctx.dims
         need = ctx.needs_input_grad

@@ -196,7 +196,8 @@ class TransformerStage(nn.Module):
         if key not in self._rope:
             if torch.cuda.is_current_stream_capturing():  # (a table made in a capture is not filled before a replay)
                 raise RuntimeError(f"TransformerStage: run one step on a {hw[0]} x {hw[1]} grid before capturing it")
-            table = A.rope_table_2d(hw[0], hw[1], self._head_dim, device=device)
+            with torch.inference_mode(False):  # (a training step saves it for its backward)
+                table = A.rope_table_2d(hw[0], hw[1], self._head_dim, device=device)
             if table[0].is_cuda:  # (later steps may run on other streams)
                 torch.cuda.current_stream(table[0].device).synchronize()
             self._rope[key] = table

@@ -308,3 +308,28 @@ def test_forward_mode_derivatives_are_refused():
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 A.qk_norm_rope(*args)
     assert torch.equal(want[0], A.attention(q, k, k))
+
+
+def test_block_options_changed_before_the_backward_raise():
+    """Slopes and rotation tables changed in place between the forward and the backward raise, as norm weights do; a table that a
+    run under inference_mode made serves a training step."""
+    import test_gpu_attention_options as TO
+    import transformer_model as TM
+
+    x = torch.randn(1, 16, 256, device=DEV, requires_grad=True)
+    for what in ("slopes", "cos", "sin"):
+        blk = TO._block(TO.ALL, 3)
+        rope = A.rope_table_2d(4, 4, 64, device=DEV)
+        for m in (blk, blk.attn):
+            y = m(x, rope)
+            with torch.no_grad():
+                {"slopes": blk.attn.slopes, "cos": rope[0], "sin": rope[1]}[what].mul_(2.0)
+            with pytest.raises(RuntimeError, match="modified by an inplace"):
+                y.sum().backward()
+            m(x, rope).sum().backward()   # (and the changed values serve the next step)
+    st = TM.TransformerStage(8, 256, depth=1, heads=4, attention=TO.ALL).to(DEV)
+    im = torch.randn(2, 8, 16, 16, device=DEV)
+    with torch.inference_mode():
+        st.eval()(im)
+    st.train()(im).float().square().sum().backward()
+    assert all(torch.isfinite(p.grad).all() for p in st.parameters())
