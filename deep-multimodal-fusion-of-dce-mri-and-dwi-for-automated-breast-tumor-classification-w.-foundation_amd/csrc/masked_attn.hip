@@ -147,8 +147,10 @@ static int at_check(const char* who, AtArgs& a, int dtype) {
   DMF_CHECK_ARG(a.batch >= 0 && a.lq >= 0 && a.lk >= 0 && a.hk >= 1 && a.hq >= 1 && a.hq % a.hk == 0,
                 "%s: %d query heads must be a multiple of %d key heads", who, a.hq, a.hk);
   DMF_CHECK_ARG(a.d >= 8 && a.d <= 128 && a.d % 8 == 0, "%s: head dim %d must be a multiple of 8 up to 128", who, a.d);
-  DMF_CHECK_ARG(a.scale > 0.f && a.scale < INFINITY, "%s: scale %g must be positive", who, a.scale);
-  DMF_CHECK_ARG(a.cap >= 0.f && a.cap < INFINITY, "%s: softcap %g must be 0 (none) or positive", who, a.cap);
+  // (inside these the score's constants stay normal numbers of f32: scale / cap, its inverse square and a slope over the scale)
+  DMF_CHECK_ARG(a.scale >= 0x1p-60f && a.scale <= 0x1p60f, "%s: scale %g must be in 2^-60 .. 2^60", who, a.scale);
+  DMF_CHECK_ARG(a.cap == 0.f || (a.cap >= 0x1p-60f && a.cap <= 0x1p60f), "%s: softcap %g must be 0 (none) or in 2^-60 .. 2^60",
+                who, a.cap);
   DMF_CHECK_ARG(a.causal || !a.prefix, "%s: a prefix needs causal", who);
   const long long rows = (long long)a.lq * a.group, nbh = (long long)a.batch * a.hk;
   DMF_CHECK_ARG(rows * a.group < (1LL << 31) && nbh < (1LL << 31) && (rows + 127) / 128 + (a.lk + 127LL) / 128 < 65536,

@@ -307,8 +307,8 @@ def attention(q, k, v, *, scale=None, softcap=0.0, slopes=None, causal=False, kv
         raise ValueError(f"{what}: head dim {d} must be a multiple of 8 up to 128")
     scale = d ** -0.5 if scale is None else float(scale)
     softcap = float(softcap)
-    if not (0 < scale < math.inf) or not (0 <= softcap < math.inf):
-        raise ValueError(f"{what}: scale {scale} must be positive and softcap {softcap} positive or 0")
+    if not 2.0 ** -60 <= scale <= 2.0 ** 60 or not (softcap == 0 or 2.0 ** -60 <= softcap <= 2.0 ** 60):
+        raise ValueError(f"{what}: scale {scale} must be in 2^-60 .. 2^60 and softcap {softcap} too, or 0")
     if prefix is not None and not causal:
         raise ValueError(f"{what}: a prefix needs causal=True")
     if slopes is not None and slopes.requires_grad:

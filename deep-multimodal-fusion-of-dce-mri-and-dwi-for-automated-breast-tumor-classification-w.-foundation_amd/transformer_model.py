@@ -85,8 +85,8 @@ def attention_options(options):
         raise ValueError(f"attention options: {extra} unknown (known: {sorted(known)})")
     got = {**known, **options}
     got["softcap"] = float(got["softcap"])
-    if not 0.0 <= got["softcap"] < float("inf"):
-        raise ValueError(f"attention options: softcap {got['softcap']} must be positive or 0 (none)")
+    if not (got["softcap"] == 0.0 or 2.0 ** -60 <= got["softcap"] <= 2.0 ** 60):
+        raise ValueError(f"attention options: softcap {got['softcap']} must be 0 (none) or in 2^-60 .. 2^60")
     return got if any(got.values()) else None
 
 

@@ -697,8 +697,8 @@ int dmf_qk_norm_rope_bwd(int dtype, const void* q, long long q_sb, long long q_s
  *   p = kv_len - lq + i (the queries are the last lq of the kv_len tokens); kv_lens [batch] (null: lk) is clamped to
  *   [0, lk]. causal: j <= p, and the first prefix[b] keys (null: 0) are seen by all. spans [batch][lq][2]
  *   (dmf_mattn_spans) takes the place of causal / prefix. A query that sees nothing has o = 0; keys that a query does not see
- *   do not reach its output, whatever they hold. d a multiple of 8 up to 128, strides and bases multiples of 16 bytes,
- *   token strides at least d.
+ *   do not reach its output, whatever they hold. scale and softcap lie in 2^-60 .. 2^60 (or softcap 0). d a multiple of 8
+ *   up to 128, strides and bases multiples of 16 bytes, token strides at least d.
  *   For the backward: lse [batch][hq][lq] and, for 16-bit types alone, o_lo (what rounding o left over); null for
  *   inference.
  *   ws: dmf_mattn_fwd_ws_floats floats (ragged: kv_lens is given; 0: null allowed), where the keys are split over

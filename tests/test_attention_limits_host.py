@@ -26,3 +26,19 @@ def test_queries_heads_may_lie_far_apart():
         N.call("dmf_mattn_bwd", *_dims(**far), None, None, PTR, PTR, PTR, PTR, PTR, PTR, None)
     with pytest.raises(RuntimeError, match="2 GiB"):
         N.call("dmf_mattn_fwd", *_dims(q_sl=1 << 28), None, None, None, None, None)
+
+
+@pytest.mark.parametrize("kw,match", [(dict(cap=1e-25), "softcap"), (dict(cap=1e30), "softcap"), (dict(cap=1e-39), "softcap"),
+                                      (dict(scale=1e-30), "scale"), (dict(scale=1e30), "scale")])
+def test_scales_and_caps_past_the_range_of_their_constants(kw, match):
+    """1 / softcap^2, scale / softcap and a slope over the scale have to be numbers of f32."""
+    import transformer_model as TM
+    from test_attention_host import _dims
+
+    with pytest.raises(RuntimeError, match=match):
+        N.call("dmf_mattn_fwd", *_dims(**kw), None, None, None, None, None)
+    with pytest.raises(RuntimeError, match=match):
+        N.call("dmf_mattn_bwd", *_dims(**kw), None, None, PTR, PTR, PTR, PTR, PTR, PTR, None)
+    if "cap" in kw:
+        with pytest.raises(ValueError, match="softcap"):
+            TM.attention_options(dict(softcap=kw["cap"]))

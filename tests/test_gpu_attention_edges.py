@@ -333,3 +333,24 @@ def test_block_options_changed_before_the_backward_raise():
         st.eval()(im)
     st.train()(im).float().square().sum().backward()
     assert all(torch.isfinite(p.grad).all() for p in st.parameters())
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_attention_scales_and_caps_at_the_ends_of_their_range(dt):
+    """The smallest and largest scale and softcap that are taken, with slopes: finite outputs and gradients by the definition."""
+    b, n, h, d = 1, 70, 2, 32
+    q, k, v, go = (T._randn((b, n, h, d), dt, s) for s in (1, 2, 3, 4))
+    sl = torch.tensor([0.1, 0.02], device=DEV)
+    see, pos = T._see(b, n, n, True, None, None, None)
+    for scale, cap in ((2.0 ** -60, 0.0), (2.0 ** -60, 2.0 ** -60), (2.0 ** -60, 2.0 ** 60), (1.0, 2.0 ** -60), (2.0 ** 60, 2.0 ** -60),
+                       (2.0 ** 20, 5.0)):
+        got = _grads(q, k, v, go, scale=scale, softcap=cap, slopes=sl, causal=True)
+        ref = T._attn_ref(q, k, v, see, pos, scale, cap if cap < 1e9 else 0.0, sl, go)
+        T._within(got[0], ref[0], ref[1], f"o at {scale}, {cap}")
+        assert torch.isfinite(got[0]).all(), (scale, cap)
+        # (1 - tanh^2 errs by up to 16 e absolute, and dq and dk carry that times the scale: past 65504 an f16 one may be infinite)
+        assert all(torch.isfinite(t).all() for t in got[1:]) or (dt == torch.float16 and 16 * T.E * scale > 65504), (scale, cap)
+        assert torch.isfinite(got[3]).all(), (scale, cap)
+    for kw in (dict(softcap=1e-25), dict(softcap=1e30), dict(scale=1e-30), dict(scale=1e30)):
+        with pytest.raises(ValueError, match="attention"):
+            A.attention(q, k, v, **kw)
