@@ -82,14 +82,14 @@ __global__ void __launch_bounds__(1024) k_mattn_spans(const I* __restrict__ docs
 // The forward's launch, from sizes alone.
 //
 // Up to 32 rows per key head (single tokens): one-wave workgroups, the keys cut until about AT_FEW_BLOCKS of them run (five
-// fit a CU; 8 x 32 query heads over 65536 keys: 279 us with 4096, 254 with 8192, 266 with 16384).
+// fit a CU; 8 x 32 query heads over 65536 keys: 282 us with 4096, 256 with 8192, 268 with 16384).
 //
 // More rows: 4 row waves (3, with 32-key tiles, where short rows would leave one of four without work and half a key tile
-// empty: 257 x 257 tokens, 12 heads of 64, batch 32: 32 -> 28 us; and the grid holds that many row blocks). The keys are cut where that evens out the CUs: a CU's
+// empty: 257 x 257 tokens, 12 heads of 64, batch 32: 29 -> 27 us capped f16, 24 -> 21 bf16; and the grid holds that many row blocks). The keys are cut where that evens out the CUs: a CU's
 // n = ceil(workgroups / 256) run two at a time (an odd one out has the CU to itself, a third faster), each costs its key
 // tiles and about four tiles' time to start and end, and the cut costs the partials' traffic and a second launch (batch 2, 413
-// queries, 16 heads over 4, 32768 keys: 5 cuts 382 us, 7: 313, 9: 280, 12: 296). Ragged lengths leave whole cuts without
-// work, which two more even out (lengths 32768 and 8192: 9 cuts 280 us, 11: 242, 13: 239).
+// queries, 16 heads over 4, 32768 keys: 1 cut 798 us, 5: 408, 7: 306, 9: 294, 12: 298). Ragged lengths leave whole cuts without
+// work, which two more even out (lengths 32768 and 8192: 7 cuts 304 us, 9: 244, 11: 211, 13: 208).
 // f32 tiles take about four times as long, and two key groups share a workgroup's rows while workgroups are scarce.
 constexpr long long AT_FEW_BLOCKS = 8192, AT_CUS = 256;
 static AtPlan at_plan(int dtype, int batch, int lq, int lk, int hk, int group, int d, bool ragged) {
@@ -134,9 +134,11 @@ static AtPlan at_plan(int dtype, int batch, int lq, int lk, int hk, int group, i
 }
 
 // Workgroups of 4 waves with 64-key tiles run two on a CU, with 32-key tiles (half the LDS, at most 168 registers) three, at
-// 3 to 10 % more time for the same work. That pays where all are equally long (no mask) and three or five come to a CU, which
-// two at a time leave an odd one of: bf16, 128 dims, 576 tokens, 4 heads, batch 32 (640 workgroups): 43 -> 36 us; 64 (1280):
-// 74 -> 63; but 48 (960): 50 -> 57, 8 (160): 20 -> 22.
+// 3 to 10 % more time for the same work. (Those 168 registers are a few too few for 128 dims under a cap or with slopes for training,
+// which spill 12 to 24 bytes.) That pays where all are equally long (no mask) and three or five come to a CU, which two at a time
+// leave an odd one of: bf16, 128 dims, 576 tokens, 4 heads, batch 32 (640 workgroups): 43 -> 36 us, capped and for training 57 -> 55;
+// 64 (1280): 72 -> 62, 99 -> 95; but 48 (960): 50 -> 55, 74 -> 79; 8 (160): 18 -> 20, 25 -> 30. Seven and nine gain as well (88 rows: 97 ->
+// 91, 134 -> 133; 112: 125 -> 113, 173 -> 169) and are not taken yet.
 static bool at_three(const AtArgs& a) {
   const long long n = ((long long)a.batch * a.hk * (((long long)a.lq * a.group + 127) / 128) + AT_CUS - 1) / AT_CUS;
   return n == 3 || n == 5;

@@ -12,9 +12,10 @@
 // both (7 products for the 5 that one pass with dQ in atomics would take): no atomics, so the same bits every run, no
 // f32 dQ in HBM, and the sum over a group's query heads happens inside the dK / dV accumulators.
 //
-// Bound: matrix pipe, vector ALU and LDS reads within a fifth of each other (32 matrix instructions, about 250 vector ones and
-// 24 + 32 LDS reads a step of 32 x 32). 2 x 8192 tokens, 32 heads over 8 of 128, bf16: 6.9 ms, 1.11 PFLOP/s of the 7 products;
-// 32 x 576, 4 heads, capped: 132 us (0.58), of which a third is the workgroups' start and end.
+// Bound: no unit is full; a step of 32 x 32 has 32 matrix instructions, about 250 vector ones and 24 + 32 LDS reads one after the
+// other, and two waves a SIMD overlap them in part (busy, 32 x 576: matrix pipe 0.32, vector ALU 0.46, LDS 0.21; 8192 tokens in
+// documents: 0.35, 0.31, 0.25). 8192 tokens, 32 heads over 8 of 128, bf16: 3.46 to 3.52 ms, 1.09 to 1.11 PFLOP/s of the 7 products;
+// 32 x 576, 4 heads, capped: 127 to 134 us (0.58), of which a third is the workgroups' start and end.
 #pragma once
 #include "masked_attn.h"
 #include "masked_attn_fwd.h"
@@ -507,7 +508,7 @@ template <typename T, int DF, bool CAP, bool SLOPE, int NW, int KW>
 static int mattn_bwd_kw(AtArgs a, hipStream_t stream) {
   typedef AtBwdLds<T, DF, NW, KW> L;
   // Without a mask the kind with the longer walks starts first: 4 lq group / groups products of a tile for a key workgroup's
-  // waves against 3 lk for a row workgroup's (1187 tokens, 12 heads of 64: 54 -> 43 us). Under a mask the first keys do (an
+  // waves against 3 lk for a row workgroup's (1187 tokens, 12 heads of 64: 52 -> 41 us). Under a mask the first keys do (an
   // order by the longest walks left was measured: even for causal masks, 20 % slower for documents).
   a.rows_first = !a.causal && !a.spans && 3LL * a.lk * L::NG > 4LL * a.lq * a.group;
   const dim3 grid((unsigned)(a.batch * a.hk), (unsigned)(cdiv(a.lk, 32 * KW) + cdiv((long long)a.lq * a.group, 32 * NW)));
@@ -516,21 +517,21 @@ static int mattn_bwd_kw(AtArgs a, hipStream_t stream) {
   return 0;
 }
 // The workgroups, from sizes and the kind of mask (bf16, 128 dims unless said, the whole backward):
-//   4 waves, two workgroups a CU: their loads, barriers and stores fall apart in time and overlap. 32 x 576 tokens, 4 heads:
-//     138 -> 126 us against the next form; 32 x 257, 12 heads of 64: 100 -> 68; 8192 tokens, 4 heads: 570 -> 444.
+//   4 waves, two workgroups a CU: their loads, barriers and stores fall apart in time and overlap. 32 x 576 tokens, 4 heads, capped:
+//     135 -> 132 us against the next form; 32 x 257, 12 heads of 64: 92 -> 67.
 //   8 waves, two groups that share a key block's walk, one workgroup a CU: where a mask makes walks unequal and the longest
 //     one, which grows with the heads of a group, would end long after the others. 4096 causal tokens, 32 heads over 8 (256 key
-//     blocks): 484 us against 766 with 4 waves, 6144 (384): 1031 against 1238; with 512 key blocks the two meet (8192:
-//     1784 against 1800; 2 x 4096: 945 against 956) and then turn (3 x 4096: 1427 against 1421), and one head a group gains
-//     from 4 waves or comes out even. Documents turn later (16384 tokens in 12, 16 heads over 4, 512 blocks: 851 against 1236;
-//     32768 in 60, 1024 blocks: 795 against 707).
+//     blocks): 514 us against 791 with 4 waves, 6144 (384): 1094 against 1293; with 512 key blocks the two meet (8192:
+//     1895 against 1905) and then turn (3 x 4096: 1503 against 1476), and one head a group gains
+//     from 4 waves or comes out even. Documents turn later (16384 tokens in 12, 16 heads over 4, 512 blocks: 684 against 784;
+//     32768 in 60, 1024 blocks: 844 against 844).
 //   8 waves over 64 keys, four groups: while 128-key blocks would leave half of the 256 CUs without one: twice the workgroups
-//     with half the walk, for twice the loads a product. 2048 causal tokens, 32 heads over 8 (128 key blocks): 237 -> 163 us
-//     against the second form; at 4096 (256) 527 -> 547. f32, 64 dims: 2 x 1024 causal tokens, 16 heads over 4: 519 -> 276 us;
+//     with half the walk, for twice the loads a product. 2048 causal tokens, 32 heads over 8 (128 key blocks): 232 -> 158 us
+//     against the second form; at 4096 (256) 514 -> 524. f32, 64 dims: 2 x 1024 causal tokens, 16 heads over 4: 519 -> 276 us;
 //     4 x 329 tokens, 4 heads: 59.6 -> 54.8.
 //     Up to one block a CU under a document mask, whose longest document is the longest walk (8192 tokens, 16 heads over 4,
-//     second form -> this: 3 documents 461 -> 443, 12: 377 -> 264, 64: 112 -> 116; one of 8192: 961 -> 985), not beyond
-//     (4 x 4096 tokens, 8 documents each, 512 blocks: 349 -> 384).
+//     second form -> this: 3 documents 655 -> 543, 12: 333 -> 278, 64: 115 -> 121), not beyond
+//     (4 x 4096 tokens, 8 documents each, 512 blocks: 354 -> 389).
 constexpr int AT_FEW_KEY_BLOCKS = 128, AT_EVEN_KEY_BLOCKS = 512;
 template <typename T, int DF, bool CAP, bool SLOPE>
 static int mattn_bwd_df(const AtArgs& a, hipStream_t stream) {

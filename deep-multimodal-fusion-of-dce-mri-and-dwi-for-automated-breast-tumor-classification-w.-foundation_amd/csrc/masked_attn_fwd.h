@@ -14,10 +14,11 @@
 // Keys outside the union of the workgroup's spans are zero-filled on load; a value inside it that is not finite stays with the
 // rows that see it by a second walk (at_accumulate_seen).
 //
-// Bound: for many rows the vector ALU (exponential, maximum, cap) beside the matrix pipe, which both waves of a SIMD share:
-// 8192 x 8192 tokens, 32 heads over 8 of 128, bf16: 1.04 to 1.18 ms by the inputs' scale (0.93 to 1.06 PFLOP/s; a large matrix
-// product reaches 1.23), capped 1.24; short rows also start and end: 32 x 576, 4 heads, capped, with the rest: 58 us (0.56). For
-// single queries HBM: 8 rows of up to 65536 keys, 32 heads over 8: 249 us + 9 us of join (5.2 TB/s).
+// Bound: for many rows the order of a wave's own work, score product, cap and exponential, value product, which only the SIMD's other
+// wave overlaps: neither unit is full (vector ALU 0.6 and matrix pipe 0.4 busy under a cap, 0.5 and 0.4 without).
+// 8192 x 8192 tokens, 32 heads over 8 of 128, bf16: 1.03 to 1.08 ms by the inputs' scale (1.02 to 1.07 PFLOP/s; a large matrix
+// product reaches 1.2 to 1.3), capped 1.26 to 1.42, for training 1.42 to 1.48; short rows also start and end: 32 x 576, 4 heads, capped,
+// for training: 55 to 60 us. For single queries HBM: 8 rows of up to 65536 keys, 32 heads over 8: 249 us + 9 us of join (5.2 TB/s).
 #pragma once
 #include "masked_attn.h"
 

@@ -382,9 +382,9 @@ static int qk_check(const char* who, const QkArgs& a, int dtype, int batch) {
 }
 
 // heads per lane group: as many as leave 16384 groups (8 waves on each CU at 8 rows a wave), so that the cos / sin
-// loads are shared without leaving CUs idle; in the forward no more than the side with fewer heads has (or 8), so that
-// its groups do not end long before the others' (2 x 8192 tokens, 32 query and 8 key heads of 128, bf16: 32 heads a group
-// 78 us, 8: 67 to 73). The backward's groups take several tokens each and leave a weight-gradient partial per chunk of heads: there
+// loads are shared without leaving CUs idle; powers of two, in the forward up to the first that reaches the heads of the side
+// with fewer (or 8), so that its groups do not end long before the others' (2 x 8192 tokens, 32 query and 8 key heads of 128,
+// bf16: 32 heads a group 76 us, 16: 80, 8: 72, 4: 74). The backward's groups take several tokens each and leave a weight-gradient partial per chunk of heads: there
 // more chunks lose (the same sizes: 122 + 5 us for the partials' sum against 130 + 6).
 static void qk_split(QkArgs& a, long long tokens, bool even) {
   const int h0 = a.s[0].heads, h1 = a.s[1].heads, few = h0 < h1 ? h0 : h1;
