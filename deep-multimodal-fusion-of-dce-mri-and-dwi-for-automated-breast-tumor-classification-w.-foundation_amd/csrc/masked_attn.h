@@ -274,9 +274,10 @@ __device__ __forceinline__ void at_accumulate(const char* tile, const AtOffsets<
 // What a mask hides. A masked pair has weight 0 exactly, but 0 * NaN is NaN: in a tile that some row sees in part, an element
 // of X that is not finite reaches the columns that may not see its row. Where accumulators end up non-finite under a mask, a
 // workgroup therefore walks its tiles once more, and takes at_accumulate_seen in such tiles with such an element (at_has_nonfinite):
-// the same sum row by row on the vector ALU, over the pairs that sees(row) lets through. Finite inputs cost nothing but the check at
-// the end. 4096 causal tokens, 16 heads of 128, bf16, forward and backward: 142 + 262 us; with one key of NaN that all see
-// 266 + 887 (the second walk); with every operand NaN 595 + 2971 (each diagonal tile pair by pair).
+// the same sum row by row on the vector ALU, over the pairs that sees(row) lets through. Columns that are NaN in every dim by
+// what they see (a score of NaN, a delta of NaN) ask for no second walk. Finite inputs cost nothing but the check at the end. 4096 causal tokens, 16 heads of 128, bf16, forward and backward: 138 + 259 us; with one key of NaN that all see, or with
+// every operand NaN, the same; with all values NaN 603 + 854, with all output gradients infinite 133 + 2254 (each diagonal tile pair
+// by pair).
 template <typename T, int DF>
 __device__ __forceinline__ bool at_has_nonfinite(const char* tile, int r0, int lane) {
   constexpr int RB = AtOffsets<T, DF>::RB;
@@ -392,15 +393,20 @@ __device__ __forceinline__ int at_wave_min(int v) {
 }
 __device__ __forceinline__ int at_wave_max(int v) { return -at_wave_min(-v); }
 
-// lanes (of 32 columns) with an accumulator that is not finite
+// columns (lane & 31) for which either half wave's lane says yes
+__device__ __forceinline__ unsigned at_columns(bool yes) {
+  const unsigned long long m = __ballot(yes);
+  return (unsigned)m | (unsigned)(m >> 32);
+}
+// columns with an accumulator that is not finite
 template <int FD>
-__device__ __forceinline__ unsigned at_bad_columns(const at_f32x16* acc, float bad = 0.f) {
+__device__ __forceinline__ unsigned at_bad_columns(const at_f32x16* acc) {
+  float bad = 0.f;
 #pragma unroll
   for (int f = 0; f < FD; ++f)
 #pragma unroll
     for (int i = 0; i < 16; ++i) bad = fmaf(acc[f][i], 0.f, bad);
-  const unsigned long long m = __ballot(bad != bad);
-  return (unsigned)m | (unsigned)(m >> 32);
+  return at_columns(bad != bad);
 }
 // does any wave of the workgroup say yes? `flag` (LDS) is 0 from before the tiles' barriers on; every wave is done with its tiles
 // after this

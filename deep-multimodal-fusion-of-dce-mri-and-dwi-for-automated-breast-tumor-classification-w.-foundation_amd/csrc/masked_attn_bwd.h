@@ -296,7 +296,14 @@ __device__ __forceinline__ void at_bwd_keys(const AtArgs& a, int bh, int ktile, 
   walk(std::false_type{});
   const bool masked = a.causal || a.spans || a.kv_lens;
   if (masked || AT_FIT<T>) {
-    const bool bad = at_bad_columns<FD>(dk) != 0 || (masked && at_bad_columns<FD>(dv) != 0);
+    bool bad = at_bad_columns<FD>(dk) != 0 || (masked && at_bad_columns<FD>(dv) != 0);
+    if (bad) {  // (a row that sees all of the wave's keys and whose lse is NaN makes both sums NaN in every dim)
+      bool nan = false;
+      for (int i = q0 + lane; i <= q1; i += 64)
+        if (w_lo[i] <= kw0 && w_hi[i] >= kw0 + 32)
+          for (int n = 0; n < a.group; ++n) nan |= a.lse[rv0 + (long long)n * a.lq + i] != a.lse[rv0 + (long long)n * a.lq + i];
+      bad = !__any(nan);
+    }
     if (__builtin_expect(at_vote(bad, range + 16), 0)) {  // (unlikely: its spills stay out of the first walk)
 #pragma unroll
       for (int f = 0; f < FD; ++f) dk[f] = at_zero(), dv[f] = at_zero();
@@ -473,7 +480,8 @@ __device__ __forceinline__ void at_bwd_rows(const AtArgs& a, int bh, int tile, c
   };
   walk(std::false_type{});
   if (a.causal || a.spans || AT_FIT<T>) {
-    if (__builtin_expect(at_vote(at_bad_columns<FD>(dq) != 0, range + 16), 0)) {
+    const bool bad = (at_bad_columns<FD>(dq) & ~at_columns(!live || lse != lse || nd != nd)) != 0;
+    if (__builtin_expect(at_vote(bad, range + 16), 0)) {
 #pragma unroll
       for (int f = 0; f < FD; ++f) dq[f] = at_zero();
       if (nt > 0) issue(0, k_lo);

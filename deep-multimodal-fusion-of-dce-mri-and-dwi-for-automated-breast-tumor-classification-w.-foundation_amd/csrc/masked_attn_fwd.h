@@ -307,7 +307,8 @@ __global__ void __launch_bounds__(64 * NW * NG, at_fwd_waves<T>(DF, CAP, NW, KT)
   };
   walk(std::false_type{});
   if (a.causal || a.spans) {
-    const bool bad = at_bad_columns<FD>(acc, (l + lx) * 0.f) != 0;
+    // (a row whose sum is NaN saw a score of NaN)
+    const bool bad = (at_bad_columns<FD>(acc) & ~at_columns(!live || (l + lx) != (l + lx))) != 0;
     if (at_vote(bad, &again_flag)) {
       m = -INFINITY, ms = l = lx = 0.f;
 #pragma unroll

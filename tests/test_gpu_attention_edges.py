@@ -354,3 +354,35 @@ def test_attention_scales_and_caps_at_the_ends_of_their_range(dt):
     for kw in (dict(softcap=1e-25), dict(softcap=1e30), dict(scale=1e-30), dict(scale=1e30)):
         with pytest.raises(ValueError, match="attention"):
             A.attention(q, k, v, **kw)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("lq,lk,d", [(2, 70, 128), (3, 3000, 64), (9, 3000, 128), (32, 200, 96), (100, 3000, 32), (257, 257, 64)])
+def test_attention_every_launch_form_hides_the_future(lq, lk, d, dt):
+    """Few and many queries, split keys and three row waves: what the last key holds reaches the last query alone."""
+    hq, hk = 4, 2
+    q, k, v, go = (T._randn((2, n, h, d), dt, s) for n, h, s in ((lq, hq, 1), (lk, hk, 2), (lk, hk, 3), (lq, hq, 4)))
+    see, at = T._see(2, lq, lk, True, None, None, None)
+    ref = T._attn_ref(q, k, v, see, at, d ** -0.5, 0.0, None, go)
+    k[:, -1, :, 2], v[:, -1, :, 1] = float("nan"), -float("inf")
+    with torch.no_grad():
+        o2 = A.attention(q, k, v, causal=True)
+    o, dq, _, _ = _grads(q, k, v, go, causal=True)
+    for got in (o, o2):
+        T._within(got[:, :-1], ref[0][:, :-1], ref[1][:, :-1], "o")
+        assert torch.isnan(got[:, -1]).all()
+    T._within(dq[:, :-1], ref[2][:, :-1], ref[3][:, :-1], "dq")
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_attention_keys_behind_the_length_have_no_gradient(dt):
+    """An output gradient that is not a number reaches the keys in use and none behind them, under key lengths alone."""
+    b, n, lk, h, d = 3, 90, 140, 2, 64
+    q, k, v, go = (T._randn((b, m, h, d), dt, s) for m, s in ((n, 1), (lk, 2), (lk, 3), (n, 4)))
+    lens = [100, 140, 0]
+    go[:, 7] = float("nan")
+    _, dq, dk, dv = _grads(q, k, v, go, kv_lens=torch.tensor(lens, dtype=torch.int32, device=DEV))
+    for i, m in enumerate(lens):
+        assert torch.isnan(dk[i, :m]).all() and torch.isnan(dv[i, :m]).all()
+        assert not dk[i, m:].any() and not dv[i, m:].any()
+    assert torch.isfinite(dq[:, 8:]).all() and torch.isnan(dq[:2, 7]).all() and not dq[2].any()
