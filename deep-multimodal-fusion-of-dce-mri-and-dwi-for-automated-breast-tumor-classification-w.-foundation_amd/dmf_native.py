@@ -142,9 +142,13 @@ class BnDesc(ctypes.Structure):
 
 
 def stream_ptr(device=None):
-    """hipStream_t of torch's current stream (graph-capture aware); of ``device``, an index, a torch.device or None
-    for the current one."""
+    """hipStream_t of torch's current stream (graph-capture aware); of ``device``, an index, a torch.device, its name or
+    None for the current one."""
+    if isinstance(device, str):
+        device = torch.device(device)
     if isinstance(device, torch.device):
+        if device.type != "cuda":
+            raise ValueError(f"stream_ptr: {device} has no stream")
         device = device.index
     if device is None:
         device = torch.cuda.current_device()

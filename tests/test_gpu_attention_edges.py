@@ -386,3 +386,16 @@ def test_attention_keys_behind_the_length_have_no_gradient(dt):
         assert torch.isnan(dk[i, :m]).all() and torch.isnan(dv[i, :m]).all()
         assert not dk[i, m:].any() and not dv[i, m:].any()
     assert torch.isfinite(dq[:, 8:]).all() and torch.isnan(dq[:2, 7]).all() and not dq[2].any()
+
+
+def test_stream_ptr_takes_what_torch_takes():
+    """An index, a torch.device, a device's name or nothing name the same current stream, a side stream too."""
+    import dmf_native as N
+
+    for s in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(s):
+            for d in (None, 0, "cuda", "cuda:0", torch.device("cuda"), torch.device("cuda", 0)):
+                assert N.stream_ptr(d) == s.cuda_stream, d
+    for d in ("cpu", torch.device("cpu")):
+        with pytest.raises(ValueError):
+            N.stream_ptr(d)
