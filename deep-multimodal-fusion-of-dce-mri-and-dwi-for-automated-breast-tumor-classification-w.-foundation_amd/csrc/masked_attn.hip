@@ -135,7 +135,7 @@ static AtPlan at_plan(int dtype, int batch, int lq, int lk, int hk, int group, i
 
 // Workgroups of 4 waves with 64-key tiles run two on a CU, with 32-key tiles (half the LDS, at most 168 registers) three, at
 // 3 to 10 % more time for the same work. (Those 168 registers are a few too few for 128 dims under a cap or with slopes for training,
-// which spill 12 to 24 bytes.) That pays where all are equally long (no mask) and three or five come to a CU, which two at a time
+// which spill 12 to 24 bytes in the first walk.) That pays where all are equally long (no mask) and three or five come to a CU, which two at a time
 // leave an odd one of: bf16, 128 dims, 576 tokens, 4 heads, batch 32 (640 workgroups): 43 -> 36 us, capped and for training 57 -> 55;
 // 64 (1280): 72 -> 62, 99 -> 95; but 48 (960): 50 -> 55, 74 -> 79; 8 (160): 18 -> 20, 25 -> 30. Seven and nine gain as well (88 rows: 97 ->
 // 91, 134 -> 133; 112: 125 -> 113, 173 -> 169) and are not taken yet.
